@@ -513,6 +513,73 @@ IEX_API int iex_graph_dump(void* graph, const char* path);
 IEX_API int iex_graph_add_child(void* graph, void* child);
 IEX_API void* iex_graph_combine(void* const* graphs, int count);
 
+/* ------------------------------------------------------------------------------------
+ * Paged key-value cache of a decoding program: appending to it, attention of new tokens
+ * over it, and choosing the pages that such attention reads.  No counterpart in the
+ * reference; it stands beside iex_attention_f32 and serves layers whose projections are
+ * the sparse and dense linears above.
+ *
+ *   k_cache, v_cache   [num_pages, kv_heads, page_size, head_dim]; a page's part is
+ *                      contiguous, pages are k_page / v_page elements apart
+ *   block_table        int32 [rows, table_width]: the pages of each sequence, in order
+ *   lengths            int32 [rows]: positions held (the new tokens included)
+ *   bf16               0: IEEE binary16 throughout, 1: bfloat16 throughout
+ *   head_dim           a multiple of 8 up to 128; page_size 16, 32, 64, 128 or 256
+ * Rows of q, k and v are x_row, their heads x_head elements apart (multiples of 8, base
+ * addresses on 16 bytes), elements of a head contiguous; other outputs are contiguous.
+ * Lengths and tables come from the device and are bounded there: a length is read as one
+ * between 0 and table_width * page_size, positions on a page outside [0, num_pages) as not
+ * held.  Nothing behind a row's length is read, whatever its bits.
+ * ------------------------------------------------------------------------------------ */
+
+/* Appends: sequence i has cu_tokens[i + 1] - cu_tokens[i] new tokens (int32, ascending from
+ * 0; NULL: one each, tokens == batch), consecutive rows of q, k and v, at the last positions below lengths[i].
+ * The first `rotary` elements (even) of every query and key are turned in pairs, (a, b) ->
+ * (a cos - b sin, b cos + a sin) with cos / sin fp32 [rope_rows, rotary / 2] at the token's
+ * position; pairs are (i, i + rotary / 2), or (2 i, 2 i + 1) if `interleaved`.
+ * q_out [tokens, heads, head_dim] gets the turned queries; rows of no sequence, and tokens
+ * without a place (position below 0 or behind the table or the angles, page not of the cache), are zero
+ * there and leave the cache as it is.
+ * boxes (or NULL) [num_pages, kv_heads, 2, head_dim]: smallest and largest key of a page in
+ * each dimension, begun anew by the token at a page's first position, else joined with what is there.
+ * A page that is written to belongs to one sequence of the call. */
+IEX_API int iex_paged_append(int tokens, int batch, int heads, int kv_heads, int head_dim, int bf16,
+                             const void* q, long long q_row, long long q_head, const void* k,
+                             long long k_row, long long k_head, const void* v, long long v_row,
+                             long long v_head, const float* cos, const float* sin, int rope_rows,
+                             int rotary, int interleaved, void* q_out, void* k_cache,
+                             long long k_page, void* v_cache, long long v_page, void* boxes,
+                             int num_pages, int page_size, const int32_t* block_table,
+                             int table_width, const int32_t* lengths, const int32_t* cu_tokens,
+                             void* stream);
+
+/* out[r, h] = sum_t softmax_t(scale * q[r, h] . k[t]) v[t] over the positions that row r
+ * holds; zero where there are none (or every score is -inf).  heads / kv_heads query heads share a key head.
+ * pages (or NULL) int32 [rows, kv_heads, count]: only the pages with these places in the row
+ * of the table, the first min(count, pages held) entries; entries that are no held page are
+ * skipped, one that is there twice counts twice. */
+IEX_API int iex_paged_attention_supported(int heads, int kv_heads, int head_dim, int page_size);
+IEX_API size_t iex_paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim);
+IEX_API int iex_paged_attention(int rows, int heads, int kv_heads, int head_dim, int bf16,
+                                const void* q, long long q_row, long long q_head,
+                                const void* k_cache, long long k_page, const void* v_cache,
+                                long long v_page, int num_pages, int page_size,
+                                const int32_t* block_table, int table_width, const int32_t* lengths,
+                                const int32_t* pages, int count, float scale, void* out,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/* pages [rows, kv_heads, count]: the pages of each row and key head with the largest
+ * sum over its query heads of sum_d max(q[d] lo[d], q[d] hi[d]), lo and hi from boxes, the
+ * `first` first and `last` last held pages always among them (first + last <= count); in
+ * ascending order, -1 behind them.  Ties go to the lower page, NaN is above all, pages not of the cache
+ * come last.  At most iex_paged_select_max_pages() columns of the table. */
+IEX_API int iex_paged_select_max_pages(void);
+IEX_API int iex_paged_select(int rows, int heads, int kv_heads, int head_dim, int bf16,
+                             const void* q, long long q_row, long long q_head, const void* boxes,
+                             int num_pages, int page_size, const int32_t* block_table,
+                             int table_width, const int32_t* lengths, int count, int first,
+                             int last, int32_t* pages, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

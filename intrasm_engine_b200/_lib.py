@@ -146,6 +146,22 @@ SIGNATURES = {
     "iex_csr_to_dense_f16": (c_int, [c_int, c_int, c_ptr, c_ptr, c_int, c_ptr, c_ptr, c_ptr]),
     # m k nnz row_offsets cols index_bits row_indices require_ascending result stream
     "iex_csr_validate": (c_int, [c_int, c_int, c_int, c_ptr, c_ptr, c_int, c_ptr, c_int, c_ptr, c_ptr]),
+    # tokens batch heads kv_heads dim bf16 q+strides k+strides v+strides cos sin rope_rows rotary interleaved q_out k_cache
+    # k_page v_cache v_page boxes num_pages page_size table table_width lengths cu_tokens stream
+    "iex_paged_append": (c_int, [c_int] * 6 + [c_ptr, c_ll, c_ll] * 3 + [c_ptr, c_ptr, c_int, c_int, c_int, c_ptr, c_ptr,
+                                 c_ll, c_ptr, c_ll, c_ptr, c_int, c_int, c_ptr, c_int, c_ptr, c_ptr, c_ptr]),
+    # heads kv_heads dim page_size
+    "iex_paged_attention_supported": (c_int, [c_int, c_int, c_int, c_int]),
+    # rows heads kv_heads dim
+    "iex_paged_attention_workspace_bytes": (c_size, [c_int, c_int, c_int, c_int]),
+    # rows heads kv_heads dim bf16 q+strides k_cache k_page v_cache v_page num_pages page_size table table_width lengths
+    # pages count scale out workspace workspace_bytes stream
+    "iex_paged_attention": (c_int, [c_int] * 5 + [c_ptr, c_ll, c_ll, c_ptr, c_ll, c_ptr, c_ll, c_int, c_int, c_ptr, c_int,
+                                    c_ptr, c_ptr, c_int, ctypes.c_float, c_ptr, c_ptr, c_size, c_ptr]),
+    "iex_paged_select_max_pages": (c_int, []),
+    # rows heads kv_heads dim bf16 q+strides boxes num_pages page_size table table_width lengths count first last pages stream
+    "iex_paged_select": (c_int, [c_int] * 5 + [c_ptr, c_ll, c_ll, c_ptr, c_int, c_int, c_ptr, c_int, c_ptr, c_int, c_int,
+                                 c_int, c_ptr, c_ptr]),
     "iex_stream_is_capturing": (c_int, [c_ptr]),
     "iex_last_device_status": (c_int, [c_int]),
     # graph constructor (opaque handle first)

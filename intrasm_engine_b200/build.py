@@ -25,7 +25,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 OBJ_DIR = os.path.join(REPO_DIR, "build", "iex_b200")
 LIB_PATH = os.path.join(PKG_DIR, "libiex_b200.so")
 EXT_DIR = os.path.join(PKG_DIR, "torch_ext")
-EXT_SRCS = [os.path.join(EXT_DIR, f) for f in ("iex_torch_ext.cpp", "iex_autograd.cpp")]
+EXT_SRCS = [os.path.join(EXT_DIR, f) for f in ("iex_torch_ext.cpp", "iex_autograd.cpp", "iex_paged.cpp")]
 EXT_PATH = os.path.join(PKG_DIR, "libiex_torch_ext.so")
 
 NVCC_FLAGS = [

@@ -1,0 +1,53 @@
+// What the kernels of the paged key-value cache share (paged_append.cu, paged_attention.cu, paged_select.cu).
+//
+// The cache: keys and values [pages, kv_heads, page_size, head_dim], one contiguous slab per page and head, pages at any
+// distance.  Row r of the block table names the pages of a sequence in order, lengths[r] says how many positions it holds.
+// Both come from the device and are not trusted: a length is read as one between 0 and what the row of the table can hold, and
+// positions of a page that is not one of the cache's are as if they were not held.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+namespace iex {
+namespace paged {
+
+constexpr int kMaxHeadDim = 128;
+constexpr int kMinPage = 16, kMaxPage = 256;
+
+inline bool page_size_ok(int page_size) {
+  return page_size >= kMinPage && page_size <= kMaxPage && (page_size & (page_size - 1)) == 0;
+}
+inline bool heads_ok(int heads, int kv_heads, int head_dim) {
+  return kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && head_dim > 0 && head_dim % 8 == 0 && head_dim <= kMaxHeadDim;
+}
+inline int log2_of(int power_of_two) {
+  int bits = 0;
+  while ((1 << bits) < power_of_two) ++bits;
+  return bits;
+}
+
+// Positions that row `row` holds.
+__device__ __forceinline__ int held(const int32_t* lengths, int row, int table_width, int page_shift) {
+  const long long most = static_cast<long long>(table_width) << page_shift;
+  const int length = lengths[row];
+  return length <= 0 ? 0 : static_cast<int>(length < most ? length : most);
+}
+
+// A matrix of rows and heads whose innermost dimension is contiguous, in elements.
+struct Rows {
+  const void* data;
+  long long row, head;
+};
+
+__device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T rounded(float v);
+template <>
+__device__ __forceinline__ __half rounded<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+}  // namespace paged
+}  // namespace iex

@@ -26,6 +26,13 @@ module only loads it.  Operators:
   spmm_plan(row_offsets, column_indices, m, k)                  pattern-only plan (build once)
   spmm_tc_planned(b, values, plan, m)                           SpMM on tensor cores (fp32),
                                                                 A [m, k] x b [k, n] -> [m, n]
+  paged_append(q, k, v, k_cache!, v_cache!, block_table, lengths, cu_tokens, cos, sin, interleaved, boxes!)
+                                                                new keys and values into a paged cache, rotated;
+                                                                the rotated q
+  paged_attention(q, k_cache, v_cache, block_table, lengths, pages, scale)
+                                                                new tokens' attention over a paged cache
+  paged_select(q, boxes, block_table, lengths, page_size, count, first, last)
+                                                                the pages each query attends to, by a cheap score
 With ``IEX_VALIDATE_CSR=1`` in the environment every sparse operator runs that check on its
 arguments first and raises on a malformed matrix (debugging aid; one extra kernel and a
 synchronisation per call).
@@ -79,4 +86,7 @@ OP_NAMES = (
     "sddmm_tc_planned",
     "spmm_plan",
     "spmm_tc_planned",
+    "paged_append",
+    "paged_attention",
+    "paged_select",
 )

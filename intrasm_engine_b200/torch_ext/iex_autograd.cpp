@@ -630,6 +630,31 @@ at::Tensor relu_down_proj(const at::Tensor& hidden, const at::Tensor& weight) {
   return out;
 }
 
+// Operators of the paged cache; nothing for calls that have to go through the dispatcher.
+using MaybeTensor = std::optional<at::Tensor>;
+std::optional<at::Tensor> native_paged_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                              const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& table,
+                                              const at::Tensor& lengths, const MaybeTensor& cu_tokens, const MaybeTensor& cos,
+                                              const MaybeTensor& sin, bool interleaved, const MaybeTensor& boxes) {
+  if (!q.is_cuda() || !plain({&q, &k, &v, &k_cache, &v_cache, &table, &lengths})) return std::nullopt;
+  for (const MaybeTensor* t : {&cu_tokens, &cos, &sin, &boxes})
+    if (t->has_value() && !plain({&**t})) return std::nullopt;
+  return paged_append(q, k, v, k_cache, v_cache, table, lengths, cu_tokens, cos, sin, interleaved, boxes);
+}
+std::optional<at::Tensor> native_paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                                 const at::Tensor& table, const at::Tensor& lengths, const MaybeTensor& pages,
+                                                 std::optional<double> scale) {
+  if (!q.is_cuda() || !plain({&q, &k_cache, &v_cache, &table, &lengths}) || (pages.has_value() && !plain({&*pages})))
+    return std::nullopt;
+  return paged_attention(q, k_cache, v_cache, table, lengths, pages, scale);
+}
+std::optional<at::Tensor> native_paged_select(const at::Tensor& q, const at::Tensor& boxes, const at::Tensor& table,
+                                              const at::Tensor& lengths, int64_t page_size, int64_t count, int64_t first,
+                                              int64_t last) {
+  if (!q.is_cuda() || !plain({&q, &boxes, &table, &lengths})) return std::nullopt;
+  return paged_select(q, boxes, table, lengths, page_size, count, first, last);
+}
+
 }  // namespace
 }  // namespace iex_torch
 
@@ -659,5 +684,8 @@ PYBIND11_MODULE(iex_torch_ext, mod) {
   mod.def("attention", &iex_torch::attention);
   mod.def("ffn_down", &iex_torch::ffn_down);
   mod.def("relu_down_proj", &iex_torch::relu_down_proj);
+  mod.def("paged_append", &iex_torch::native_paged_append);
+  mod.def("paged_attention", &iex_torch::native_paged_attention);
+  mod.def("paged_select", &iex_torch::native_paged_select);
   mod.def("fused_spmm_linear_half", &iex_torch::fused_spmm_linear_half);
 }

@@ -6,6 +6,7 @@
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <optional>
 #include <tuple>
 
 #include "iex_b200.h"
@@ -54,6 +55,16 @@ at::Tensor linear_fp16_wgrad(const at::Tensor& grad, const at::Tensor& input);
 std::tuple<at::Tensor, at::Tensor> fused_spmm_linear_half(const at::Tensor& x, const at::Tensor& row_offsets,
                                                           const at::Tensor& values, const at::Tensor& column_indices,
                                                           int64_t m, const at::Tensor& weight);
+// Operators of the paged key-value cache (iex_paged.cpp)
+at::Tensor paged_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache,
+                        const at::Tensor& v_cache, const at::Tensor& block_table, const at::Tensor& lengths,
+                        const std::optional<at::Tensor>& cu_tokens, const std::optional<at::Tensor>& cos,
+                        const std::optional<at::Tensor>& sin, bool interleaved, const std::optional<at::Tensor>& boxes);
+at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                           const at::Tensor& block_table, const at::Tensor& lengths, const std::optional<at::Tensor>& pages,
+                           std::optional<double> scale);
+at::Tensor paged_select(const at::Tensor& q, const at::Tensor& boxes, const at::Tensor& block_table, const at::Tensor& lengths,
+                        int64_t page_size, int64_t count, int64_t first, int64_t last);
 // With IEX_VALIDATE_CSR=1: device-side check of a CSR argument before it is used.
 void maybe_validate(const at::Tensor& row_offsets, const at::Tensor& column_indices, int64_t m, int64_t k,
                     const at::Tensor* row_indices, bool require_ascending);

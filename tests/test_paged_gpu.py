@@ -1,0 +1,600 @@
+"""GPU: the paged cache's operators against their definitions in 64 bits (paged_util.py)."""
+import pytest
+import torch
+
+from intrasm_engine_b200.pytorch import paged_attention as paged
+
+from . import paged_util as U
+from .paged_util import DEV
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def ints(values):
+    return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+
+def case(lengths, heads, kv_heads, dim, page, dtype, seed=0, std=1.0, **kwargs):
+    gen = torch.Generator().manual_seed(seed)
+    k, v, table = U.make_cache(gen, lengths, kv_heads, dim, page, dtype, **kwargs)
+    q = (torch.randn(len(lengths), heads, dim, generator=gen) * std).to(dtype).to(DEV)
+    return q, k, v, table, ints(lengths)
+
+
+# ------------------------------------------------------------------------------------------------- attention
+
+SHAPES = [
+    # lengths, heads, kv_heads, dim, page
+    ([1], 1, 1, 8, 16),
+    ([0, 1, 2, 15, 16, 17, 0, 31, 33], 4, 2, 64, 16),
+    ([63, 64, 65, 127, 128, 129, 0], 8, 1, 128, 64),
+    ([500], 32, 32, 128, 64),
+    ([1003, 1, 700, 0, 333], 6, 6, 80, 16),
+    ([257, 4096, 5], 10, 2, 96, 256),
+    ([3000, 40], 16, 1, 128, 32),
+    ([100, 2000, 31], 24, 1, 64, 128),
+    ([777], 33, 1, 40, 16),
+    ([0, 0, 0], 2, 2, 32, 16),
+    ([50] * 70, 12, 4, 64, 32),
+    ([9000, 10], 4, 4, 128, 64),
+    ([200, 900], 5, 1, 104, 64),
+    ([1500], 48, 2, 120, 64),
+]
+
+
+@pytest.mark.parametrize("dtype", U.DTYPES)
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim,page", SHAPES)
+def test_attention(lengths, heads, kv_heads, dim, page, dtype):
+    # what nobody holds is NaN, entries of the table behind a row's pages lie outside the cache
+    q, k, v, table, held = case(lengths, heads, kv_heads, dim, page, dtype)
+    got = paged.paged_attention(q, k, v, table, held)
+    assert got.shape == q.shape and got.dtype == dtype and got.is_contiguous()
+    U.check_attention(got, q, k, v, table, lengths)
+    for i, n in enumerate(lengths):
+        if n == 0:
+            assert not got[i].any()
+
+
+@pytest.mark.parametrize("dtype", U.DTYPES)
+def test_attention_of_large_and_small_scores(dtype):
+    for seed, std in enumerate((0.0, 0.01, 8.0, 40.0)):
+        q, k, v, table, held = case([700, 90], 8, 2, 64, 32, dtype, seed=seed, std=std)
+        U.check_attention(paged.paged_attention(q, k, v, table, held), q, k, v, table, [700, 90])
+    for scale in (0.0, -0.3, 2.5):
+        got = paged.paged_attention(q, k, v, table, held, scale=scale)
+        U.check_attention(got, q, k, v, table, [700, 90], scale=scale)
+
+
+@pytest.mark.parametrize("dtype", U.DTYPES)
+def test_attention_follows_a_rising_maximum(dtype):
+    """Scores that grow with the position, and ones that fall: the running maximum changes all the time, or never."""
+    for sign in (1.0, -1.0):
+        q, k, v, table, held = case([2500], 4, 1, 64, 64, dtype)
+        q.fill_(0.0)
+        q[..., 0] = sign
+        for j in range((2500 + 63) // 64):
+            k[int(table[0, j]), 0, :, 0] = (torch.arange(64, device=DEV) + 64 * j).to(dtype) * 0.25
+        U.check_attention(paged.paged_attention(q, k, v, table, held), q, k, v, table, [2500])
+
+
+def test_what_is_not_finite_reaches_the_rows_that_hold_it():
+    lengths = [300, 200, 64]
+    q, k, v, table, held = case(lengths, 4, 2, 64, 32, F16)
+    k[int(table[0, 3]), 1, 7, 5] = float("nan")   # row 0, key head 1
+    v[int(table[1, 2]), 0, 3, 9] = float("inf")   # row 1, key head 0, one element
+    q[2, 3, 0] = float("nan")
+    got = paged.paged_attention(q, k, v, table, held)
+    clean = torch.isfinite(got)
+    assert not clean[0, 2:].any() and clean[0, :2].all()
+    assert clean[1, 2:].all() and (got[1, :2, 9] == float("inf")).all() and clean[1, :2].sum() == 2 * 63
+    assert clean[2, :3].all() and not clean[2, 3].any()
+
+
+def test_scores_of_minus_infinity_weigh_nothing():
+    q, k, v, table, held = case([150, 40], 2, 1, 64, 16, BF16)
+    q.fill_(1.0)
+    for j in range(1, 10):  # all of row 0 behind its first page
+        k[int(table[0, j]), 0, :, 3] = float("-inf")
+    for j in range(3):      # all of row 1
+        k[int(table[1, j]), 0, :, 3] = float("-inf")
+    got = paged.paged_attention(q, k, v, table, held)
+    U.check_attention(got, q, k, v, table, [16, 0])
+
+
+def test_the_lowest_values_of_the_type_are_scores_like_others():
+    for dtype in U.DTYPES:
+        q, k, v, table, held = case([150], 2, 1, 64, 16, dtype)
+        q.fill_(0.0)
+        q[..., 0] = 1.0
+        k[..., 0] = 0.0
+        k[int(table[0, 2]), 0, 5:, 0] = torch.finfo(dtype).min
+        U.check_attention(paged.paged_attention(q, k, v, table, held, scale=1.0), q, k, v, table, [150], scale=1.0)
+
+
+def test_lengths_and_tables_are_bounded_by_the_kernel():
+    lengths = [100, 64, 30, 10]
+    q, k, v, table, held = case(lengths, 4, 2, 64, 16, F16)
+    # longer than the table: as long as the table; the entries of row 1 behind its 4 pages are not the cache's
+    wild = [2 ** 31 - 1, 2 ** 31 - 1, -5, 10]
+    got = paged.paged_attention(q, k, v, table, ints(wild))
+    U.check_attention(got, q, k, v, table, wild)
+    assert torch.isnan(got[0]).all() and not torch.isnan(got[1:]).any() and not got[2].any()
+    holes = table.clone()
+    holes[0, 2], holes[1, 0], holes[2, :] = -1, k.size(0), -2 ** 31
+    got = paged.paged_attention(q, k, v, holes, held)
+    U.check_attention(got, q, k, v, holes, lengths)
+    assert not got[2].any()
+    assert not paged.paged_attention(q, k[:0], v[:0], table, held).any()
+    assert not paged.paged_attention(q, k, v, table[:, :0].contiguous(), held).any()
+    assert paged.paged_attention(q[:0], k, v, table[:0], held[:0]).shape == (0, 4, 64)
+
+
+def test_rows_of_q_and_pages_of_the_cache_at_other_distances():
+    lengths, dim = [130, 77, 500], 64
+    q, k, v, table, held = case(lengths, 8, 2, dim, 32, F16)
+    ref = paged.paged_attention(q, k, v, table, held)
+    fused = torch.randn(3, 8 * dim + 128, device=DEV).half()
+    fused[:, 64:64 + 8 * dim] = q.reshape(3, -1)
+    view = fused[:, 64:64 + 8 * dim].view(3, 8, dim)
+    assert not view.is_contiguous() and torch.equal(paged.paged_attention(view, k, v, table, held), ref)
+    odd = torch.zeros(3, 8, dim + 1, device=DEV).half()  # rows that are not on 16-byte boundaries
+    odd[..., 1:] = q
+    assert torch.equal(paged.paged_attention(odd[..., 1:], k, v, table, held), ref)
+    assert torch.equal(paged.paged_attention(q.transpose(0, 1).contiguous().transpose(0, 1), k, v, table, held), ref)
+    kv = torch.stack([k, v], 1)
+    assert torch.equal(paged.paged_attention(q, kv[:, 0], kv[:, 1], table, held), ref)
+
+
+@pytest.mark.parametrize("dtype", U.DTYPES)
+def test_places_behind_two_to_the_32_bytes(dtype):
+    """Pages 2^31 elements and more from the cache's start."""
+    lengths, page, dim, far = [100], 16, 64, (1 << 31) + 1024
+    q, k, v, table, held = case(lengths, 4, 2, dim, page, dtype)
+    room = torch.empty(2 * far + 4096, dtype=dtype, device=DEV)
+    wide = room.as_strided((3, 2, page, dim), (far, page * dim, dim, 1))
+    to = [0, 2, 1]
+    for j in range(3):
+        wide[to[j]] = k[int(table[0, j])]
+    near_v = torch.stack([v[int(table[0, j])] for j in (0, 2, 1)])
+    got = paged.paged_attention(q, wide, near_v, ints([to]), ints([48]))
+    U.check_attention(got, q, torch.stack([wide[j] for j in range(3)]), near_v, ints([to]), [48])
+
+
+@pytest.mark.parametrize("dtype", U.DTYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(8, 2, 128, 64), (6, 6, 80, 16), (20, 1, 64, 32)])
+def test_attention_over_listed_pages(heads, kv_heads, dim, page, dtype):
+    lengths = [1000, 3 * page + 1, page, 0, 5]
+    q, k, v, table, held = case(lengths, heads, kv_heads, dim, page, dtype)
+    gen = torch.Generator().manual_seed(4)
+    count = 7
+    lists = torch.full((len(lengths), kv_heads, count), -1, dtype=torch.int32)
+    for i, n in enumerate(lengths):
+        pages = (n + page - 1) // page
+        for h in range(kv_heads):
+            some = torch.randperm(pages, generator=gen)[:count].sort().values
+            lists[i, h, :len(some)] = some.int()
+    got = paged.paged_attention(q, k, v, table, held, pages=lists.to(DEV))
+    U.check_attention(got, q, k, v, table, lengths, pages=lists)
+    # any order, one page twice, entries that are no page, and behind what the row holds nothing is read
+    rough = lists.clone()
+    rough[0, 0] = torch.tensor([5, 2, 2, 2 ** 31 - 1, 0, -9, 1000 // page])
+    rough[1, 0] = torch.tensor([3, 0, 3, 1, 2, 1, 0])
+    rough[2, 0] = torch.tensor([0, 0, 0, 0, 0, 0, 0])
+    got = paged.paged_attention(q, k, v, table, held, pages=rough.to(DEV))
+    U.check_attention(got, q, k, v, table, lengths, pages=rough)
+    none = torch.zeros(len(lengths), kv_heads, 0, dtype=torch.int32, device=DEV)
+    assert not paged.paged_attention(q, k, v, table, held, pages=none).any()
+    every = torch.arange(table.size(1), dtype=torch.int32, device=DEV).expand(len(lengths), kv_heads, -1).contiguous()
+    U.check_attention(paged.paged_attention(q, k, v, table, held, pages=every), q, k, v, table, lengths)
+
+
+def test_attention_refuses():
+    q, k, v, table, held = case([50, 20], 4, 2, 64, 16, F16)
+    def refused(q=q, k=k, v=v, table=table, held=held, **kwargs):
+        with pytest.raises(RuntimeError):
+            paged.paged_attention(q, k, v, table, held, **kwargs)
+    refused(q=q.float())
+    refused(q=q.bfloat16())
+    refused(q=q[:, :3])
+    refused(q=q[..., :32])
+    refused(q=q[:1])
+    refused(q=q[0])
+    refused(q=q.clone().requires_grad_(True))
+    refused(k=k.clone().requires_grad_(True))
+    refused(k=k[:, :1])
+    refused(k=k.transpose(2, 3).contiguous().transpose(2, 3))
+    refused(k=k[:1].expand(k.shape))
+    refused(v=v.bfloat16())
+    refused(v=v[:1])
+    refused(k=k[:, :, :8].contiguous(), v=v[:, :, :8].contiguous())
+    refused(table=table.long())
+    refused(table=table[:1])
+    refused(table=torch.cat([table, table], 1)[:, ::2])
+    refused(table=table.cpu())
+    refused(held=held.long())
+    refused(held=held.cpu())
+    refused(scale=float("inf"))
+    refused(pages=torch.zeros(2, 4, 3, dtype=torch.int32, device=DEV))
+    refused(pages=torch.zeros(2, 2, 3, device=DEV))
+    refused(pages=torch.zeros(2, 2, 3, dtype=torch.int32))
+    with torch.no_grad():
+        paged.paged_attention(q.clone().requires_grad_(True), k, v, table, held)
+
+
+# ------------------------------------------------------------------------------------------------- selection
+
+@pytest.mark.parametrize("dtype", U.DTYPES)
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim,page,count,first,last", [
+    ([1000, 64, 65, 0, 1, 16], 8, 2, 128, 16, 4, 1, 1),
+    ([4096, 3000], 6, 6, 80, 16, 33, 1, 1),
+    ([5000], 16, 1, 64, 32, 1, 0, 0),
+    ([5000], 16, 1, 64, 32, 1, 1, 0),
+    ([700, 699], 5, 1, 8, 16, 40, 3, 5),
+    ([2000, 100], 32, 32, 96, 64, 16, 8, 8),
+    ([30000, 17], 4, 2, 32, 16, 200, 0, 2),
+    ([70000], 4, 1, 128, 16, 64, 1, 1),
+])
+def test_selection(lengths, heads, kv_heads, dim, page, count, first, last, dtype):
+    q, k, v, table, held = case(lengths, heads, kv_heads, dim, page, dtype)
+    boxes = U.boxes_of(k, table, lengths, page)
+    got = paged.paged_select(q, boxes, table, held, page, count, first, last)
+    assert torch.equal(got.cpu(), U.select(q, boxes, table, lengths, page, count, first, last))
+
+
+def test_selection_of_equal_scores_takes_the_lower_pages():
+    lengths = [1600, 1600, 333]
+    q, k, v, table, held = case(lengths, 4, 2, 64, 16, F16)
+    boxes = U.boxes_of(k, table, lengths, 16)
+    q[0] = 0.0                      # all scores are zero
+    boxes[...] = (torch.randn(boxes.shape, device=DEV) * 2).round()
+    q[1] = (q[1] * 2).round()       # small whole numbers: many scores are equal
+    boxes[table[1, :100].long(), 0, :, 1:] = 0.0
+    got = paged.paged_select(q, boxes, table, held, 16, 20, 1, 1)
+    assert torch.equal(got.cpu(), U.select(q, boxes, table, lengths, 16, 20, 1, 1))
+    assert got[0, 0].tolist() == list(range(19)) + [99]
+
+
+def test_selection_tells_scores_apart_that_are_equal_in_32_bits():
+    """Two pages whose scores differ by 2^-40 of their size."""
+    q, k, v, table, held = case([160], 1, 1, 64, 16, BF16)
+    boxes = torch.zeros(k.size(0), 1, 2, 64, dtype=BF16, device=DEV)
+    q.zero_()
+    q[0, 0, 0], q[0, 0, 1] = 1.0, 2.0 ** -40
+    for j in range(10):
+        boxes[int(table[0, j]), 0, 1, 0] = 1.0
+    for j in (7, 4):
+        boxes[int(table[0, j]), 0, 1, 1] = 1.0
+    assert paged.paged_select(q, boxes, table, held, 16, 2, 0, 0)[0, 0].tolist() == [4, 7]
+
+
+def test_selection_of_scores_that_are_not_finite():
+    lengths = [1600]
+    q, k, v, table, held = case(lengths, 4, 1, 64, 16, BF16)
+    boxes = U.boxes_of(k, table, lengths, 16)
+    boxes[int(table[0, 40]), 0, 1, 3] = float("nan")
+    boxes[int(table[0, 50]), 0, 1, :] = float("inf")
+    boxes[int(table[0, 60]), 0, :, :] = torch.finfo(BF16).max
+    boxes[int(table[0, 70]), 0, 0, :] = float("-inf")
+    table[0, 80], table[0, 81] = -1, 10 ** 6  # not the cache's: behind all others
+    for count in (1, 2, 3, 4, 5, 97, 98, 99):
+        got = paged.paged_select(q, boxes, table, held, 16, count, 0, 0)
+        assert torch.equal(got.cpu(), U.select(q, boxes, table, lengths, 16, count, 0, 0)), count
+
+
+def test_selection_is_bounded_and_refuses():
+    q, k, v, table, held = case([500, 200], 4, 2, 64, 16, F16)
+    boxes = U.boxes_of(k, table, [500, 200], 16)
+    wide = paged.paged_select(q, boxes, table, ints([2 ** 31 - 1, -3]), 16, 8)
+    assert torch.equal(wide.cpu(), U.select(q, boxes, table, [2 ** 31 - 1, -3], 16, 8, 1, 1)) and (wide[1] == -1).all()
+    assert paged.paged_select(q[:0], boxes, table[:0], held[:0], 16, 8).shape == (0, 2, 8)
+    assert (paged.paged_select(q, boxes, table[:, :0].contiguous(), held, 16, 8) == -1).all()
+    def refused(q=q, boxes=boxes, table=table, held=held, page=16, count=8, first=1, last=1):
+        with pytest.raises(RuntimeError):
+            paged.paged_select(q, boxes, table, held, page, count, first, last)
+    refused(count=0)
+    refused(count=1)
+    refused(first=-1)
+    refused(last=8)
+    refused(first=2 ** 62, last=2 ** 62)
+    refused(page=24)
+    refused(boxes=boxes.bfloat16())
+    refused(boxes=boxes[:, :, :1])
+    refused(boxes=boxes[::2])
+    refused(q=q.clone().requires_grad_(True))
+    refused(table=torch.zeros(2, 20000, dtype=torch.int32, device=DEV))
+    refused(held=held[:1])
+
+
+# ------------------------------------------------------------------------------------------------- appending
+
+APPENDS = [
+    # lengths, new tokens, heads, kv_heads, dim, page, rotary, interleaved, rows behind the last sequence
+    ([1], [1], 1, 1, 8, 16, 8, False, 0),
+    ([5, 16, 17, 1, 33], [1, 1, 1, 1, 1], 4, 2, 64, 16, 64, False, 0),
+    ([500, 64, 65], [500, 64, 3], 8, 2, 128, 64, 128, False, 0),
+    ([100, 0, 40, 7], [37, 0, 40, 7], 6, 6, 80, 16, 48, True, 5),
+    ([300, 301], [200, 1], 4, 1, 96, 32, 20, False, 1),
+    ([90], [90], 10, 2, 40, 16, 6, True, 0),
+    ([70, 256, 20], [33, 255, 20], 16, 1, 120, 256, 0, False, 70),
+    ([2000], [1999], 5, 5, 128, 64, 128, True, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", U.DTYPES)
+@pytest.mark.parametrize("lengths,new,heads,kv_heads,dim,page,rotary,interleaved,padded", APPENDS)
+def test_append(lengths, new, heads, kv_heads, dim, page, rotary, interleaved, padded, dtype):
+    gen = torch.Generator().manual_seed(1)
+    old = [a - b for a, b in zip(lengths, new)]
+    k_cache, v_cache, table = U.make_cache(gen, lengths, kv_heads, dim, page, dtype, fill=0.0)
+    boxes = U.boxes_of(k_cache, table, old, page)
+    before = k_cache.clone(), v_cache.clone(), boxes.clone()
+    tokens = sum(new) + padded
+    fused = torch.randn(tokens, (heads + 2 * kv_heads) * dim, generator=gen).to(dtype).to(DEV)
+    q = fused[:, :heads * dim].view(tokens, heads, dim)
+    k = fused[:, heads * dim:(heads + kv_heads) * dim].view(tokens, kv_heads, dim)
+    v = fused[:, (heads + kv_heads) * dim:].view(tokens, kv_heads, dim)
+    cos, sin = paged.rope_table(max(lengths) + 3, rotary, device=DEV)
+    cu = [sum(new[:i]) for i in range(len(new) + 1)]
+    got = paged.paged_append(q, k, v, k_cache, v_cache, table, ints(lengths), ints(cu), rope=(cos, sin), interleaved=interleaved,
+                             boxes=boxes)
+    assert got.shape == q.shape and not got[cu[-1]:].any()
+    for i in range(len(lengths)):
+        if new[i] == 0:
+            continue
+        at = torch.arange(old[i], lengths[i], device=DEV)
+        rows = slice(cu[i], cu[i + 1])
+        U.check_turned(got[rows], q[rows], cos[at], sin[at], interleaved)
+        to = table[i].long()[at // page]
+        U.check_turned(k_cache[to, :, at % page], k[rows], cos[at], sin[at], interleaved)
+        assert torch.equal(v_cache[to, :, at % page], v[rows])
+        before[0][to, :, at % page] = k_cache[to, :, at % page]
+        before[1][to, :, at % page] = v[rows]
+    assert torch.equal(before[0], k_cache) and torch.equal(before[1], v_cache)  # all else is as it was
+    assert torch.equal(boxes, U.boxes_of(k_cache, table, lengths, page))
+    # without boxes, again: the same
+    again = paged.paged_append(q, k, v, k_cache, v_cache, table, ints(lengths), ints(cu), rope=(cos, sin), interleaved=interleaved)
+    assert torch.equal(again, got) and torch.equal(before[0], k_cache)
+
+
+@pytest.mark.parametrize("dtype", U.DTYPES)
+def test_append_without_rotation_copies_bits(dtype):
+    gen = torch.Generator().manual_seed(1)
+    k_cache, v_cache, table = U.make_cache(gen, [40, 16], 2, 64, 16, dtype, fill=0.0)
+    q, k, v = (torch.randint(-2 ** 15, 2 ** 15, (2, h, 64), generator=gen, dtype=torch.int16).view(dtype).to(DEV) for h in (4, 2, 2))
+    out = paged.paged_append(q, k, v, k_cache, v_cache, table, ints([40, 16]))
+    bits = lambda t: t.view(torch.int16)
+    assert torch.equal(bits(out), bits(q))
+    for i, (place, slot) in enumerate([(2, 7), (0, 15)]):
+        assert torch.equal(bits(k_cache[int(table[i, place]), :, slot].contiguous()), bits(k[i]))
+        assert torch.equal(bits(v_cache[int(table[i, place]), :, slot].contiguous()), bits(v[i]))
+
+
+def test_append_one_token_each_equals_ragged():
+    gen = torch.Generator().manual_seed(2)
+    lengths = [1, 0, 64, 65, 200]
+    k_cache, v_cache, table = U.make_cache(gen, lengths, 2, 128, 64, F16, fill=0.0)
+    rope = paged.rope_table(300, 128, device=DEV)
+    q, k, v = (torch.randn(5, h, 128, generator=gen).half().to(DEV) for h in (8, 2, 2))
+    a, b = [t.clone() for t in (k_cache, v_cache)], [t.clone() for t in (k_cache, v_cache)]
+    one = paged.paged_append(q, k, v, *a, table, ints(lengths), rope=rope)
+    two = paged.paged_append(q, k, v, *b, table, ints(lengths), ints([0, 1, 2, 3, 4, 5]), rope=rope)
+    assert torch.equal(one, two) and torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    assert not one[1].any() and one[0].any()  # an idle sequence
+
+
+def test_boxes_propagate_nan_and_begin_anew():
+    gen = torch.Generator().manual_seed(3)
+    k_cache, v_cache, table = U.make_cache(gen, [32], 1, 64, 16, BF16, fill=0.0)
+    boxes = torch.full((k_cache.size(0), 1, 2, 64), 99.0, dtype=BF16, device=DEV)
+    def put(length, value):
+        x = torch.full((1, 1, 64), value, dtype=BF16, device=DEV)
+        paged.paged_append(x, x, x, k_cache, v_cache, table, ints([length]), boxes=boxes)
+        return boxes[int(table[0, (length - 1) // 16]), 0, :, 0].tolist()
+    assert put(1, 2.0) == [2.0, 2.0]          # what was there before the page's first position does not count
+    assert put(2, -1.0) == [-1.0, 2.0]
+    assert put(3, 0.5) == [-1.0, 2.0]
+    assert all(x != x for x in put(4, float("nan")))
+    assert all(x != x for x in put(5, 1.0))
+    assert put(17, 3.0) == [3.0, 3.0]
+    assert put(1, 7.0) == [7.0, 7.0]
+
+
+def test_append_drops_tokens_without_a_place():
+    gen = torch.Generator().manual_seed(4)
+    k_cache, v_cache, table = U.make_cache(gen, [64, 64, 64], 2, 64, 16, F16, spare=0, fill=0.0)
+    rope = paged.rope_table(60, 64, device=DEV)
+    table[1, 2] = -1
+    table[2, 0] = k_cache.size(0)
+    before = k_cache.clone(), v_cache.clone()
+    boxes = U.boxes_of(k_cache, table[:1], [64], 16)
+    kept = boxes.clone()
+    q, k, v = (torch.randn(3 * 50, h, 64, generator=gen).half().to(DEV) for h in (2, 2, 2))
+    # sequence 0: positions 14 .. 63, angles for 60; 1: a page is missing; 2: begins 20 positions in front of 0, first page missing
+    out = paged.paged_append(q, k, v, k_cache, v_cache, table, ints([64, 64, 30]), ints([0, 50, 100, 150]), rope=rope, boxes=boxes)
+    written = [(0, p) for p in range(14, 60)] + [(1, p) for p in range(14, 60) if not 32 <= p < 48] + [(2, p) for p in range(16, 30)]
+    start = [14, 14, -20]
+    rows = {50 * i + p - start[i] for i, p in written}
+    for r in range(150):
+        assert bool(out[r].any()) == (r in rows), r
+    for i, p in written:
+        before[0][int(table[i, p // 16]), :, p % 16] = k_cache[int(table[i, p // 16]), :, p % 16]
+        before[1][int(table[i, p // 16]), :, p % 16] = v[50 * i + p - start[i]]
+    assert torch.equal(before[0], k_cache) and torch.equal(before[1], v_cache)
+    touched = {int(table[i, p // 16]) for i, p in written}
+    rest = [p for p in range(k_cache.size(0)) if p not in touched]
+    assert torch.equal(boxes[rest], kept[rest])
+    # behind the table
+    out = paged.paged_append(q[:1], k[:1], v[:1], k_cache, v_cache, table[:1], ints([65]))
+    assert not out.any() and torch.equal(before[0], k_cache)
+    out = paged.paged_append(q[:2], k[:2], v[:2], k_cache, v_cache, table[:2], ints([2 ** 31 - 1, -2 ** 31]))
+    assert not out.any() and torch.equal(before[0], k_cache)
+    # no sequences at all: nothing but rows behind the last one
+    assert not paged.paged_append(q, k, v, k_cache, v_cache, table[:0], ints([]), ints([0])).any()
+    assert paged.paged_append(q[:0], k[:0], v[:0], k_cache, v_cache, table[:0], ints([])).shape == (0, 2, 64)
+    assert torch.equal(before[0], k_cache) and torch.equal(before[1], v_cache)
+
+
+def test_append_refuses():
+    gen = torch.Generator().manual_seed(5)
+    k_cache, v_cache, table = U.make_cache(gen, [20, 20], 2, 64, 16, F16, fill=0.0)
+    held, rope = ints([20, 20]), paged.rope_table(64, 64, device=DEV)
+    q, k, v = (torch.randn(2, h, 64, generator=gen).half().to(DEV) for h in (4, 2, 2))
+    boxes = U.boxes_of(k_cache, table, [20, 20], 16)
+    def refused(q=q, k=k, v=v, k_cache=k_cache, v_cache=v_cache, table=table, held=held, cu=None, rope=rope, boxes=boxes):
+        with pytest.raises(RuntimeError):
+            paged.paged_append(q, k, v, k_cache, v_cache, table, held, cu, rope, False, boxes)
+    refused(k=k[:1])
+    refused(v=v[:, :1])
+    refused(k=k.bfloat16())
+    refused(q=q.clone().requires_grad_(True))
+    refused(k_cache=k_cache.bfloat16(), v_cache=v_cache.bfloat16())
+    refused(v_cache=v_cache[:1])
+    refused(q=torch.cat([q, q]), k=torch.cat([k, k]), v=torch.cat([v, v]))
+    refused(cu=ints([0, 1]))
+    refused(cu=torch.tensor([0, 1, 2], device=DEV))
+    refused(rope=(rope[0], rope[1][:, :5]))
+    refused(rope=(rope[0].double(), rope[1].double()))
+    refused(rope=paged.rope_table(64, 128, device=DEV))
+    refused(rope=(rope[0], None))
+    refused(boxes=boxes[:1])
+    refused(boxes=boxes.bfloat16())
+    refused(held=held[:1])
+    version = k_cache._version
+    paged.paged_append(q, k, v, k_cache, v_cache, table, held)
+    assert k_cache._version > version
+
+
+# -------------------------------------------------------------------------------------------------- together
+
+def _decode(cache, rope, steps, heads, kv_heads, dim, table, start, gen, count=None):
+    """`steps` decoding steps of a batch; the outputs, and q, k, v as they came."""
+    outs, seen = [], []
+    lengths = list(start)
+    for _ in range(steps):
+        lengths = [n + 1 for n in lengths]
+        held = ints(lengths)
+        q, k, v = (torch.randn(len(start), h, dim, generator=gen).to(cache.k.dtype).to(DEV) for h in (heads, kv_heads, kv_heads))
+        turned = cache.append(q, k, v, table, held, rope=rope)
+        out = cache.attend(turned, table, held) if count is None else cache.attend_selected(turned, table, held, count)
+        outs.append(out)
+        seen.append((turned, lengths))
+    return outs, seen
+
+
+@pytest.mark.parametrize("dtype", U.DTYPES)
+def test_a_prompt_and_decoding_steps(dtype):
+    """Prompts of uneven lengths appended at once, then tokens one by one, with full and with selected attention."""
+    heads, kv_heads, dim, page = 8, 2, 64, 16
+    gen = torch.Generator().manual_seed(7)
+    cache = paged.PagedKVCache(64, kv_heads, dim, page, dtype, device=DEV)
+    rope = paged.rope_table(512, dim, device=DEV)
+    table = torch.randperm(60, generator=gen)[:48].reshape(3, 16).to(torch.int32).to(DEV)
+    prompt = [130, 1, 47]
+    q, k, v = (torch.randn(sum(prompt), h, dim, generator=gen).to(dtype).to(DEV) for h in (heads, kv_heads, kv_heads))
+    turned = cache.append(q, k, v, table, ints(prompt), ints([0, 130, 131, 178]), rope=rope)
+    # the prompt's own attention, causal: a row for each token
+    rows_table = torch.cat([table[i:i + 1].expand(n, -1) for i, n in enumerate(prompt)]).contiguous()
+    sees = [j + 1 for n in prompt for j in range(n)]
+    U.check_attention(cache.attend(turned, rows_table, ints(sees)), turned, cache.k, cache.v, rows_table, sees)
+    outs, seen = _decode(cache, rope, 20, heads, kv_heads, dim, table, prompt, gen)
+    U.check_attention(outs[-1], seen[-1][0], cache.k, cache.v, table, seen[-1][1])
+    assert torch.equal(cache.boxes[table[0, :9].long()], U.boxes_of(cache.k, table, seen[-1][1], page)[table[0, :9].long()])
+    outs, seen = _decode(cache, rope, 3, heads, kv_heads, dim, table, seen[-1][1], gen, count=4)
+    out, pages = outs[-1]
+    assert torch.equal(pages.cpu(), U.select(seen[-1][0], cache.boxes, table, seen[-1][1], page, 4, 1, 1))
+    U.check_attention(out, seen[-1][0], cache.k, cache.v, table, seen[-1][1], pages=pages)
+
+
+def test_steps_captured_into_two_graphs_and_replayed_in_turn():
+    heads, kv_heads, dim, page = 8, 2, 128, 64
+    gen = torch.Generator().manual_seed(8)
+    rope = paged.rope_table(2048, dim, device=DEV)
+    sets = []
+    for lengths in ([900, 30], [100, 1500]):
+        k, v, table = U.make_cache(gen, [n + 10 for n in lengths], kv_heads, dim, page, F16, fill=0.0)
+        boxes = U.boxes_of(k, table, [n + 10 for n in lengths], page)
+        held = ints(lengths)
+        x = [torch.randn(2, h, dim, generator=gen).half().to(DEV) for h in (heads, kv_heads, kv_heads)]
+        def step(k=k, v=v, table=table, boxes=boxes, held=held, x=x):
+            q = paged.paged_append(*x, k, v, table, held, rope=rope, boxes=boxes)
+            pages = paged.paged_select(q, boxes, table, held, page, 4)
+            return q, paged.paged_attention(q, k, v, table, held), paged.paged_attention(q, k, v, table, held, pages=pages), pages
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+        sets.append((graph, outs, step, held, x))
+    for turn in range(3):
+        for graph, outs, step, held, x in sets:
+            held += 1
+            for t in x:
+                t.mul_(-0.9)
+            graph.replay()
+        torch.cuda.synchronize()
+        for graph, outs, step, held, x in sets:
+            for a, b in zip(outs, step()):
+                assert torch.equal(a, b)
+
+
+def test_two_streams_at_once_and_another_than_the_tensors_own():
+    q, k, v, table, held = case([3000, 200, 0, 1500], 16, 4, 128, 64, BF16)
+    boxes = U.boxes_of(k, table, [3000, 200, 0, 1500], 64)
+    ref = paged.paged_attention(q, k, v, table, held)
+    ref_pages = paged.paged_select(q, boxes, table, held, 64, 5)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append((paged.paged_attention(q, k, v, table, held), paged.paged_select(q, boxes, table, held, 64, 5)))
+    torch.cuda.synchronize()
+    for out, pages in got:
+        assert torch.equal(out, ref) and torch.equal(pages, ref_pages)
+
+
+def test_chained_calls_read_what_the_one_in_front_has_written():
+    """Launches overlap: nothing is read before the kernel in front is done."""
+    gen = torch.Generator().manual_seed(9)
+    k, v, table = U.make_cache(gen, [4000] * 4, 4, 128, 64, F16, fill=0.0)
+    boxes = U.boxes_of(k, table, [4000] * 4, 64)
+    rope = paged.rope_table(4096, 128, device=DEV)
+    xs = [[torch.randn(4, h, 128, generator=gen).half().to(DEV) for h in (16, 4, 4)] for _ in range(20)]
+    def walk(sync):
+        kk, vv, bb, held, outs = k.clone(), v.clone(), boxes.clone(), ints([3900] * 4), []
+        for x in xs:
+            torch.add(held, 1, out=held)
+            for call in range(3):
+                if call == 0:
+                    q = paged.paged_append(*x, kk, vv, table, held, rope=rope, boxes=bb)
+                elif call == 1:
+                    pages = paged.paged_select(q, bb, table, held, 64, 6)
+                else:
+                    outs.append(paged.paged_attention(q, kk, vv, table, held, pages=pages))
+                    outs.append(paged.paged_attention(q, kk, vv, table, held))
+                if sync:
+                    torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return outs
+    for a, b in zip(walk(True), walk(False)):
+        assert torch.equal(a, b)
+
+
+def test_random_calls():
+    import random
+    rng = random.Random(11)
+    for _ in range(60):
+        kv_heads = rng.choice([1, 2, 3, 8])
+        heads, dim, page, dtype = kv_heads * rng.choice([1, 2, 3, 4, 7, 8, 9, 16, 17]), 8 * rng.randint(1, 16), rng.choice([16, 32, 64, 128, 256]), rng.choice(U.DTYPES)
+        lengths = [rng.choice([0, 1, rng.randint(1, 64), rng.randint(1, 1500)]) for _ in range(rng.randint(1, 9))]
+        q, k, v, table, held = case(lengths, heads, kv_heads, dim, page, dtype, seed=rng.randint(0, 99))
+        U.check_attention(paged.paged_attention(q, k, v, table, held), q, k, v, table, lengths)
+        first, last = rng.randint(0, 2), rng.randint(0, 2)
+        count = max(1, first + last) + rng.randint(0, 6)
+        boxes = U.boxes_of(k, table, lengths, page)
+        pages = paged.paged_select(q, boxes, table, held, page, count, first, last)
+        assert torch.equal(pages.cpu(), U.select(q, boxes, table, lengths, page, count, first, last))
+        U.check_attention(paged.paged_attention(q, k, v, table, held, pages=pages), q, k, v, table, lengths, pages=pages)
