@@ -541,7 +541,8 @@ IEX_API void* iex_graph_combine(void* const* graphs, int count);
  * without a place (position below 0 or behind the table or the angles, page not of the cache), are zero
  * there and leave the cache as it is.
  * boxes (or NULL) [num_pages, kv_heads, 2, head_dim]: smallest and largest key of a page in
- * each dimension, begun anew by the token at a page's first position, else joined with what is there.
+ * each dimension; those of the pages that are written to are formed from all positions of the
+ * page up to the last new one.
  * A page that is written to belongs to one sequence of the call. */
 IEX_API int iex_paged_append(int tokens, int batch, int heads, int kv_heads, int head_dim, int bf16,
                              const void* q, long long q_row, long long q_head, const void* k,

@@ -4,8 +4,8 @@
 // Sequence i has n = cu_tokens[i + 1] - cu_tokens[i] new tokens (one without cu_tokens); its j-th new token takes position
 // lengths[i] - n + j.  Of every query and key the first `rotary` elements are turned in pairs by the angles of the position,
 //   (a, b) -> (a cos - b sin, b cos + a sin),   pairs (i, i + rotary / 2), or (2 i, 2 i + 1) if interleaved,
-// in fp32, and rounded once.  boxes (optional) holds the smallest and largest key of every page and head in each dimension: begun
-// anew by the token at the page's first position, joined with what is there by the others.
+// in fp32, and rounded once.  boxes (optional) holds the smallest and largest key of every page and head in each dimension: of a
+// page that is written to they are formed anew from all its positions up to the last new one.
 //
 // A block does one page's new tokens of one key head and its query heads, so that a box has one writer.
 #include "paged.cuh"
@@ -105,10 +105,14 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
     any = true;
   }
   if (p.boxes != nullptr && any) {
+    const T* held_keys = static_cast<const T*>(p.k_cache) + at * p.k_page + static_cast<long long>(kv) * page * p.dim + d;
+    for (int slot = 0; slot < from % page; ++slot) {
+      lo = smaller(lo, held_keys[slot * p.dim]);
+      hi = larger(hi, held_keys[slot * p.dim]);
+    }
     T* box = static_cast<T*>(p.boxes) + (static_cast<long long>(at) * p.kv_heads + kv) * 2 * p.dim + d;
-    const bool anew = from % page == 0;
-    box[0] = anew ? lo : smaller(lo, box[0]);
-    box[p.dim] = anew ? hi : larger(hi, box[p.dim]);
+    box[0] = lo;
+    box[p.dim] = hi;
   }
 }
 

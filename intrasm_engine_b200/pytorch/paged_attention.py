@@ -47,9 +47,8 @@ def paged_append(q, k, v, k_cache, v_cache, block_table, lengths, cu_tokens=None
     lie).  Sequence ``i`` has the rows ``cu_tokens[i]`` to ``cu_tokens[i + 1]`` (int32 ``[sequences + 1]``, ascending from 0), or without it
     row ``i``; its last one takes position ``lengths[i] - 1``.  ``rope`` is ``(cos, sin)`` as ``rope_table`` makes them: the first
     ``2 * cos.size(1)`` elements of a head are turned, element ``i`` with ``i + cos.size(1)``, or ``2 i`` with ``2 i + 1`` if ``interleaved``.
-    ``boxes`` ``[pages, kv_heads, 2, head_dim]`` keeps the smallest and largest key of each page in each dimension: begun anew by the token
-    at a page's first position, else joined with what is there (a sequence that is cut back and grows again has boxes
-    that are larger than needed).
+    ``boxes`` ``[pages, kv_heads, 2, head_dim]`` keeps the smallest and largest key of each page in each dimension: those of the pages that
+    are written to are formed from all positions of the page up to the last new one (also where a sequence was cut back).
 
     Rows behind the last sequence, and tokens that have no place (position below 0, behind the table or behind ``rope``, a page that
     is not one of the cache's), come back as zeros and leave the cache as it is.  A page that is written belongs to one sequence of the call."""

@@ -401,6 +401,17 @@ def test_boxes_propagate_nan_and_begin_anew():
     assert put(1, 7.0) == [7.0, 7.0]
 
 
+def test_boxes_of_a_sequence_that_was_cut_back():
+    """What a box said before does not count, nor do keys behind the last new one."""
+    gen = torch.Generator().manual_seed(3)
+    k_cache, v_cache, table = U.make_cache(gen, [60], 2, 64, 32, F16, fill=0.0)
+    boxes = torch.full((k_cache.size(0), 2, 2, 64), 99.0, dtype=F16, device=DEV)
+    x = torch.randn(3, 2, 64, generator=gen).half().to(DEV)
+    paged.paged_append(x, x, x, k_cache, v_cache, table, ints([41]), ints([0, 3]), boxes=boxes)
+    ref = U.boxes_of(k_cache, table, [41], 32)
+    assert torch.equal(boxes[int(table[0, 1])], ref[int(table[0, 1])]) and (boxes[int(table[0, 0])] == 99.0).all()
+
+
 def test_append_drops_tokens_without_a_place():
     gen = torch.Generator().manual_seed(4)
     k_cache, v_cache, table = U.make_cache(gen, [64, 64, 64], 2, 64, 16, F16, spare=0, fill=0.0)
