@@ -2,7 +2,24 @@
 //
 //   out[r, h] = sum_t softmax_t(scale * q[r, h] . k[t]) v[t],   t over the positions that row r holds,
 //
-// with heads / kv_heads query heads to a key head, or over the positions of the pages that pages[r, kv_head] lists.
+// with heads / kv_heads query heads to a key head, or over the positions of the pages that pages[r, kv_head] lists.  A segment is
+// what one row and one key head (up to 16 of its query heads) have to read, in chunks of 16 positions.  One to sixteen flops a byte: HBM bounds it.
+//
+// Work: the chunks of all segments, in order, are shared out evenly to the warps of one block per SM, whatever the rows'
+// lengths; a warp that has a whole segment writes its rows, the others leave maximum, sum and product, which the block joins through
+// shared memory and, where a segment reaches over several blocks, join_kernel joins from the workspace, in order.
+//
+// A chunk: keys and values come straight from global memory into registers, 16 bytes a lane, the next chunk's keys requested
+// when this one's scores are formed and its values after the product; the lengths of what a warp has on its way (8 KB) and nothing else covers
+// the latency, no barriers.  Products are m16n8k16 with the positions (scores) or the elements of v (output) as
+// the 16 rows and 8 query heads as the columns, so that a key head with few query heads does not pay for 16:
+//   S^T = K Q^T    a lane's 16 bytes of a key are its fragments of two instructions: the order of a sum's terms is free as
+//                  long as both operands agree
+//   O^T = V^T P^T  a lane's 16 bytes of four positions, bytes paired up by prmt, are its fragments of four; the scores'
+//                  accumulators become P^T by movmatrix
+// The running maximum, sum and O are fp32.  P enters the second product as a 16-bit head and the 16-bit rest, so that what is lost of it
+// does not show beside the output's own rounding; fp16 weights carry 2^15, which keeps small ones out of the subnormals.
+#include <algorithm>
 #include <cmath>
 
 #include "paged.cuh"
@@ -11,50 +28,543 @@ namespace iex {
 namespace paged {
 namespace {
 
+constexpr int kWarps = 8;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kChunk = 16;
+constexpr int kMinChunks = 2;  // of a warp: with less to do, fewer warps
+constexpr int kJoinThreads = 128;
+
 struct AttentionParams {
-  int rows, heads, kv_heads, dim, num_pages, page_shift, table_width, count;
+  int rows, heads, kv_heads, dim, num_pages, page_shift, table_width, count, parts;  // parts: segments of a key head
   Rows q;
   const void *k_cache, *v_cache;
   long long k_page, v_page;
   const int32_t *table, *lengths, *pages;
-  float scale;
+  float scale_log2;  // the factor of a score in an exponent of 2
   void* out;
+  int2* open;      // [blocks]: the segment that begins in a block and ends in another, or -1; the block that it ends in
+  float2* stats;   // [blocks][2][heads of a segment]: maximum and sum of a block's part of a segment that ...
+  float* product;  // [blocks][2][heads of a segment][dim bucket]  ... 0: began in front of the block, 1: begins in it
 };
 
-// A warp per row and query head, a lane per 32nd element.
 template <typename T>
-__global__ void __launch_bounds__(32) attention_kernel(const __grid_constant__ AttentionParams p) {
+struct Half2;
+template <>
+struct Half2<__half> {
+  static constexpr float kBias = 15.f;  // weights are 2^15 times as large
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return reinterpret_cast<const uint32_t&>(v);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(reinterpret_cast<const __half2&>(v)); }
+};
+template <>
+struct Half2<__nv_bfloat16> {
+  static constexpr float kBias = 0.f;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return reinterpret_cast<const uint32_t&>(v);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t v) {
+    return __bfloat1622float2(reinterpret_cast<const __nv_bfloat162&>(v));
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma<__half>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                            uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                   uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The 8 x 8 matrix of 16-bit elements that the warp holds, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t t;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(v));
+  return t;
+}
+// Read once by this SM; may have been written by the kernel in front (see linear_few.cu on loads that are not volatile).
+__device__ __forceinline__ uint4 load_once(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t& word(uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ float max_over_positions(float v) {  // of the lanes with the same lane % 4
+  for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+  return v;
+}
+__device__ __forceinline__ float sum_over_positions(float v) {
+  for (int d = 4; d < 32; d <<= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+
+// Chunks of a segment of row `row`.
+__device__ __forceinline__ int chunks_of(const AttentionParams& p, int row) {
+  const int length = held(p.lengths, row, p.table_width, p.page_shift);
+  if (p.pages == nullptr) return (length + kChunk - 1) / kChunk;
+  const int pages = (length + (1 << p.page_shift) - 1) >> p.page_shift;
+  return min(p.count, pages) << (p.page_shift - 4);
+}
+
+// PIECES: of 64 elements of a head; NT: groups of 8 query heads of a segment.
+template <typename T, int PIECES, int NT>
+__global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ AttentionParams p) {
+  constexpr int kHeads = 8 * NT, kDim = 64 * PIECES, kPitch = kDim + 4;
+  extern __shared__ float parts_of_warps[];  // [warp][2][kHeads][kPitch], then [warp][2][kHeads] float2
+  __shared__ long long before[kThreads + 1];  // chunks (of one segment) of the rows in front of a thread's
+  __shared__ long long warp_sums[kWarps];
+  __shared__ int segment_of[kWarps][2], last_block[kWarps], ends[kWarps];
+  float2* const stats_of_warps = reinterpret_cast<float2*>(parts_of_warps + 2 * kWarps * kHeads * kPitch);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int per_row = p.kv_heads * p.parts, group = p.heads / p.kv_heads, page = 1 << p.page_shift, sub_shift = p.page_shift - 4;
+  const long long head_stride = static_cast<long long>(page) * p.dim;
+
   grid_dependency_wait();
-  const int row = blockIdx.x / p.heads, head = blockIdx.x % p.heads, kv = head / (p.heads / p.kv_heads), lane = threadIdx.x;
-  const int page = 1 << p.page_shift, held_here = held(p.lengths, row, p.table_width, p.page_shift);
-  const int held_pages = (held_here + page - 1) >> p.page_shift, entries = p.pages ? min(p.count, held_pages) : held_pages;
-  const T* q = static_cast<const T*>(p.q.data) + row * p.q.row + head * p.q.head;
-  float mine[4], acc[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, total = 0.f;
-  for (int i = 0; i < 4; ++i) mine[i] = lane + 32 * i < p.dim ? as_float(q[lane + 32 * i]) * p.scale : 0.f;
-  for (int e = 0; e < entries; ++e) {
-    const int nth = p.pages ? p.pages[(static_cast<long long>(row) * p.kv_heads + kv) * p.count + e] : e;
-    if (nth < 0 || nth >= held_pages) continue;
-    const int at = p.table[static_cast<long long>(row) * p.table_width + nth];
-    if (at < 0 || at >= p.num_pages) continue;
-    const T* k = static_cast<const T*>(p.k_cache) + at * p.k_page + static_cast<long long>(kv) * page * p.dim;
-    const T* v = static_cast<const T*>(p.v_cache) + at * p.v_page + static_cast<long long>(kv) * page * p.dim;
-    const int here = min(page, held_here - (nth << p.page_shift));
-    for (int t = 0; t < here; ++t, k += p.dim, v += p.dim) {
-      float s = 0.f;
-      for (int i = 0; i < 4; ++i)
-        if (lane + 32 * i < p.dim) s = fmaf(mine[i], as_float(k[lane + 32 * i]), s);
-      for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-      const float now = fmaxf(top, s), base = now == -INFINITY ? 0.f : now;
-      const float old = __expf(top - base), weight = __expf(s - base);
-      top = now;
-      total = total * old + weight;
-      for (int i = 0; i < 4; ++i)
-        if (lane + 32 * i < p.dim) acc[i] = acc[i] * old + weight * as_float(v[lane + 32 * i]);
+  // ---- how the chunks are shared out
+  const int rows_each = (p.rows + kThreads - 1) / kThreads;
+  {
+    long long mine = 0;
+    for (int r = threadIdx.x * rows_each, i = 0; i < rows_each && r < p.rows; ++i, ++r) mine += chunks_of(p, r);
+    long long sum = mine;
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long other = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += other;
+    }
+    if (lane == 31) warp_sums[warp] = sum;
+    __syncthreads();
+    long long front = 0;
+    for (int w = 0; w < warp; ++w) front += warp_sums[w];
+    before[threadIdx.x] = front + sum - mine;
+    if (threadIdx.x == kThreads - 1) before[kThreads] = front + sum;
+    if (lane < 2) segment_of[warp][lane] = -1;
+    __syncthreads();
+  }
+  const long long total = before[kThreads] * per_row;
+  const long long workers = min(static_cast<long long>(gridDim.x) * kWarps, (total + kMinChunks - 1) / kMinChunks);
+  const long long worker = static_cast<long long>(blockIdx.x) * kWarps + warp;
+  const long long begin = worker < workers ? total * worker / workers : 0, end = worker < workers ? total * (worker + 1) / workers : 0;
+
+  // rows that hold nothing
+  for (int r = blockIdx.x; r < p.rows; r += gridDim.x)
+    if (chunks_of(p, r) == 0) {
+      uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + static_cast<long long>(r) * p.heads * p.dim);
+      for (int i = threadIdx.x; i < p.heads * p.dim / 8; i += kThreads) to[i] = make_uint4(0, 0, 0, 0);
+    }
+
+  // ---- the warp's own chunks
+  int row = 0, part_of_row = 0, chunks = 0, first = 0;  // the segment, its chunks, the first one that is this warp's
+  if (begin < end) {
+    int lo = 0, hi = kThreads;  // the last thread whose rows begin at or in front of `begin`
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (before[mid] * per_row <= begin) lo = mid; else hi = mid;
+    }
+    row = lo * rows_each;
+    long long rest = begin - before[lo] * per_row;
+    for (chunks = chunks_of(p, row); rest >= static_cast<long long>(chunks) * per_row; chunks = chunks_of(p, ++row))
+      rest -= static_cast<long long>(chunks) * per_row;
+    part_of_row = static_cast<int>(rest / chunks);
+    first = static_cast<int>(rest - static_cast<long long>(part_of_row) * chunks);
+  }
+  for (long long at = begin; at < end;) {
+    const int stop = static_cast<int>(min(static_cast<long long>(chunks), first + (end - at)));
+    const int kv = part_of_row / p.parts, head0 = kv * group + (part_of_row - kv * p.parts) * kHeads;
+    const int here = min(kHeads, (kv + 1) * group - head0);  // query heads
+    const int length = held(p.lengths, row, p.table_width, p.page_shift), held_pages = (length + page - 1) >> p.page_shift;
+    const T* const k_head = static_cast<const T*>(p.k_cache) + kv * head_stride;
+    const T* const v_head = static_cast<const T*>(p.v_cache) + kv * head_stride;
+
+    // which pages: lane i has entry `entry0 + i`
+    int entry0 = 0, page_at = -1, page_nth = 0;
+    const auto look_up = [&](int entry) {
+      entry0 = entry;
+      const int e = entry + lane;
+      page_at = -1;
+      page_nth = e;
+      if (e < (chunks + (1 << sub_shift) - 1) >> sub_shift) {
+        if (p.pages != nullptr) page_nth = p.pages[(static_cast<long long>(row) * p.kv_heads + kv) * p.count + e];
+        if (page_nth >= 0 && page_nth < held_pages) page_at = p.table[static_cast<long long>(row) * p.table_width + page_nth];
+        if (page_at >= p.num_pages) page_at = -1;
+      }
+    };
+    struct Chunk {
+      int valid;            // positions
+      long long k, v;       // elements from k_head, v_head
+    };
+    const auto locate = [&](int c) {
+      Chunk found{0, 0, 0};
+      if (c >= stop) return found;
+      const int e = c >> sub_shift, slot = (c & ((1 << sub_shift) - 1)) * kChunk;
+      if (e >= entry0 + 32) look_up(e);
+      const int where = __shfl_sync(0xffffffffu, page_at, e - entry0), nth = __shfl_sync(0xffffffffu, page_nth, e - entry0);
+      if (where >= 0) {
+        found.valid = max(0, min(kChunk, length - (nth << p.page_shift) - slot));
+        found.k = where * p.k_page + slot * p.dim;
+        found.v = where * p.v_page + slot * p.dim;
+      }
+      return found;
+    };
+    uint4 kr[2][PIECES][2], vr[4][PIECES];
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    const auto request_k = [&](const Chunk& c) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int t = g + 8 * r, d = i * 64 + h * 32 + q * 8;
+            kr[r][i][h] = none;
+            if (t < c.valid && d < p.dim) kr[r][i][h] = load_once(k_head + c.k + t * p.dim + d);
+          }
+    };
+    const auto request_v = [&](const Chunk& c) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+          const int t = 2 * q + (r & 1) + (r & 2) * 4, d = i * 64 + g * 8;
+          vr[r][i] = none;
+          if (t < c.valid && d < p.dim) vr[r][i] = load_once(v_head + c.v + t * p.dim + d);
+        }
+    };
+
+    uint4 qr[NT][PIECES][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int d = i * 64 + h * 32 + q * 8;
+          qr[n][i][h] = none;
+          if (n * 8 + g < here && d < p.dim)
+            qr[n][i][h] = load_once(static_cast<const T*>(p.q.data) + row * p.q.row + (head0 + n * 8 + g) * p.q.head + d);
+        }
+    float o[NT][PIECES][4][4], top[NT][2], sum[NT][2];
+    float* const scratch = parts_of_warps + (warp * 2 + 1) * kHeads * kPitch;  // the warp's last part is written last
+    // A rest of a weight that is 0 or below would turn an infinite element of v into NaN.  So where elements of the product
+    // come out not finite, it is formed a second time with all weights above zero as 1, and those elements are taken from there.
+    for (bool again = false;;) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        top[n][0] = top[n][1] = -INFINITY;
+        sum[n][0] = sum[n][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][i][j][e] = 0.f;
+      }
+      look_up(first >> sub_shift);
+      Chunk now = locate(first);
+      request_k(now);
+      request_v(now);
+      for (int c = first; c < stop; ++c) {
+        const Chunk next = locate(c + 1);
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+          for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint4 a = kr[0][i][h], b = kr[1][i][h], x = qr[n][i][h];
+              mma<T>(s[n], a.x, b.x, a.y, b.y, x.x, x.y);
+              mma<T>(s[n], a.z, b.z, a.w, b.w, x.z, x.w);
+            }
+        }
+        request_k(next);
+        uint32_t head[NT][2], rest[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          // s[e]: position g + (e & 2) * 4, query head 2 q + (e & 1)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] = g + (e & 2) * 4 < now.valid ? s[n][e] * p.scale_log2 : -INFINITY;
+          float old[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float high = fmaxf(top[n][e], max_over_positions(fmaxf(s[n][e], s[n][e + 2])));
+            const float base = high == -INFINITY ? 0.f : high;
+            old[e] = exp2f(top[n][e] - base);
+            top[n][e] = high;
+            s[n][e] = exp2f(s[n][e] - base + Half2<T>::kBias);
+            s[n][e + 2] = exp2f(s[n][e + 2] - base + Half2<T>::kBias);
+            sum[n][e] = sum[n][e] * old[e] + (s[n][e] + s[n][e + 2]);
+          }
+          if (__any_sync(0xffffffffu, old[0] != 1.f || old[1] != 1.f)) {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][i][j][e] *= old[e & 1];
+          }
+          if (again) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[n][e] = s[n][e] > 0.f ? 1.f : s[n][e];
+          }
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const uint32_t both = Half2<T>::pack(s[n][2 * t], s[n][2 * t + 1]);
+            const float2 kept = Half2<T>::unpack(both);
+            head[n][t] = transposed(both);
+            rest[n][t] = transposed(Half2<T>::pack(s[n][2 * t] - kept.x, s[n][2 * t + 1] - kept.y));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            // rows g and g + 8 of the instruction: elements 2 j and 2 j + 1 of the lanes' 8
+            const uint32_t v0 = word(vr[0][i], j), v1 = word(vr[1][i], j), v2 = word(vr[2][i], j), v3 = word(vr[3][i], j);
+            const uint32_t a0 = __byte_perm(v0, v1, 0x5410), a1 = __byte_perm(v0, v1, 0x7632);
+            const uint32_t a2 = __byte_perm(v2, v3, 0x5410), a3 = __byte_perm(v2, v3, 0x7632);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma<T>(o[n][i][j], a0, a1, a2, a3, head[n][0], head[n][1]);
+              if (!again) mma<T>(o[n][i][j], a0, a1, a2, a3, rest[n][0], rest[n][1]);
+            }
+          }
+        request_v(next);
+        now = next;
+      }
+      bool odd = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float& mine = o[n][i][j][e];
+              const int h = n * 8 + 2 * q + (e & 1);
+              float* const kept = scratch + h * kPitch + i * 64 + g * 8 + 2 * j + (e >> 1);
+              if (!again) {
+                odd |= h < here && !(fabsf(mine) < INFINITY);
+              } else if (fabsf(*kept) < INFINITY) {
+                mine = *kept;
+              }
+            }
+      if (again || !__any_sync(0xffffffffu, odd)) break;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              scratch[(n * 8 + 2 * q + (e & 1)) * kPitch + i * 64 + g * 8 + 2 * j + (e >> 1)] = o[n][i][j][e];
+      again = true;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) sum[n][e] = sum_over_positions(sum[n][e]);
+
+    if (first == 0 && stop == chunks) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int h = n * 8 + 2 * q + e;
+          const float factor = sum[n][e] == 0.f ? 0.f : 1.f / sum[n][e];
+          T* const to = static_cast<T*>(p.out) + (static_cast<long long>(row) * p.heads + head0 + h) * p.dim;
+#pragma unroll
+          for (int i = 0; i < PIECES; ++i) {
+            uint4 v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) word(v, j) = Half2<T>::pack(o[n][i][j][e] * factor, o[n][i][j][e + 2] * factor);
+            if (h < here && i * 64 + g * 8 < p.dim) *reinterpret_cast<uint4*>(to + i * 64 + g * 8) = v;
+          }
+        }
+    } else {
+      const int slot = first == 0 ? 1 : 0;
+      float* const to = parts_of_warps + (warp * 2 + slot) * kHeads * kPitch;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int h = n * 8 + 2 * q + e;
+#pragma unroll
+          for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<float2*>(to + h * kPitch + i * 64 + g * 8 + 2 * j) = make_float2(o[n][i][j][e], o[n][i][j][e + 2]);
+          if (g == 0) stats_of_warps[(warp * 2 + slot) * kHeads + h] = make_float2(top[n][e], sum[n][e]);
+        }
+      if (lane == 0) {
+        segment_of[warp][slot] = row * per_row + part_of_row;
+        if (slot == 0) ends[warp] = stop == chunks;
+        // the block whose warp has the segment's last chunk, at + chunks - 1
+        else last_block[warp] = static_cast<int>(((at + chunks) * workers - 1) / total / kWarps);
+      }
+    }
+    at += stop - first;
+    first = 0;
+    if (at < end && ++part_of_row == per_row) {
+      part_of_row = 0;
+      do chunks = chunks_of(p, ++row);
+      while (chunks == 0);
     }
   }
-  T* out = static_cast<T*>(p.out) + (static_cast<long long>(row) * p.heads + head) * p.dim;
-  for (int i = 0; i < 4; ++i)
-    if (lane + 32 * i < p.dim) out[lane + 32 * i] = rounded<T>(total == 0.f ? 0.f : acc[i] / total);
+  __syncthreads();
+  grid_launch_dependents();
+
+  // ---- parts of one segment that several warps have
+  int opened = -1, opened_until = 0;
+  for (int from = 0; from < 2 * kWarps;) {
+    const int segment = segment_of[from / 2][from % 2];
+    if (segment < 0) {
+      ++from;
+      continue;
+    }
+    int until = from + 1, last = from;  // parts [from, until) of the segment, some of them empty
+    for (; until < 2 * kWarps; ++until) {
+      const int other = segment_of[until / 2][until % 2];
+      if (other >= 0 && other != segment) break;
+      if (other >= 0) last = until;
+    }
+    const bool begins = from % 2 == 1, finished = last % 2 == 0 && ends[last / 2];
+    const int seg_row = segment / per_row, seg_part = segment - seg_row * per_row, kv = seg_part / p.parts;
+    const int head0 = kv * group + (seg_part - kv * p.parts) * kHeads, here = min(kHeads, (kv + 1) * group - head0);
+    const int vectors = p.dim / 4;
+    for (int x = threadIdx.x; x < here * vectors; x += kThreads) {
+      const int h = x / vectors, d = (x - h * vectors) * 4;
+      float high = -INFINITY;
+      for (int i = from; i <= last; ++i)
+        if (segment_of[i / 2][i % 2] >= 0) high = fmaxf(high, stats_of_warps[i * kHeads + h].x);
+      const float base = high == -INFINITY ? 0.f : high;
+      float sum = 0.f, o0 = 0.f, o1 = 0.f, o2 = 0.f, o3 = 0.f;
+      for (int i = from; i <= last; ++i) {
+        if (segment_of[i / 2][i % 2] < 0) continue;
+        const float2 s = stats_of_warps[i * kHeads + h];
+        const float weight = exp2f(s.x - base);
+        const float4 v = *reinterpret_cast<const float4*>(parts_of_warps + (i * kHeads + h) * kPitch + d);
+        sum += s.y * weight;
+        o0 += v.x * weight;
+        o1 += v.y * weight;
+        o2 += v.z * weight;
+        o3 += v.w * weight;
+      }
+      if (begins && finished) {
+        const float factor = sum == 0.f ? 0.f : 1.f / sum;
+        T* const to = static_cast<T*>(p.out) + (static_cast<long long>(seg_row) * p.heads + head0 + h) * p.dim + d;
+        *reinterpret_cast<uint2*>(to) = make_uint2(Half2<T>::pack(o0 * factor, o1 * factor), Half2<T>::pack(o2 * factor, o3 * factor));
+      } else {
+        const long long slot = (static_cast<long long>(blockIdx.x) * 2 + begins) * kHeads + h;
+        *reinterpret_cast<float4*>(p.product + slot * kDim + d) = make_float4(o0, o1, o2, o3);
+        if (d == 0) p.stats[slot] = make_float2(high, sum);
+      }
+    }
+    if (begins && !finished) {
+      opened = segment;
+      opened_until = last_block[from / 2];
+    }
+    from = until;
+  }
+  if (threadIdx.x == 0) p.open[blockIdx.x] = make_int2(opened, opened_until);
+}
+
+// A block for each query head of the segment that begins in block blockIdx.x of the kernel in front and ends in another.
+template <typename T, int PIECES, int NT>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ AttentionParams p) {
+  constexpr int kHeads = 8 * NT, kDim = 64 * PIECES, kJoinWarps = kJoinThreads / 32;
+  __shared__ float highs[kJoinWarps], sums[kJoinWarps];
+  __shared__ float4 products[kJoinWarps][32];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int2 open = p.open[blockIdx.x];
+  if (open.x < 0) return;
+  const int per_row = p.kv_heads * p.parts, group = p.heads / p.kv_heads, h = blockIdx.y;
+  const int row = open.x / per_row, part = open.x - row * per_row, kv = part / p.parts;
+  const int head0 = kv * group + (part - kv * p.parts) * kHeads;
+  if (head0 + h >= (kv + 1) * group) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = lane * 4;
+  const int n = open.y - static_cast<int>(blockIdx.x) + 1;
+  const auto slot = [&](int i) { return (static_cast<long long>(blockIdx.x + i) * 2 + (i == 0)) * kHeads + h; };
+  float high = -INFINITY;
+  for (int i = threadIdx.x; i < n; i += kJoinThreads) high = fmaxf(high, p.stats[slot(i)].x);
+  for (int s = 16; s > 0; s >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, s));
+  if (lane == 0) highs[warp] = high;
+  __syncthreads();
+  for (int w = 0; w < kJoinWarps; ++w) high = fmaxf(high, highs[w]);
+  const float base = high == -INFINITY ? 0.f : high;
+  float sum = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = warp; i < n; i += kJoinWarps) {
+    const float2 s = p.stats[slot(i)];
+    const float weight = exp2f(s.x - base);
+    sum += s.y * weight;
+    if (d < p.dim) {
+      const float4 v = *reinterpret_cast<const float4*>(p.product + slot(i) * kDim + d);
+      o.x += v.x * weight;
+      o.y += v.y * weight;
+      o.z += v.z * weight;
+      o.w += v.w * weight;
+    }
+  }
+  if (lane == 0) sums[warp] = sum;
+  products[warp][lane] = o;
+  __syncthreads();
+  if (warp != 0 || d >= p.dim) return;
+  for (int w = 1; w < kJoinWarps; ++w) {
+    const float4 v = products[w][lane];
+    sum += sums[w];
+    o.x += v.x;
+    o.y += v.y;
+    o.z += v.z;
+    o.w += v.w;
+  }
+  const float factor = sum == 0.f ? 0.f : 1.f / sum;
+  T* const to = static_cast<T*>(p.out) + (static_cast<long long>(row) * p.heads + head0 + h) * p.dim + d;
+  *reinterpret_cast<uint2*>(to) = make_uint2(Half2<T>::pack(o.x * factor, o.y * factor), Half2<T>::pack(o.z * factor, o.w * factor));
+}
+
+// Query heads of a segment: 8, or 16 where a key head has more than 8.
+int segment_heads(int heads, int kv_heads) { return heads / kv_heads > 8 ? 16 : 8; }
+
+size_t open_bytes() { return (kNumSMs * sizeof(int2) + 255) / 256 * 256; }
+size_t stats_bytes(int heads) { return static_cast<size_t>(kNumSMs) * 2 * heads * sizeof(float2); }
+size_t product_bytes(int heads, int head_dim) {
+  return static_cast<size_t>(kNumSMs) * 2 * heads * (head_dim > 64 ? 128 : 64) * sizeof(float);
+}
+
+template <typename T, int PIECES, int NT>
+int launch(const AttentionParams& p, int blocks, cudaStream_t stream) {
+  constexpr int kHeads = 8 * NT;
+  constexpr int smem = 2 * kWarps * kHeads * ((64 * PIECES + 4) * 4 + 8);
+  const auto kern = attention_kernel<T, PIECES, NT>;
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  const int st = launch_overlapped(kern, dim3(blocks), dim3(kThreads), smem, stream, p);
+  if (st != 0) return st;
+  return launch_overlapped(join_kernel<T, PIECES, NT>, dim3(blocks, std::min(kHeads, p.heads / p.kv_heads)), dim3(kJoinThreads), 0,
+                           stream, p);
+}
+
+template <typename T>
+int launch(const AttentionParams& p, int blocks, cudaStream_t stream) {
+  const bool wide = p.dim > 64, many = segment_heads(p.heads, p.kv_heads) > 8;
+  if (wide) return many ? launch<T, 2, 2>(p, blocks, stream) : launch<T, 2, 1>(p, blocks, stream);
+  return many ? launch<T, 1, 2>(p, blocks, stream) : launch<T, 1, 1>(p, blocks, stream);
 }
 
 }  // namespace
@@ -65,7 +575,12 @@ extern "C" int iex_paged_attention_supported(int heads, int kv_heads, int head_d
   return iex::paged::heads_ok(heads, kv_heads, head_dim) && iex::paged::page_size_ok(page_size) ? 1 : 0;
 }
 
-extern "C" size_t iex_paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim) { return 0; }
+extern "C" size_t iex_paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim) {
+  using namespace iex::paged;
+  if (rows <= 0 || !heads_ok(heads, kv_heads, head_dim)) return 0;
+  const int n = segment_heads(heads, kv_heads);
+  return open_bytes() + stats_bytes(n) + product_bytes(n, head_dim);
+}
 
 extern "C" int iex_paged_attention(int rows, int heads, int kv_heads, int head_dim, int bf16, const void* q, long long q_row,
                                    long long q_head, const void* k_cache, long long k_page, const void* v_cache,
@@ -79,8 +594,11 @@ extern "C" int iex_paged_attention(int rows, int heads, int kv_heads, int head_d
   if (!q || !out || !lengths || (table_width > 0 && !block_table) || (num_pages > 0 && (!k_cache || !v_cache)))
     return IEX_ERR_BAD_ARG;
   if (q_row % 8 != 0 || q_head % 8 != 0 || k_page % 8 != 0 || v_page % 8 != 0 || !iex::aligned16(q) || !iex::aligned16(out) ||
-      !iex::aligned16(k_cache) || !iex::aligned16(v_cache))
+      !iex::aligned16(k_cache) || !iex::aligned16(v_cache) || !iex::aligned16(workspace))
     return IEX_ERR_UNSUPPORTED;
+  if (static_cast<long long>(rows) * heads > 0x7fffffffll) return IEX_ERR_TOO_LARGE;
+  if (!workspace || workspace_bytes < iex_paged_attention_workspace_bytes(rows, heads, kv_heads, head_dim)) return IEX_ERR_BAD_ARG;
+  const int segment = segment_heads(heads, kv_heads);
   AttentionParams p{};
   p.rows = rows;
   p.heads = heads;
@@ -90,6 +608,7 @@ extern "C" int iex_paged_attention(int rows, int heads, int kv_heads, int head_d
   p.page_shift = log2_of(page_size);
   p.table_width = table_width;
   p.count = count;
+  p.parts = (heads / kv_heads + segment - 1) / segment;
   p.q = {q, q_row, q_head};
   p.k_cache = k_cache;
   p.v_cache = v_cache;
@@ -98,8 +617,16 @@ extern "C" int iex_paged_attention(int rows, int heads, int kv_heads, int head_d
   p.table = block_table;
   p.lengths = lengths;
   p.pages = pages;
-  p.scale = scale;
+  p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   p.out = out;
-  const auto kern = bf16 ? attention_kernel<__nv_bfloat16> : attention_kernel<__half>;
-  return iex::launch_overlapped(kern, dim3(rows * heads), dim3(32), 0, static_cast<cudaStream_t>(stream), p);
+  char* const ws = static_cast<char*>(workspace);
+  p.open = reinterpret_cast<int2*>(ws);
+  p.stats = reinterpret_cast<float2*>(ws + open_bytes());
+  p.product = reinterpret_cast<float*>(ws + open_bytes() + stats_bytes(segment));
+  // no more blocks than the longest rows could need
+  const double most = static_cast<double>(rows) * kv_heads * p.parts * (pages ? std::min(count, table_width) : table_width) *
+                      (page_size / kChunk);
+  const int blocks = static_cast<int>(std::min<double>(iex::kNumSMs, std::max(1.0, std::ceil(most / (kMinChunks * kWarps)))));
+  return bf16 ? launch<__nv_bfloat16>(p, blocks, static_cast<cudaStream_t>(stream))
+              : launch<__half>(p, blocks, static_cast<cudaStream_t>(stream));
 }
