@@ -5,9 +5,11 @@
 // with heads / kv_heads query heads to a key head, or over the positions of the pages that pages[r, kv_head] lists.  A segment is
 // what one row and one key head (up to 16 of its query heads) have to read, in chunks of 16 positions.  One to sixteen flops a byte: HBM bounds it.
 //
-// Work: the chunks of all segments, in order, are shared out evenly to the warps of one block per SM, whatever the rows'
-// lengths; a warp that has a whole segment writes its rows, the others leave maximum, sum and product, which the block joins through
-// shared memory and, where a segment reaches over several blocks, join_kernel joins from the workspace, in order.
+// Work, where segments are many or uneven (attention_kernel): the chunks of all segments, in order, are shared out evenly to the
+// warps of one block per SM, whatever the rows' lengths, a segment's start counted as kStart chunks; a warp that has a whole segment
+// writes its rows, the others leave maximum, sum and product, which the block joins through shared memory and, where a segment reaches over
+// several blocks, join_kernel joins from the workspace, in order.  Where there are few segments (cluster_kernel): a cluster of blocks for
+// each, joined through distributed shared memory, without workspace or second launch.
 //
 // A chunk: keys and values come straight from global memory into registers, 16 bytes a lane, the next chunk's keys requested
 // when this one's scores are formed and its values after the product; the lengths of what a warp has on its way (8 KB) and nothing else covers
@@ -22,20 +24,27 @@
 #include <algorithm>
 #include <cmath>
 
+#include <cooperative_groups.h>
+
 #include "paged.cuh"
 
 namespace iex {
 namespace paged {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = 32 * kWarps;
+namespace cg = cooperative_groups;
+
 constexpr int kChunk = 16;
-constexpr int kMinChunks = 2;  // of a warp: with less to do, fewer warps
+constexpr int kStart = 2;     // what a segment's start costs, in chunks
+constexpr int kMinUnits = 4;  // of a warp, starts included: with less to do, fewer warps
 constexpr int kJoinThreads = 128;
+constexpr int kClusterWarps = 8;
+constexpr int kMostBlocks = 8;  // of a cluster
 
 struct AttentionParams {
-  int rows, heads, kv_heads, dim, num_pages, page_shift, table_width, count, parts;  // parts: segments of a key head
+  int rows, heads, kv_heads, dim, num_pages, page_shift, table_width, count;
+  int parts;   // segments of a key head
+  int blocks;  // of a cluster, or 0
   Rows q;
   const void *k_cache, *v_cache;
   long long k_page, v_page;
@@ -116,73 +125,35 @@ __device__ __forceinline__ int chunks_of(const AttentionParams& p, int row) {
   return min(p.count, pages) << (p.page_shift - 4);
 }
 
-// PIECES: of 64 elements of a head; NT: groups of 8 query heads of a segment.
+// What a warp has of a segment: of its chunks [first, stop), for the 8 NT query heads from head0.
+//   PIECES: of 64 elements of a head; NT: groups of 8 query heads
 template <typename T, int PIECES, int NT>
-__global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ AttentionParams p) {
-  constexpr int kHeads = 8 * NT, kDim = 64 * PIECES, kPitch = kDim + 4;
-  extern __shared__ float parts_of_warps[];  // [warp][2][kHeads][kPitch], then [warp][2][kHeads] float2
-  __shared__ long long before[kThreads + 1];  // chunks (of one segment) of the rows in front of a thread's
-  __shared__ long long warp_sums[kWarps];
-  __shared__ int segment_of[kWarps][2], last_block[kWarps], ends[kWarps];
-  float2* const stats_of_warps = reinterpret_cast<float2*>(parts_of_warps + 2 * kWarps * kHeads * kPitch);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const int per_row = p.kv_heads * p.parts, group = p.heads / p.kv_heads, page = 1 << p.page_shift, sub_shift = p.page_shift - 4;
-  const long long head_stride = static_cast<long long>(page) * p.dim;
+struct Walk {
+  static constexpr int kHeads = 8 * NT, kDim = 64 * PIECES, kPitch = kDim + 4;
+  float o[NT][PIECES][4][4], top[NT][2], sum[NT][2];
 
-  grid_dependency_wait();
-  // ---- how the chunks are shared out
-  const int rows_each = (p.rows + kThreads - 1) / kThreads;
-  {
-    long long mine = 0;
-    for (int r = threadIdx.x * rows_each, i = 0; i < rows_each && r < p.rows; ++i, ++r) mine += chunks_of(p, r);
-    long long sum = mine;
-    for (int d = 1; d < 32; d <<= 1) {
-      const long long other = __shfl_up_sync(0xffffffffu, sum, d);
-      if (lane >= d) sum += other;
-    }
-    if (lane == 31) warp_sums[warp] = sum;
-    __syncthreads();
-    long long front = 0;
-    for (int w = 0; w < warp; ++w) front += warp_sums[w];
-    before[threadIdx.x] = front + sum - mine;
-    if (threadIdx.x == kThreads - 1) before[kThreads] = front + sum;
-    if (lane < 2) segment_of[warp][lane] = -1;
-    __syncthreads();
-  }
-  const long long total = before[kThreads] * per_row;
-  const long long workers = min(static_cast<long long>(gridDim.x) * kWarps, (total + kMinChunks - 1) / kMinChunks);
-  const long long worker = static_cast<long long>(blockIdx.x) * kWarps + warp;
-  const long long begin = worker < workers ? total * worker / workers : 0, end = worker < workers ? total * (worker + 1) / workers : 0;
-
-  // rows that hold nothing
-  for (int r = blockIdx.x; r < p.rows; r += gridDim.x)
-    if (chunks_of(p, r) == 0) {
-      uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + static_cast<long long>(r) * p.heads * p.dim);
-      for (int i = threadIdx.x; i < p.heads * p.dim / 8; i += kThreads) to[i] = make_uint4(0, 0, 0, 0);
-    }
-
-  // ---- the warp's own chunks
-  int row = 0, part_of_row = 0, chunks = 0, first = 0;  // the segment, its chunks, the first one that is this warp's
-  if (begin < end) {
-    int lo = 0, hi = kThreads;  // the last thread whose rows begin at or in front of `begin`
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (before[mid] * per_row <= begin) lo = mid; else hi = mid;
-    }
-    row = lo * rows_each;
-    long long rest = begin - before[lo] * per_row;
-    for (chunks = chunks_of(p, row); rest >= static_cast<long long>(chunks) * per_row; chunks = chunks_of(p, ++row))
-      rest -= static_cast<long long>(chunks) * per_row;
-    part_of_row = static_cast<int>(rest / chunks);
-    first = static_cast<int>(rest - static_cast<long long>(part_of_row) * chunks);
-  }
-  for (long long at = begin; at < end;) {
-    const int stop = static_cast<int>(min(static_cast<long long>(chunks), first + (end - at)));
-    const int kv = part_of_row / p.parts, head0 = kv * group + (part_of_row - kv * p.parts) * kHeads;
-    const int here = min(kHeads, (kv + 1) * group - head0);  // query heads
+  // `scratch`: kHeads x kPitch of shared memory that is this warp's; `here`: query heads that there are
+  __device__ __forceinline__ void run(const AttentionParams& p, int row, int kv, int head0, int here, int first, int stop, int chunks,
+                                      float* scratch) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3, page = 1 << p.page_shift, sub_shift = p.page_shift - 4;
+    const long long head_stride = static_cast<long long>(page) * p.dim;
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    uint4 qr[NT][PIECES][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int d = i * 64 + h * 32 + q * 8;
+          qr[n][i][h] = none;
+          if (n * 8 + g < here && d < p.dim)
+            qr[n][i][h] = load_once(static_cast<const T*>(p.q.data) + row * p.q.row + (head0 + n * 8 + g) * p.q.head + d);
+        }
     const int length = held(p.lengths, row, p.table_width, p.page_shift), held_pages = (length + page - 1) >> p.page_shift;
-    const T* const k_head = static_cast<const T*>(p.k_cache) + kv * head_stride;
-    const T* const v_head = static_cast<const T*>(p.v_cache) + kv * head_stride;
+    // a lane's places in a chunk
+    const T* const k_lane = static_cast<const T*>(p.k_cache) + kv * head_stride + g * p.dim + q * 8;
+    const T* const v_lane = static_cast<const T*>(p.v_cache) + kv * head_stride + 2 * q * p.dim + g * 8;
 
     // which pages: lane i has entry `entry0 + i`
     int entry0 = 0, page_at = -1, page_nth = 0;
@@ -198,8 +169,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       }
     };
     struct Chunk {
-      int valid;            // positions
-      long long k, v;       // elements from k_head, v_head
+      int valid;       // positions
+      long long k, v;  // elements from the lane's place in the first page
     };
     const auto locate = [&](int c) {
       Chunk found{0, 0, 0};
@@ -214,45 +185,42 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       }
       return found;
     };
+    // What lies behind the head's elements or the row's positions is zero and never read.
     uint4 kr[2][PIECES][2], vr[4][PIECES];
-    const uint4 none = make_uint4(0, 0, 0, 0);
+    const auto clear = [&](auto& regs) {
+#pragma unroll
+      for (auto& some : regs)
+#pragma unroll
+        for (auto& one : some) one = uint4{};
+    };
+    const auto clear_k = [&] {
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) kr[r][i][0] = kr[r][i][1] = none;
+    };
     const auto request_k = [&](const Chunk& c) {
+      if (c.valid < kChunk) clear_k();
 #pragma unroll
       for (int r = 0; r < 2; ++r)
 #pragma unroll
         for (int i = 0; i < PIECES; ++i)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int t = g + 8 * r, d = i * 64 + h * 32 + q * 8;
-            kr[r][i][h] = none;
-            if (t < c.valid && d < p.dim) kr[r][i][h] = load_once(k_head + c.k + t * p.dim + d);
-          }
+          for (int h = 0; h < 2; ++h)
+            if (g + 8 * r < c.valid && i * 64 + h * 32 + q * 8 < p.dim)
+              kr[r][i][h] = load_once(k_lane + c.k + 8 * r * p.dim + i * 64 + h * 32);
     };
     const auto request_v = [&](const Chunk& c) {
+      if (c.valid < kChunk) clear(vr);
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-          const int t = 2 * q + (r & 1) + (r & 2) * 4, d = i * 64 + g * 8;
-          vr[r][i] = none;
-          if (t < c.valid && d < p.dim) vr[r][i] = load_once(v_head + c.v + t * p.dim + d);
+          const int t = (r & 1) + (r & 2) * 4;
+          if (2 * q + t < c.valid && i * 64 + g * 8 < p.dim) vr[r][i] = load_once(v_lane + c.v + t * p.dim + i * 64);
         }
     };
 
-    uint4 qr[NT][PIECES][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int d = i * 64 + h * 32 + q * 8;
-          qr[n][i][h] = none;
-          if (n * 8 + g < here && d < p.dim)
-            qr[n][i][h] = load_once(static_cast<const T*>(p.q.data) + row * p.q.row + (head0 + n * 8 + g) * p.q.head + d);
-        }
-    float o[NT][PIECES][4][4], top[NT][2], sum[NT][2];
-    float* const scratch = parts_of_warps + (warp * 2 + 1) * kHeads * kPitch;  // the warp's last part is written last
     // A rest of a weight that is 0 or below would turn an infinite element of v into NaN.  So where elements of the product
     // come out not finite, it is formed a second time with all weights above zero as 1, and those elements are taken from there.
     for (bool again = false;;) {
@@ -267,10 +235,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[n][i][j][e] = 0.f;
       }
+      clear_k();
+      clear(vr);
       look_up(first >> sub_shift);
       Chunk now = locate(first);
       request_k(now);
       request_v(now);
+#pragma unroll 1
       for (int c = first; c < stop; ++c) {
         const Chunk next = locate(c + 1);
         float s[NT][4];
@@ -322,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             const uint32_t both = Half2<T>::pack(s[n][2 * t], s[n][2 * t + 1]);
             const float2 kept = Half2<T>::unpack(both);
             head[n][t] = transposed(both);
-            rest[n][t] = transposed(Half2<T>::pack(s[n][2 * t] - kept.x, s[n][2 * t + 1] - kept.y));
+            rest[n][t] = transposed(again ? 0 : Half2<T>::pack(s[n][2 * t] - kept.x, s[n][2 * t + 1] - kept.y));
           }
         }
 #pragma unroll
@@ -342,6 +313,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         request_v(next);
         now = next;
       }
+      if (again) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float before = scratch[(n * 8 + 2 * q + (e & 1)) * kPitch + i * 64 + g * 8 + 2 * j + (e >> 1)];
+                if (fabsf(before) < INFINITY) o[n][i][j][e] = before;
+              }
+        break;
+      }
       bool odd = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -350,73 +335,176 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float& mine = o[n][i][j][e];
-              const int h = n * 8 + 2 * q + (e & 1);
-              float* const kept = scratch + h * kPitch + i * 64 + g * 8 + 2 * j + (e >> 1);
-              if (!again) {
-                odd |= h < here && !(fabsf(mine) < INFINITY);
-              } else if (fabsf(*kept) < INFINITY) {
-                mine = *kept;
-              }
-            }
-      if (again || !__any_sync(0xffffffffu, odd)) break;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              scratch[(n * 8 + 2 * q + (e & 1)) * kPitch + i * 64 + g * 8 + 2 * j + (e >> 1)] = o[n][i][j][e];
+            for (int e = 0; e < 4; ++e) odd |= n * 8 + 2 * q + (e & 1) < here && !(fabsf(o[n][i][j][e]) < INFINITY);
+      if (!__any_sync(0xffffffffu, odd)) break;
+      keep(scratch);
       again = true;
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) sum[n][e] = sum_over_positions(sum[n][e]);
+  }
 
-    if (first == 0 && stop == chunks) {
+  // The product as it is, [kHeads][kPitch]; every lane writes what it alone reads again.
+  __device__ __forceinline__ void keep(float* to) const {
+    const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int h = n * 8 + 2 * q + e;
-          const float factor = sum[n][e] == 0.f ? 0.f : 1.f / sum[n][e];
-          T* const to = static_cast<T*>(p.out) + (static_cast<long long>(row) * p.heads + head0 + h) * p.dim;
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-          for (int i = 0; i < PIECES; ++i) {
-            uint4 v;
+        for (int i = 0; i < PIECES; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) word(v, j) = Half2<T>::pack(o[n][i][j][e] * factor, o[n][i][j][e + 2] * factor);
-            if (h < here && i * 64 + g * 8 < p.dim) *reinterpret_cast<uint4*>(to + i * 64 + g * 8) = v;
-          }
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<float2*>(to + (n * 8 + 2 * q + e) * kPitch + i * 64 + g * 8 + 2 * j) =
+                make_float2(o[n][i][j][e], o[n][i][j][e + 2]);
+  }
+  __device__ __forceinline__ void keep(float* to, float2* stats) const {
+    const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    keep(to);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (g == 0) stats[n * 8 + 2 * q + e] = make_float2(top[n][e], sum[n][e]);
+  }
+  __device__ __forceinline__ void write(const AttentionParams& p, int row, int head0, int here) const {
+    const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int h = n * 8 + 2 * q + e;
+        const float factor = sum[n][e] == 0.f ? 0.f : 1.f / sum[n][e];
+        T* const to = static_cast<T*>(p.out) + (static_cast<long long>(row) * p.heads + head0 + h) * p.dim;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+          uint4 v;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) word(v, j) = Half2<T>::pack(o[n][i][j][e] * factor, o[n][i][j][e + 2] * factor);
+          if (h < here && i * 64 + g * 8 < p.dim) *reinterpret_cast<uint4*>(to + i * 64 + g * 8) = v;
         }
-    } else {
-      const int slot = first == 0 ? 1 : 0;
-      float* const to = parts_of_warps + (warp * 2 + slot) * kHeads * kPitch;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int h = n * 8 + 2 * q + e;
-#pragma unroll
-          for (int i = 0; i < PIECES; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              *reinterpret_cast<float2*>(to + h * kPitch + i * 64 + g * 8 + 2 * j) = make_float2(o[n][i][j][e], o[n][i][j][e + 2]);
-          if (g == 0) stats_of_warps[(warp * 2 + slot) * kHeads + h] = make_float2(top[n][e], sum[n][e]);
+      }
+  }
+};
+
+// Four elements of the product, and the sum, of several parts of a segment.
+struct Joined {
+  float high, sum, o[4];
+};
+template <typename Stats, typename Product>
+__device__ __forceinline__ Joined join(int from, int until, Stats stats, Product product) {
+  Joined j{-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
+  for (int i = from; i < until; ++i) j.high = fmaxf(j.high, stats(i).x);
+  const float base = j.high == -INFINITY ? 0.f : j.high;
+  for (int i = from; i < until; ++i) {
+    const float2 s = stats(i);
+    const float4 v = product(i);
+    const float weight = exp2f(s.x - base);
+    j.sum += s.y * weight;
+    j.o[0] += v.x * weight;
+    j.o[1] += v.y * weight;
+    j.o[2] += v.z * weight;
+    j.o[3] += v.w * weight;
+  }
+  return j;
+}
+template <typename T>
+__device__ __forceinline__ void write4(const AttentionParams& p, int row, int head, int d, float sum, float o0, float o1, float o2,
+                                       float o3) {
+  const float factor = sum == 0.f ? 0.f : 1.f / sum;
+  T* const to = static_cast<T*>(p.out) + (static_cast<long long>(row) * p.heads + head) * p.dim + d;
+  *reinterpret_cast<uint2*>(to) = make_uint2(Half2<T>::pack(o0 * factor, o1 * factor), Half2<T>::pack(o2 * factor, o3 * factor));
+}
+
+// Warps of a block: as many as there are registers for.
+constexpr int warps_of(int pieces, int nt) { return pieces * nt == 1 ? 16 : pieces * nt == 2 ? 12 : 8; }
+
+template <typename T, int PIECES, int NT>
+__global__ void __launch_bounds__(32 * warps_of(PIECES, NT), 1) attention_kernel(const __grid_constant__ AttentionParams p) {
+  using W = Walk<T, PIECES, NT>;
+  constexpr int kHeads = W::kHeads, kDim = W::kDim, kPitch = W::kPitch, kWarps = warps_of(PIECES, NT), kThreads = 32 * kWarps;
+  extern __shared__ float parts_of_warps[];  // [warp][2][kHeads][kPitch], then [warp][2][kHeads] float2
+  __shared__ long long before[kThreads + 1];  // units (of one segment) of the rows in front of a thread's
+  __shared__ long long warp_sums[kWarps];
+  __shared__ int segment_of[kWarps][2], last_block[kWarps], ends[kWarps];
+  float2* const stats_of_warps = reinterpret_cast<float2*>(parts_of_warps + 2 * kWarps * kHeads * kPitch);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per_row = p.kv_heads * p.parts, group = p.heads / p.kv_heads;
+
+  grid_dependency_wait();
+  // ---- how the work is shared out: a segment is a unit for each chunk behind kStart units
+  const int rows_each = (p.rows + kThreads - 1) / kThreads;
+  const auto units_of = [&](int chunks) { return chunks == 0 ? 0 : chunks + kStart; };
+  {
+    long long mine = 0;
+    for (int r = threadIdx.x * rows_each, i = 0; i < rows_each && r < p.rows; ++i, ++r) mine += units_of(chunks_of(p, r));
+    long long sum = mine;
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long other = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += other;
+    }
+    if (lane == 31) warp_sums[warp] = sum;
+    __syncthreads();
+    long long front = 0;
+    for (int w = 0; w < warp; ++w) front += warp_sums[w];
+    before[threadIdx.x] = front + sum - mine;
+    if (threadIdx.x == kThreads - 1) before[kThreads] = front + sum;
+    if (lane < 2) segment_of[warp][lane] = -1;
+    __syncthreads();
+  }
+  const long long total = before[kThreads] * per_row;
+  const long long workers = min(static_cast<long long>(gridDim.x) * kWarps, (total + kMinUnits - 1) / kMinUnits);
+  const long long worker = static_cast<long long>(blockIdx.x) * kWarps + warp;
+  const long long begin = worker < workers ? total * worker / workers : 0, end = worker < workers ? total * (worker + 1) / workers : 0;
+
+  // rows that hold nothing
+  for (int r = blockIdx.x; r < p.rows; r += gridDim.x)
+    if (chunks_of(p, r) == 0) {
+      uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + static_cast<long long>(r) * p.heads * p.dim);
+      for (int i = threadIdx.x; i < p.heads * p.dim / 8; i += kThreads) to[i] = make_uint4(0, 0, 0, 0);
+    }
+
+  // ---- the warp's own part
+  int row = 0, part_of_row = 0, chunks = 0;  // the segment
+  long long at = begin, segment_begin = begin;
+  if (begin < end) {
+    int lo = 0, hi = kThreads;  // the last thread whose rows begin at or in front of `begin`
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (before[mid] * per_row <= begin) lo = mid; else hi = mid;
+    }
+    row = lo * rows_each;
+    long long rest = begin - before[lo] * per_row;
+    for (chunks = chunks_of(p, row); rest >= static_cast<long long>(units_of(chunks)) * per_row; chunks = chunks_of(p, ++row))
+      rest -= static_cast<long long>(units_of(chunks)) * per_row;
+    part_of_row = static_cast<int>(rest / units_of(chunks));
+    segment_begin = begin - (rest - static_cast<long long>(part_of_row) * units_of(chunks));
+  }
+  while (at < end) {
+    const int first = static_cast<int>(max(0ll, at - segment_begin - kStart));
+    const int stop = static_cast<int>(min(static_cast<long long>(chunks), max(0ll, end - segment_begin - kStart)));
+    if (first < stop) {
+      const int kv = part_of_row / p.parts, head0 = kv * group + (part_of_row - kv * p.parts) * kHeads;
+      const int here = min(kHeads, (kv + 1) * group - head0);  // query heads
+      W walk;
+      // the warp's last part is written last: its place is free until then
+      walk.run(p, row, kv, head0, here, first, stop, chunks, parts_of_warps + (warp * 2 + 1) * kHeads * kPitch);
+      if (first == 0 && stop == chunks) {
+        walk.write(p, row, head0, here);
+      } else {
+        const int slot = first == 0 ? 1 : 0;
+        walk.keep(parts_of_warps + (warp * 2 + slot) * kHeads * kPitch, stats_of_warps + (warp * 2 + slot) * kHeads);
+        if (lane == 0) {
+          segment_of[warp][slot] = row * per_row + part_of_row;
+          if (slot == 0) ends[warp] = stop == chunks;
+          // the block whose warp has the segment's last unit
+          else last_block[warp] = static_cast<int>(((segment_begin + units_of(chunks)) * workers - 1) / total / kWarps);
         }
-      if (lane == 0) {
-        segment_of[warp][slot] = row * per_row + part_of_row;
-        if (slot == 0) ends[warp] = stop == chunks;
-        // the block whose warp has the segment's last chunk, at + chunks - 1
-        else last_block[warp] = static_cast<int>(((at + chunks) * workers - 1) / total / kWarps);
       }
     }
-    at += stop - first;
-    first = 0;
+    at = segment_begin += units_of(chunks);
     if (at < end && ++part_of_row == per_row) {
       part_of_row = 0;
       do chunks = chunks_of(p, ++row);
@@ -434,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
       ++from;
       continue;
     }
-    int until = from + 1, last = from;  // parts [from, until) of the segment, some of them empty
+    int until = from + 1, last = from;  // parts [from, last] of the segment, some of them empty
     for (; until < 2 * kWarps; ++until) {
       const int other = segment_of[until / 2][until % 2];
       if (other >= 0 && other != segment) break;
@@ -446,30 +534,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     const int vectors = p.dim / 4;
     for (int x = threadIdx.x; x < here * vectors; x += kThreads) {
       const int h = x / vectors, d = (x - h * vectors) * 4;
-      float high = -INFINITY;
-      for (int i = from; i <= last; ++i)
-        if (segment_of[i / 2][i % 2] >= 0) high = fmaxf(high, stats_of_warps[i * kHeads + h].x);
-      const float base = high == -INFINITY ? 0.f : high;
-      float sum = 0.f, o0 = 0.f, o1 = 0.f, o2 = 0.f, o3 = 0.f;
-      for (int i = from; i <= last; ++i) {
-        if (segment_of[i / 2][i % 2] < 0) continue;
-        const float2 s = stats_of_warps[i * kHeads + h];
-        const float weight = exp2f(s.x - base);
-        const float4 v = *reinterpret_cast<const float4*>(parts_of_warps + (i * kHeads + h) * kPitch + d);
-        sum += s.y * weight;
-        o0 += v.x * weight;
-        o1 += v.y * weight;
-        o2 += v.z * weight;
-        o3 += v.w * weight;
-      }
+      const auto there = [&](int i) { return segment_of[i / 2][i % 2] >= 0; };
+      const Joined j = join(
+          from, last + 1, [&](int i) { return there(i) ? stats_of_warps[i * kHeads + h] : make_float2(-INFINITY, 0.f); },
+          [&](int i) {
+            return there(i) ? *reinterpret_cast<const float4*>(parts_of_warps + (i * kHeads + h) * kPitch + d) : float4{};
+          });
       if (begins && finished) {
-        const float factor = sum == 0.f ? 0.f : 1.f / sum;
-        T* const to = static_cast<T*>(p.out) + (static_cast<long long>(seg_row) * p.heads + head0 + h) * p.dim + d;
-        *reinterpret_cast<uint2*>(to) = make_uint2(Half2<T>::pack(o0 * factor, o1 * factor), Half2<T>::pack(o2 * factor, o3 * factor));
+        write4<T>(p, seg_row, head0 + h, d, j.sum, j.o[0], j.o[1], j.o[2], j.o[3]);
       } else {
         const long long slot = (static_cast<long long>(blockIdx.x) * 2 + begins) * kHeads + h;
-        *reinterpret_cast<float4*>(p.product + slot * kDim + d) = make_float4(o0, o1, o2, o3);
-        if (d == 0) p.stats[slot] = make_float2(high, sum);
+        *reinterpret_cast<float4*>(p.product + slot * kDim + d) = make_float4(j.o[0], j.o[1], j.o[2], j.o[3]);
+        if (d == 0) p.stats[slot] = make_float2(j.high, j.sum);
       }
     }
     if (begins && !finished) {
@@ -479,6 +555,68 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     from = until;
   }
   if (threadIdx.x == 0) p.open[blockIdx.x] = make_int2(opened, opened_until);
+}
+
+// A cluster of p.blocks blocks per segment.  Query head h of the segment is joined by block h % p.blocks, to which the others send what
+// they have of it.
+template <typename T, int PIECES, int NT>
+__global__ void __launch_bounds__(32 * kClusterWarps, 1) cluster_kernel(const __grid_constant__ AttentionParams p) {
+  using W = Walk<T, PIECES, NT>;
+  constexpr int kHeads = W::kHeads, kPitch = W::kPitch, kThreads = 32 * kClusterWarps;
+  extern __shared__ float parts_of_warps[];                       // [warp][kHeads][kPitch]
+  __shared__ float2 stats_of_warps[kClusterWarps][kHeads];
+  __shared__ alignas(16) float received[kHeads + kMostBlocks][kPitch];  // [block][head / blocks], (blocks - 1 places stay free)
+  __shared__ float2 received_stats[kHeads + kMostBlocks];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int warp = threadIdx.x >> 5, blocks = p.blocks, rank = blocks > 1 ? static_cast<int>(cluster.block_rank()) : 0;
+  const int per_row = p.kv_heads * p.parts, group = p.heads / p.kv_heads, segment = blockIdx.x / blocks;
+  const int row = segment / per_row, part = segment - row * per_row, kv = part / p.parts;
+  const int head0 = kv * group + (part - kv * p.parts) * kHeads, here = min(kHeads, (kv + 1) * group - head0);
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int chunks = chunks_of(p, row), vectors = p.dim / 4;
+  if (chunks == 0) {
+    for (int x = threadIdx.x; rank == 0 && x < here * vectors; x += kThreads)
+      write4<T>(p, row, head0 + x / vectors, x % vectors * 4, 0.f, 0.f, 0.f, 0.f, 0.f);
+    return;
+  }
+  if (blocks > 1) cluster.barrier_arrive();
+  // the warps of all blocks side by side, so that few chunks are spread over all of them
+  const int workers = min(chunks, blocks * kClusterWarps), worker = warp * blocks + rank;
+  if (worker < workers) {
+    W walk;
+    float* const mine = parts_of_warps + warp * kHeads * kPitch;
+    walk.run(p, row, kv, head0, here, static_cast<int>(static_cast<long long>(chunks) * worker / workers),
+             static_cast<int>(static_cast<long long>(chunks) * (worker + 1) / workers), chunks, mine);
+    walk.keep(mine, stats_of_warps[warp]);
+  }
+  __syncthreads();
+  const int working = workers > rank ? (workers - rank + blocks - 1) / blocks : 0;
+  const int heads_each = (kHeads + blocks - 1) / blocks;
+  if (blocks > 1) cluster.barrier_wait();  // the others have begun: their shared memory may be written
+  for (int x = threadIdx.x; x < here * vectors; x += kThreads) {
+    const int h = x / vectors, d = (x - h * vectors) * 4;
+    const Joined j = join(
+        0, working, [&](int i) { return stats_of_warps[i][h]; },
+        [&](int i) { return *reinterpret_cast<const float4*>(parts_of_warps + (i * kHeads + h) * kPitch + d); });
+    if (blocks == 1) {
+      write4<T>(p, row, head0 + h, d, j.sum, j.o[0], j.o[1], j.o[2], j.o[3]);
+    } else {
+      const int place = rank * heads_each + h / blocks, owner = h % blocks;
+      *cluster.map_shared_rank(reinterpret_cast<float4*>(&received[place][d]), owner) = make_float4(j.o[0], j.o[1], j.o[2], j.o[3]);
+      if (d == 0) *cluster.map_shared_rank(&received_stats[place], owner) = make_float2(j.high, j.sum);
+    }
+  }
+  if (blocks == 1) return;
+  cluster.sync();
+  for (int x = threadIdx.x; x < heads_each * vectors; x += kThreads) {
+    const int nth = x / vectors, h = nth * blocks + rank, d = (x - nth * vectors) * 4;
+    if (h >= here) break;
+    const Joined j = join(
+        0, blocks, [&](int i) { return received_stats[i * heads_each + nth]; },
+        [&](int i) { return *reinterpret_cast<const float4*>(&received[i * heads_each + nth][d]); });
+    write4<T>(p, row, head0 + h, d, j.sum, j.o[0], j.o[1], j.o[2], j.o[3]);
+  }
 }
 
 // A block for each query head of the segment that begins in block blockIdx.x of the kernel in front and ends in another.
@@ -531,9 +669,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     o.z += v.z;
     o.w += v.w;
   }
-  const float factor = sum == 0.f ? 0.f : 1.f / sum;
-  T* const to = static_cast<T*>(p.out) + (static_cast<long long>(row) * p.heads + head0 + h) * p.dim + d;
-  *reinterpret_cast<uint2*>(to) = make_uint2(Half2<T>::pack(o.x * factor, o.y * factor), Half2<T>::pack(o.z * factor, o.w * factor));
+  write4<T>(p, row, head0 + h, d, sum, o.x, o.y, o.z, o.w);
 }
 
 // Query heads of a segment: 8, or 16 where a key head has more than 8.
@@ -545,26 +681,71 @@ size_t product_bytes(int heads, int head_dim) {
   return static_cast<size_t>(kNumSMs) * 2 * heads * (head_dim > 64 ? 128 : 64) * sizeof(float);
 }
 
+// Blocks of a cluster for each segment, or 0 for attention_kernel; from the most that the rows could hold.
+//
+// A launch of attention_kernel, with join_kernel behind it, costs about kSaved us more than a cluster kernel's, which in turn leaves SMs
+// idle and is as uneven as the rows.
+int cluster_blocks(long long segments, long long most_chunks, int head_dim) {
+  constexpr double kSaved = 4.0, kRate = 6.5e6;  // bytes a us
+  if (segments > kNumSMs) return 0;
+  int blocks = 1;
+  while (blocks < kMostBlocks && segments * blocks * 2 <= kNumSMs && most_chunks > blocks * kClusterWarps) blocks *= 2;
+  const double us = segments * static_cast<double>(most_chunks) * kChunk * head_dim * 4 / kRate;
+  return us * (static_cast<double>(kNumSMs) / (segments * blocks) - 1.0) < kSaved ? blocks : 0;
+}
+
+template <typename Kernel>
+int allow_shared(Kernel kern, int smem) {
+  return smem > 40 * 1024 ? static_cast<int>(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) : 0;
+}
+
 template <typename T, int PIECES, int NT>
-int launch(const AttentionParams& p, int blocks, cudaStream_t stream) {
-  constexpr int kHeads = 8 * NT;
-  constexpr int smem = 2 * kWarps * kHeads * ((64 * PIECES + 4) * 4 + 8);
-  const auto kern = attention_kernel<T, PIECES, NT>;
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return static_cast<int>(e);
+int launch(const AttentionParams& p, double chunks, cudaStream_t stream) {
+  using W = Walk<T, PIECES, NT>;
+  if (p.blocks > 0) {
+    const auto kern = cluster_kernel<T, PIECES, NT>;
+    constexpr int smem = kClusterWarps * W::kHeads * W::kPitch * 4;
+    if (const int st = allow_shared(kern, smem)) return st;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.rows * p.kv_heads * p.parts * p.blocks);
+    cfg.blockDim = dim3(32 * kClusterWarps);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = p.blocks;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+    return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
   }
-  const int st = launch_overlapped(kern, dim3(blocks), dim3(kThreads), smem, stream, p);
-  if (st != 0) return st;
-  return launch_overlapped(join_kernel<T, PIECES, NT>, dim3(blocks, std::min(kHeads, p.heads / p.kv_heads)), dim3(kJoinThreads), 0,
+  constexpr int kWarps = warps_of(PIECES, NT), smem = 2 * kWarps * W::kHeads * (W::kPitch * 4 + 8);
+  const int blocks = static_cast<int>(std::min<double>(kNumSMs, std::max(1.0, std::ceil(chunks / (2 * kWarps)))));
+  const auto kern = attention_kernel<T, PIECES, NT>;
+  if (const int st = allow_shared(kern, smem)) return st;
+  if (const int st = launch_overlapped(kern, dim3(blocks), dim3(32 * kWarps), smem, stream, p)) return st;
+  return launch_overlapped(join_kernel<T, PIECES, NT>, dim3(blocks, std::min(W::kHeads, p.heads / p.kv_heads)), dim3(kJoinThreads), 0,
                            stream, p);
 }
 
 template <typename T>
-int launch(const AttentionParams& p, int blocks, cudaStream_t stream) {
+int launch(const AttentionParams& p, double chunks, cudaStream_t stream) {
   const bool wide = p.dim > 64, many = segment_heads(p.heads, p.kv_heads) > 8;
-  if (wide) return many ? launch<T, 2, 2>(p, blocks, stream) : launch<T, 2, 1>(p, blocks, stream);
-  return many ? launch<T, 1, 2>(p, blocks, stream) : launch<T, 1, 1>(p, blocks, stream);
+  if (wide) return many ? launch<T, 2, 2>(p, chunks, stream) : launch<T, 2, 1>(p, chunks, stream);
+  return many ? launch<T, 1, 2>(p, chunks, stream) : launch<T, 1, 1>(p, chunks, stream);
+}
+
+// Segments of a call, and the chunks that each could have.
+struct Extent {
+  long long segments, chunks;
+};
+Extent extent(int rows, int heads, int kv_heads, int page_size, int table_width, bool listed, int count) {
+  const int n = segment_heads(heads, kv_heads);
+  return {static_cast<long long>(rows) * kv_heads * ((heads / kv_heads + n - 1) / n),
+          static_cast<long long>(listed ? std::min(count, table_width) : table_width) * (page_size / kChunk)};
 }
 
 }  // namespace
@@ -575,9 +756,12 @@ extern "C" int iex_paged_attention_supported(int heads, int kv_heads, int head_d
   return iex::paged::heads_ok(heads, kv_heads, head_dim) && iex::paged::page_size_ok(page_size) ? 1 : 0;
 }
 
-extern "C" size_t iex_paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim) {
+extern "C" size_t iex_paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim, int page_size,
+                                                      int table_width, int listed, int count) {
   using namespace iex::paged;
-  if (rows <= 0 || !heads_ok(heads, kv_heads, head_dim)) return 0;
+  if (rows <= 0 || table_width < 0 || count < 0 || !iex_paged_attention_supported(heads, kv_heads, head_dim, page_size)) return 0;
+  const Extent e = extent(rows, heads, kv_heads, page_size, table_width, listed != 0, count);
+  if (cluster_blocks(e.segments, e.chunks, head_dim) > 0) return 0;
   const int n = segment_heads(heads, kv_heads);
   return open_bytes() + stats_bytes(n) + product_bytes(n, head_dim);
 }
@@ -597,8 +781,10 @@ extern "C" int iex_paged_attention(int rows, int heads, int kv_heads, int head_d
       !iex::aligned16(k_cache) || !iex::aligned16(v_cache) || !iex::aligned16(workspace))
     return IEX_ERR_UNSUPPORTED;
   if (static_cast<long long>(rows) * heads > 0x7fffffffll) return IEX_ERR_TOO_LARGE;
-  if (!workspace || workspace_bytes < iex_paged_attention_workspace_bytes(rows, heads, kv_heads, head_dim)) return IEX_ERR_BAD_ARG;
+  const size_t need = iex_paged_attention_workspace_bytes(rows, heads, kv_heads, head_dim, page_size, table_width, pages != nullptr, count);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return IEX_ERR_BAD_ARG;
   const int segment = segment_heads(heads, kv_heads);
+  const Extent e = extent(rows, heads, kv_heads, page_size, table_width, pages != nullptr, count);
   AttentionParams p{};
   p.rows = rows;
   p.heads = heads;
@@ -609,6 +795,7 @@ extern "C" int iex_paged_attention(int rows, int heads, int kv_heads, int head_d
   p.table_width = table_width;
   p.count = count;
   p.parts = (heads / kv_heads + segment - 1) / segment;
+  p.blocks = cluster_blocks(e.segments, e.chunks, head_dim);
   p.q = {q, q_row, q_head};
   p.k_cache = k_cache;
   p.v_cache = v_cache;
@@ -619,14 +806,13 @@ extern "C" int iex_paged_attention(int rows, int heads, int kv_heads, int head_d
   p.pages = pages;
   p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   p.out = out;
-  char* const ws = static_cast<char*>(workspace);
-  p.open = reinterpret_cast<int2*>(ws);
-  p.stats = reinterpret_cast<float2*>(ws + open_bytes());
-  p.product = reinterpret_cast<float*>(ws + open_bytes() + stats_bytes(segment));
-  // no more blocks than the longest rows could need
-  const double most = static_cast<double>(rows) * kv_heads * p.parts * (pages ? std::min(count, table_width) : table_width) *
-                      (page_size / kChunk);
-  const int blocks = static_cast<int>(std::min<double>(iex::kNumSMs, std::max(1.0, std::ceil(most / (kMinChunks * kWarps)))));
-  return bf16 ? launch<__nv_bfloat16>(p, blocks, static_cast<cudaStream_t>(stream))
-              : launch<__half>(p, blocks, static_cast<cudaStream_t>(stream));
+  if (need > 0) {
+    char* const ws = static_cast<char*>(workspace);
+    p.open = reinterpret_cast<int2*>(ws);
+    p.stats = reinterpret_cast<float2*>(ws + open_bytes());
+    p.product = reinterpret_cast<float*>(ws + open_bytes() + stats_bytes(segment));
+  }
+  const double chunks = static_cast<double>(e.segments) * static_cast<double>(e.chunks);
+  return bf16 ? launch<__nv_bfloat16>(p, chunks, static_cast<cudaStream_t>(stream))
+              : launch<__half>(p, chunks, static_cast<cudaStream_t>(stream));
 }

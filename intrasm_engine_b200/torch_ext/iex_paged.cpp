@@ -171,14 +171,16 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
   at::Tensor out = empty(q, {rows, heads, kc.dim});
   if (rows == 0) return out;
   const Operand qo(q);
-  const size_t bytes = iex_paged_attention_workspace_bytes(rows, heads, kc.kv_heads, kc.dim);
-  at::Tensor workspace = empty_bytes(q, std::max<size_t>(bytes, 16));
+  const size_t bytes = iex_paged_attention_workspace_bytes(rows, heads, kc.kv_heads, kc.dim, kc.page_size, block_table.size(1),
+                                                           pages.has_value(), count);
+  at::Tensor workspace;
+  if (bytes > 0) workspace = empty_bytes(q, bytes);
   // a list of no pages is a list all the same
   const int32_t* listed = pages.has_value() ? (count > 0 ? ints(*pages) : ints(lengths)) : nullptr;
   check_status(iex_paged_attention(rows, heads, kc.kv_heads, kc.dim, is_bf16(q), qo.t.data_ptr(), qo.row, qo.head,
                                    k_cache.data_ptr(), kc.page_stride, v_cache.data_ptr(), vc.page_stride, kc.pages,
                                    kc.page_size, ints(block_table), block_table.size(1), ints(lengths), listed, count,
-                                   static_cast<float>(factor), out.data_ptr(), workspace.data_ptr(), bytes, stream_of(q)),
+                                   static_cast<float>(factor), out.data_ptr(), bytes > 0 ? workspace.data_ptr() : nullptr, bytes, stream_of(q)),
                "iex_paged_attention");
   return out;
 }

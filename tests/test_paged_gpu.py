@@ -358,6 +358,21 @@ def test_append(lengths, new, heads, kv_heads, dim, page, rotary, interleaved, p
     assert torch.equal(again, got) and torch.equal(before[0], k_cache)
 
 
+def test_append_with_angles_off_16_bytes():
+    gen = torch.Generator().manual_seed(6)
+    k_cache, v_cache, table = U.make_cache(gen, [40], 2, 64, 16, F16, fill=0.0)
+    boxes = torch.zeros(k_cache.size(0), 2, 2, 64, dtype=F16, device=DEV)
+    cos, sin = paged.rope_table(40, 64, device=DEV)
+    room = torch.zeros(2 * 40 * 32 + 2, device=DEV)
+    off = [room[1:1 + 40 * 32].view(40, 32), room[2 + 40 * 32:2 + 80 * 32].view(40, 32)]
+    off[0].copy_(cos), off[1].copy_(sin)
+    q, k, v = (torch.randn(40, h, 64, generator=gen).half().to(DEV) for h in (4, 2, 2))
+    out = paged.paged_append(q, k, v, k_cache, v_cache, table, ints([40]), ints([0, 40]), rope=tuple(off), boxes=boxes)
+    kept = k_cache.clone(), boxes.clone()
+    ref = paged.paged_append(q, k, v, k_cache, v_cache, table, ints([40]), ints([0, 40]), rope=(cos, sin), boxes=boxes)
+    assert torch.equal(out, ref) and torch.equal(kept[0], k_cache) and torch.equal(kept[1], boxes)
+
+
 @pytest.mark.parametrize("dtype", U.DTYPES)
 def test_append_without_rotation_copies_bits(dtype):
     gen = torch.Generator().manual_seed(1)
