@@ -101,12 +101,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(v));
   return t;
 }
-// Read once by this SM; may have been written by the kernel in front (see linear_few.cu on loads that are not volatile).
-__device__ __forceinline__ uint4 load_once(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
-  return v;
-}
 __device__ __forceinline__ uint32_t& word(uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 __device__ __forceinline__ float max_over_positions(float v) {  // of the lanes with the same lane % 4
   for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
@@ -147,8 +141,8 @@ struct Walk {
         for (int h = 0; h < 2; ++h) {
           const int d = i * 64 + h * 32 + q * 8;
           qr[n][i][h] = none;
-          if (n * 8 + g < here && d < p.dim)
-            qr[n][i][h] = load_once(static_cast<const T*>(p.q.data) + row * p.q.row + (head0 + n * 8 + g) * p.q.head + d);
+          load_if(qr[n][i][h], static_cast<const T*>(p.q.data) + row * p.q.row + (head0 + n * 8 + g) * p.q.head + d,
+                  n * 8 + g < here && d < p.dim);
         }
     const int length = held(p.lengths, row, p.table_width, p.page_shift), held_pages = (length + page - 1) >> p.page_shift;
     // a lane's places in a chunk
@@ -207,8 +201,8 @@ struct Walk {
         for (int i = 0; i < PIECES; ++i)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            if (g + 8 * r < c.valid && i * 64 + h * 32 + q * 8 < p.dim)
-              kr[r][i][h] = load_once(k_lane + c.k + 8 * r * p.dim + i * 64 + h * 32);
+            load_once_if(kr[r][i][h], k_lane + c.k + 8 * r * p.dim + i * 64 + h * 32,
+                         g + 8 * r < c.valid && i * 64 + h * 32 + q * 8 < p.dim);
     };
     const auto request_v = [&](const Chunk& c) {
       if (c.valid < kChunk) clear(vr);
@@ -217,7 +211,7 @@ struct Walk {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
           const int t = (r & 1) + (r & 2) * 4;
-          if (2 * q + t < c.valid && i * 64 + g * 8 < p.dim) vr[r][i] = load_once(v_lane + c.v + t * p.dim + i * 64);
+          load_once_if(vr[r][i], v_lane + c.v + t * p.dim + i * 64, 2 * q + t < c.valid && i * 64 + g * 8 < p.dim);
         }
     };
 

@@ -5,8 +5,12 @@
 //   sum_g sum_d max(q[g, d] lo[d], q[g, d] hi[d]) = sum_d hi[d] sum_g max(q[g, d], 0) + lo[d] sum_g min(q[g, d], 0):
 //
 // two products a dimension however many query heads there are.  The `first` first and `last` last pages are always taken, then
-// those with the largest scores (NaN above all, ties to the lower page).  Scores are summed in 64 bits: which of two pages is
-// taken depends on their difference.  The terms of all pages are added in one order, so equal boxes have equal scores.
+// those with the largest scores (NaN above all, ties to the lower page).
+//
+// Which of two pages is taken depends on their scores' difference, so what counts is scores in 64 bits, whose terms are added in one order
+// for all pages (equal boxes have equal scores).  But converting a box to 64 bits takes longer than reading it: all pages are scored
+// in 32 bits with a bound on the error, the border between taken and not is found, and only where pages lie so near to it that their
+// scores in 32 bits do not tell are they scored again (any score that is not finite has all of them scored again).
 //
 // A cluster of blocks per row and key head: each scores a part of the pages (lanes side by side on a box, eight boxes in flight
 // a lane) and stores the scores, as whole numbers of the same order, in the first block's shared memory, which selects: 8 bits at
@@ -47,17 +51,21 @@ __device__ __forceinline__ Key ordered(double score) {
   return static_cast<Key>(bits) ^ (bits < 0 ? ~0ull : 1ull << 63);
 }
 
-__device__ __forceinline__ uint4 load_box(const void* p) {  // may have been written by the kernel in front
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
-  return v;
-}
-
 template <typename T>
 __device__ __forceinline__ void unpack(const uint4& v, float (&to)[8]) {
   const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
   for (int i = 0; i < 8; ++i) to[i] = as_float(e[i]);
+}
+
+// The larger of each of two elements without their signs.
+__device__ __forceinline__ uint32_t larger_size(uint32_t a, uint32_t b, __half) {
+  const __half2 v = __hmax2(reinterpret_cast<const __half2&>(a), __habs2(reinterpret_cast<const __half2&>(b)));
+  return reinterpret_cast<const uint32_t&>(v);
+}
+__device__ __forceinline__ uint32_t larger_size(uint32_t a, uint32_t b, __nv_bfloat16) {
+  const __nv_bfloat162 v = __hmax2(reinterpret_cast<const __nv_bfloat162&>(a), __habs2(reinterpret_cast<const __nv_bfloat162&>(b)));
+  return reinterpret_cast<const uint32_t&>(v);
 }
 
 // The sum of v over all threads in front of this one, and over all.
@@ -79,13 +87,162 @@ __device__ __forceinline__ uint2 scan(uint32_t v, uint32_t* warps) {
   return make_uint2(front + sum - v, all);
 }
 
+__device__ __forceinline__ double number(Key key) {  // the other way round, for numbers
+  return __longlong_as_double(static_cast<long long>(key >> 63 ? key ^ 1ull << 63 : ~key));
+}
+
+// The positive part, NaN if x is.  No branches in what follows: lanes would go their own ways element by element (weighing took 6000
+// cycles with them, 400 without).
+__device__ __forceinline__ float positive(float x) {
+  float v;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(x), "f"(0.f));
+  return v;
+}
+
+// What a lane's 8 elements of a box weigh: the sums of the query heads' positive (high) or negative parts.
+template <typename T, typename Number>
+__device__ __forceinline__ void weigh(const SelectParams& p, int row, int head0, int group, int d, bool high, bool mine,
+                                      Number (&weight)[8]) {
+  const float sign = high ? 1.f : -1.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) weight[i] = 0;
+  for (int g0 = 0; g0 < group; g0 += 4) {
+    uint4 some[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      some[g] = make_uint4(0, 0, 0, 0);
+      load_if(some[g], static_cast<const T*>(p.q.data) + row * p.q.row + (head0 + g0 + g) * p.q.head + d, mine && g0 + g < group);
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float x[8];
+      unpack<T>(some[g], x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) weight[i] += positive(sign * x[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) weight[i] *= sign;
+}
+
+// A lane's terms of kAhead boxes, added over the LANES lanes of a box: while a lane has several boxes, it gives half of them away and
+// adds the other lane's to its own.  Returns which of the boxes is left, in sum[0].
+template <int LANES, typename Number>
+__device__ __forceinline__ int add_up(Number (&sum)[kAhead]) {
+  const int lane = threadIdx.x & 31;
+  int width = kAhead, which = 0;
+#pragma unroll
+  for (int off = LANES / 2; off > 0; off >>= 1) {
+    if (width > 1) {
+      width >>= 1;
+      const bool upper = (lane & off) != 0;
+      which = which * 2 + upper;
+#pragma unroll
+      for (int u = 0; u < kAhead / 2; ++u) {
+        if (u >= width) break;
+        const Number give = upper ? sum[u] : sum[u + width];
+        const Number other = __shfl_xor_sync(0xffffffffu, give, off);
+        sum[u] = (upper ? sum[u + width] : sum[u]) + other;
+      }
+    } else {
+      sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], off);
+    }
+  }
+  return which;
+}
+
+// Where the taken pages begin: all those with keys >> shift above prefix, and `need` of those with it.
+struct Border {
+  Key prefix;
+  int shift;
+  uint32_t need;
+};
+
+__device__ __forceinline__ Key warp_max(Key v) {
+  const uint32_t high = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(v >> 32));
+  const uint32_t low = __reduce_max_sync(0xffffffffu, high == v >> 32 ? static_cast<uint32_t>(v) : 0u);
+  return static_cast<Key>(high) << 32 | low;
+}
+
+struct Shared {
+  alignas(16) uint32_t bins[3][kBins];
+  Key most[kWarps], least[kWarps];  // least: of the complements
+  uint32_t warps[kWarps];
+  uint32_t bound;  // the largest sum of a page's terms without their signs, as bits
+};
+
+// The border of the `need` largest of keys [from, to), which are more than that; called by all threads of the block.
+__device__ __forceinline__ Border find_border(const Key* keys, int from, int to, uint32_t need, Shared& sh) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Key most = 0, least = 0;
+  for (int i = from + threadIdx.x; i < to; i += kThreads) {
+    most = max(most, keys[i]);
+    least = max(least, ~keys[i]);
+  }
+  most = warp_max(most);
+  least = warp_max(least);
+  if (lane == 0) {
+    sh.most[warp] = most;
+    sh.least[warp] = least;
+  }
+  sh.bins[0][threadIdx.x] = 0;
+  __syncthreads();
+  for (int w = 0; w < kWarps; ++w) {
+    most = max(most, sh.most[w]);
+    least = max(least, sh.least[w]);
+  }
+  least = ~least;
+  if (need == 0) return {~0ull, 0, 0};
+  if (most == least) return {most, 0, need};
+  // Of the keys that begin with prefix (all bits from shift + bits up), the next `bits` bits are looked at.
+  int shift = max(0, 56 - __clzll(most ^ least)), bits = 8;
+  Key prefix = most >> shift >> 8;
+  for (int round = 0;; ++round) {
+    uint32_t* const bins = sh.bins[round % 3];
+    sh.bins[(round + 1) % 3][threadIdx.x] = 0;  // last read two rounds ago
+    for (int i = from + threadIdx.x; i < to; i += kThreads) {
+      const Key key = keys[i] >> shift;
+      if (key >> bits == prefix) atomicAdd(&bins[key & ((1u << bits) - 1)], 1u);
+    }
+    __syncthreads();
+    // every warp for itself: a lane has 8 bins, the first lane the highest
+    const uint4 upper = *reinterpret_cast<const uint4*>(bins + kBins - 4 - lane * 8);
+    const uint4 lower = *reinterpret_cast<const uint4*>(bins + kBins - 8 - lane * 8);
+    const uint32_t mine[8] = {upper.w, upper.z, upper.y, upper.x, lower.w, lower.z, lower.y, lower.x};
+    uint32_t here = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) here += mine[j];
+    uint32_t above = here;
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t other = __shfl_up_sync(0xffffffffu, above, d);
+      above += lane >= d ? other : 0;
+    }
+    above -= here;
+    const int owner = __ffs(__ballot_sync(0xffffffffu, (above < need) & (need <= above + here))) - 1;
+    uint32_t bin = 0, in_bin = 0, open = 1;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t hit = open & (need <= above + mine[j]);
+      bin += hit * (kBins - 1 - lane * 8 - j);
+      in_bin += hit * mine[j];
+      open -= hit;
+      above += open * mine[j];
+    }
+    bin = __shfl_sync(0xffffffffu, bin, owner);
+    in_bin = __shfl_sync(0xffffffffu, in_bin, owner);
+    need -= __shfl_sync(0xffffffffu, above, owner);
+    prefix = prefix << bits | bin;
+    if (shift == 0 || in_bin == need) return {prefix, shift, need};
+    bits = min(8, shift);
+    shift -= bits;
+  }
+}
+
 // LANES: side by side on a box, 8 elements each.
 template <typename T, int LANES>
 __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant__ SelectParams p) {
   extern __shared__ Key keys[];  // of all pages; the first block's are used
-  __shared__ uint32_t bins[kBins], warp_sums[kWarps];
-  __shared__ Key ends[2][kWarps];
-  __shared__ uint32_t found[2];
+  __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = cluster.num_blocks(), part = cluster.block_rank(), segment = blockIdx.x / parts;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -100,158 +257,163 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
       for (int i = threadIdx.x; i < p.count; i += kThreads) chosen[i] = i < pages ? i : -1;
     return;
   }
+  if (threadIdx.x == 0) sh.bound = 0;
+  if (parts > 1) cluster.barrier_arrive(); else __syncthreads();
   const int from = p.first, to = pages - p.last;  // those that are chosen by their scores
 
   // ---- scores
-  if (parts > 1) cluster.sync();  // the first block has begun: its shared memory may be written
-  Key* const shared_keys = parts > 1 ? cluster.map_shared_rank(keys, 0) : keys;
-  const int along = lane % LANES, side = lane / LANES;
-  const bool mine = along * 8 < 2 * p.dim, high = along * 8 >= p.dim;
-  const int d = along * 8 - (high ? p.dim : 0);
-  double weight[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) weight[i] = 0.0;
-  if (mine)
-    for (int g0 = 0; g0 < group; g0 += 4) {
-      uint4 some[4];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        some[g] = make_uint4(0, 0, 0, 0);
-        if (g0 + g < group)
-          some[g] = load_box(static_cast<const T*>(p.q.data) + row * p.q.row + (kv * group + g0 + g) * p.q.head + d);
-      }
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float x[8];
-        unpack<T>(some[g], x);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (high ? !(x[i] <= 0.f) : !(x[i] >= 0.f)) weight[i] += x[i];
-      }
-    }
   constexpr int kSides = 32 / LANES, kBatch = kAhead * kSides;  // pages of a warp's turn
+  const int along = lane % LANES, side = lane / LANES, d0 = along * 8;
+  const bool mine = d0 < 2 * p.dim, high = d0 >= p.dim;
+  const int d = d0 - (high ? p.dim : 0);
   const int32_t* const table = p.table + static_cast<long long>(row) * p.table_width;
-  const T* const boxes = static_cast<const T*>(p.boxes) + static_cast<long long>(kv) * 2 * p.dim + along * 8;
+  const T* const boxes = static_cast<const T*>(p.boxes) + static_cast<long long>(kv) * 2 * p.dim + d0;
   const long long box_stride = static_cast<long long>(p.kv_heads) * 2 * p.dim;
-  const int step = parts * kWarps * kBatch;
-  int base = from + (part * kWarps + warp) * kBatch;
-  int at = base + lane < to && lane < kBatch ? table[base + lane] : -1;
-  for (; base < to; base += step) {
-    uint4 box[kAhead];
+  const auto look_up = [&](int base) { return base + lane < to && lane < kBatch ? table[base + lane] : -1; };
+  const auto real = [&](int where) { return where >= 0 && where < p.num_pages; };
+  const auto request = [&](int at, uint4 (&box)[kAhead]) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int where = __shfl_sync(0xffffffffu, at, u * kSides + side);
       box[u] = make_uint4(0, 0, 0, 0);
-      if (mine && where >= 0 && where < p.num_pages) box[u] = load_box(boxes + where * box_stride);
+      load_once_if(box[u], boxes + where * box_stride, mine && real(where));
     }
-    const int here = at;
-    at = base + step + lane < to && lane < kBatch ? table[base + step + lane] : -1;
-    double sum[kAhead];
+  };
+  const bool holder = along % (LANES / kAhead) == 0;  // one lane for each box that is added up
+  {
+    const int step = parts * kWarps * kBatch;
+    int base = from + (part * kWarps + warp) * kBatch;
+    int at = look_up(base);
+    float weight[8];
+    uint4 largest = make_uint4(0, 0, 0, 0);  // of the lane's elements of all boxes, without their signs
+    bool finite = true;
+    weigh<T>(p, row, kv * group, group, d, high, mine, weight);
+    Key* const shared_keys = parts > 1 ? cluster.map_shared_rank(keys, 0) : keys;
+    bool waited = parts == 1;
+    for (; base < to; base += step) {
+      uint4 box[kAhead];
+      request(at, box);
+      const int here = at;
+      at = look_up(base + step);
+      float sum[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      float x[8];
-      unpack<T>(box[u], x);
-      sum[u] = 0.0;
+      for (int u = 0; u < kAhead; ++u) {
+        float x[8];
+        unpack<T>(box[u], x);
+        float2 two = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum[u] = fma(static_cast<double>(x[i]), weight[i], sum[u]);
-    }
-    // over the lanes of a box: while a lane has several boxes, it gives half of them away and adds the other lane's to its own
-    int width = kAhead, which = 0;
-#pragma unroll
-    for (int off = LANES / 2; off > 0; off >>= 1) {
-      if (width > 1) {
-        width >>= 1;
-        const bool upper = (lane & off) != 0;
-        which = which * 2 + upper;
-#pragma unroll
-        for (int u = 0; u < kAhead / 2; ++u) {
-          if (u >= width) break;
-          const double give = upper ? sum[u] : sum[u + width];
-          const double other = __shfl_xor_sync(0xffffffffu, give, off);
-          sum[u] = (upper ? sum[u + width] : sum[u]) + other;
-        }
-      } else {
-        sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], off);
+        for (int i = 0; i < 4; ++i)
+          two = ffma2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(weight[2 * i], weight[2 * i + 1]), two);
+        sum[u] = two.x + two.y;
+        largest.x = larger_size(largest.x, box[u].x, T());
+        largest.y = larger_size(largest.y, box[u].y, T());
+        largest.z = larger_size(largest.z, box[u].z, T());
+        largest.w = larger_size(largest.w, box[u].w, T());
       }
+      const int nth = add_up<LANES>(sum) * kSides + side, where = __shfl_sync(0xffffffffu, here, nth);
+      if (!waited) {  // the first block has begun: its shared memory may be written
+        cluster.barrier_wait();
+        waited = true;
+      }
+      if (holder && base + nth < to) {
+        shared_keys[base + nth] = real(where) ? ordered(static_cast<double>(sum[0])) : 0;
+      }
+      finite &= fabsf(sum[0]) < INFINITY;
     }
-    // LANES >= 8: one box is left
-    const int nth = which * kSides + side, where = __shfl_sync(0xffffffffu, here, nth);
-    if (along % (LANES / kAhead) == 0 && base + nth < to)
-      shared_keys[base + nth] = where >= 0 && where < p.num_pages ? ordered(sum[0]) : 0;
+    if (!waited) cluster.barrier_wait();
+    // A sum of the largest elements' terms is no less than that of any page's.
+    float x[8], most = 0.f;
+    unpack<T>(largest, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = fmaf(x[i], fabsf(weight[i]), most);
+    if (!finite) most = INFINITY;
+    for (int off = LANES / 2; off > 0; off >>= 1) most += __shfl_xor_sync(0xffffffffu, most, off);
+    const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+    if (lane == 0) atomicMax(parts > 1 ? cluster.map_shared_rank(&sh.bound, 0) : &sh.bound, bits);  // NaN is above infinity
   }
   if (parts > 1) cluster.sync(); else __syncthreads();
   if (part != 0) return;
 
-  // ---- the smallest score that is taken
-  uint32_t need = p.count - p.first - p.last;  // of the pages [from, to), of which there are more
-  Key most = 0, least = ~0ull;
-  for (int i = from + threadIdx.x; i < to; i += kThreads) {
-    most = max(most, keys[i]);
-    least = min(least, keys[i]);
-  }
-  for (int off = 16; off > 0; off >>= 1) {
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
-    least = min(least, __shfl_xor_sync(0xffffffffu, least, off));
-  }
-  if (lane == 0) {
-    ends[0][warp] = most;
-    ends[1][warp] = least;
-  }
-  __syncthreads();
-  for (int w = 0; w < kWarps; ++w) {
-    most = max(most, ends[0][w]);
-    least = min(least, ends[1][w]);
-  }
-  // Of the keys that begin with `prefix` (all bits from shift + bits up), the next `bits` bits are looked at.
-  int shift = most == least ? 0 : max(0, 56 - __clzll(most ^ least)), bits = 8;
-  Key prefix = most >> shift >> 8;
-  bool settled = false;  // of the keys whose bits from `shift` up are `prefix`, the first `need` are taken
-  if (most == least || need == 0) {
-    settled = true;
-    shift = 0;
-    prefix = need == 0 ? ~0ull : most;
-  }
-  while (!settled) {
-    bins[threadIdx.x] = 0;
-    __syncthreads();
+  // ---- where the taken ones begin, and the pages that are too near to it
+  const uint32_t wanted = p.count - p.first - p.last;  // of the pages [from, to), of which there are more
+  Border border = find_border(keys, from, to, wanted, sh);
+  if (wanted > 0) {
+    // Off by at most: a rounding for each of a lane's 4 products and sums, one for their sum, 5 over lanes and one for every query head,
+    // relative to the terms without their signs; and products below the smallest numbers.
+    const float bound = __uint_as_float(sh.bound);
+    const double error = bound * (group + 16.0) * 0x1p-24 + 1e-40;
+    const Key lowest = border.prefix << border.shift, highest = lowest | ((1ull << border.shift) - 1);
+    const Key minus = ordered(-INFINITY);
+    const double low = lowest <= minus ? -INFINITY : number(lowest) - 2 * error;
+    const double top = highest <= minus ? -INFINITY : highest >= ordered(INFINITY) ? INFINITY : number(highest) + 2 * error;
+    const bool all = !(bound < INFINITY);
+    // 0 not taken, 1 near, 2 taken
+    const auto side_of = [&](Key key) {
+      if (all) return 1;
+      const double score = key == 0 ? -INFINITY : number(key);
+      return key != 0 && score > top ? 2 : score >= low ? 1 : 0;
+    };
+    uint32_t counts = 0;
     for (int i = from + threadIdx.x; i < to; i += kThreads) {
-      const Key key = keys[i] >> shift;
-      if (key >> bits == prefix) atomicAdd(&bins[key & ((1u << bits) - 1)], 1u);
+      const int side_here = side_of(keys[i]);
+      counts += side_here == 2 ? 1u << 16 : side_here;
     }
-    __syncthreads();
-    const int bin = kBins - 1 - threadIdx.x;  // threads from the highest bin down
-    const uint32_t in_bin = bins[bin], above = scan(in_bin, warp_sums).x;
-    if (above < need && need <= above + in_bin) {
-      found[0] = bin;
-      found[1] = above;
-    }
-    __syncthreads();
-    prefix = prefix << bits | found[0];
-    need -= found[1];
-    settled = shift == 0 || bins[found[0]] == need;
-    if (!settled) {
-      bits = min(8, shift);
-      shift -= bits;
+    const uint32_t sums = scan(counts, sh.warps).y, near = sums & 0xffffu, taken = sums >> 16;
+    if (near + taken == wanted) {
+      // all that are near are taken: above the lowest of them nothing is left out
+      for (int i = from + threadIdx.x; i < to; i += kThreads) keys[i] = side_of(keys[i]) > 0 ? 1 : 0;
+      border = {0, 0, 0};
+    } else {
+      double weight[8];
+      weigh<T>(p, row, kv * group, group, d, high, mine, weight);
+      for (int base = from + warp * kBatch; base < to; base += kWarps * kBatch) {
+        const bool inside = lane < kBatch && base + lane < to;
+        const Key old = inside ? keys[base + lane] : 0;
+        const int side_here = inside ? side_of(old) : 0;
+        Key key = side_here == 2 ? ~0ull : 0;
+        if (__any_sync(0xffffffffu, side_here == 1)) {
+          const int at = look_up(base);
+          uint4 box[kAhead];
+          request(at, box);
+          double sum[kAhead];
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            float x[8];
+            unpack<T>(box[u], x);
+            sum[u] = 0.0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[u] = fma(static_cast<double>(x[i]), weight[i], sum[u]);
+          }
+          const int nth = add_up<LANES>(sum) * kSides + side, where = __shfl_sync(0xffffffffu, at, nth);
+          const int side_there = __shfl_sync(0xffffffffu, side_here, nth);
+          if (holder && base + nth < to && side_there == 1) keys[base + nth] = real(where) ? ordered(sum[0]) : 0;
+        }
+        __syncwarp();
+        if (inside && side_here != 1) keys[base + lane] = key;
+      }
+      __syncthreads();
+      border = find_border(keys, from, to, wanted, sh);
     }
     __syncthreads();
   }
 
   // ---- the chosen pages in order: every thread a run of them
   const int each = (pages + kThreads - 1) / kThreads, begin = threadIdx.x * each, end = min(pages, begin + each);
-  const auto above = [&](int i) { return i < from || i >= to || keys[i] >> shift > prefix; };
-  const auto equal = [&](int i) { return i >= from && i < to && keys[i] >> shift == prefix; };
-  uint32_t counts = 0;  // above in the lower half, equal in the upper one
-  for (int i = begin; i < end; ++i) counts += above(i) ? 1u : equal(i) ? 1u << 16 : 0u;
-  const uint32_t front = scan(counts, warp_sums).x;
+  // above in the lower half, equal in the upper one; keys outside [from, to) are whatever they are
+  const auto kind = [&](int i) {
+    const Key key = keys[i] >> border.shift;
+    const bool forced = (i < from) | (i >= to);
+    return forced | (key > border.prefix) ? 1u : key == border.prefix ? 1u << 16 : 0u;
+  };
+  uint32_t counts = 0;
+  for (int i = begin; i < end; ++i) counts += kind(i);
+  const uint32_t front = scan(counts, sh.warps).x;
   uint32_t higher = front & 0xffffu, same = front >> 16;
   for (int i = begin; i < end; ++i) {
-    if (above(i)) {
-      chosen[higher + min(same, need)] = i;
-      ++higher;
-    } else if (equal(i)) {
-      if (same < need) chosen[higher + same] = i;
-      ++same;
-    }
+    const uint32_t here = kind(i), is_above = here & 1u, is_equal = here >> 16;
+    if (is_above | (is_equal & (same < border.need))) chosen[higher + min(same, border.need)] = i;
+    higher += is_above;
+    same += is_equal;
   }
 }
 
