@@ -34,6 +34,11 @@ __device__ __forceinline__ int held(const int32_t* lengths, int row, int table_w
   return length <= 0 ? 0 : static_cast<int>(length < most ? length : most);
 }
 
+// This block has begun, and so have the others of its cluster: from then on their shared memory may be written.  Nothing that was
+// written before is seen by them (ordering that takes half a microsecond).
+__device__ __forceinline__ void cluster_begun() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait_begun() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // A matrix of rows and heads whose innermost dimension is contiguous, in elements.
 struct Rows {
   const void* data;

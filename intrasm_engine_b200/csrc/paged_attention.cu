@@ -329,7 +329,7 @@ struct Walk {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) odd |= n * 8 + 2 * q + (e & 1) < here && !(fabsf(o[n][i][j][e]) < INFINITY);
+            for (int e = 0; e < 4; ++e) odd |= (n * 8 + 2 * q + (e & 1) < here) & !(fabsf(o[n][i][j][e]) < INFINITY);
       if (!__any_sync(0xffffffffu, odd)) break;
       keep(scratch);
       again = true;
@@ -574,7 +574,7 @@ __global__ void __launch_bounds__(32 * kClusterWarps, 1) cluster_kernel(const __
       write4<T>(p, row, head0 + x / vectors, x % vectors * 4, 0.f, 0.f, 0.f, 0.f, 0.f);
     return;
   }
-  if (blocks > 1) cluster.barrier_arrive();
+  if (blocks > 1) cluster_begun();
   // the warps of all blocks side by side, so that few chunks are spread over all of them
   const int workers = min(chunks, blocks * kClusterWarps), worker = warp * blocks + rank;
   if (worker < workers) {
@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(32 * kClusterWarps, 1) cluster_kernel(const __
   __syncthreads();
   const int working = workers > rank ? (workers - rank + blocks - 1) / blocks : 0;
   const int heads_each = (kHeads + blocks - 1) / blocks;
-  if (blocks > 1) cluster.barrier_wait();  // the others have begun: their shared memory may be written
+  if (blocks > 1) cluster_wait_begun();
   for (int x = threadIdx.x; x < here * vectors; x += kThreads) {
     const int h = x / vectors, d = (x - h * vectors) * 4;
     const Joined j = join(

@@ -33,6 +33,8 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kAhead = 8;         // boxes that a lane has on their way
 constexpr int kMaxPages = 16384;  // keys of 8 bytes in shared memory
 constexpr int kBins = 256;
+constexpr int kMostBlocks = 8;  // of a cluster
+static_assert(kThreads == kBins, "a thread clears a bin");
 
 struct SelectParams {
   int rows, heads, kv_heads, dim, num_pages, page_shift, table_width, count, first, last;
@@ -68,23 +70,25 @@ __device__ __forceinline__ uint32_t larger_size(uint32_t a, uint32_t b, __nv_bfl
   return reinterpret_cast<const uint32_t&>(v);
 }
 
-// The sum of v over all threads in front of this one, and over all.
-__device__ __forceinline__ uint2 scan(uint32_t v, uint32_t* warps) {
+// The sum of v over all threads in front of this one.  `warps` has not been read since the last barrier.
+__device__ __forceinline__ uint32_t sum_in_front(uint32_t v, uint32_t* warps) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t sum = v;
   for (int d = 1; d < 32; d <<= 1) {
     const uint32_t other = __shfl_up_sync(0xffffffffu, sum, d);
-    if (lane >= d) sum += other;
+    sum += lane >= d ? other : 0;
   }
-  __syncthreads();
   if (lane == 31) warps[warp] = sum;
   __syncthreads();
-  uint32_t front = 0, all = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) front += warps[w];
-    all += warps[w];
-  }
-  return make_uint2(front + sum - v, all);
+  return sum - v + __reduce_add_sync(0xffffffffu, lane < warp ? warps[lane] : 0);
+}
+// The sum of v over all threads, likewise.
+__device__ __forceinline__ uint32_t sum_of_all(uint32_t v, uint32_t* warps) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t sum = __reduce_add_sync(0xffffffffu, v);
+  if (lane == 0) warps[warp] = sum;
+  __syncthreads();
+  return __reduce_add_sync(0xffffffffu, lane < kWarps ? warps[lane] : 0);
 }
 
 __device__ __forceinline__ double number(Key key) {  // the other way round, for numbers
@@ -151,91 +155,64 @@ __device__ __forceinline__ int add_up(Number (&sum)[kAhead]) {
   return which;
 }
 
-// Where the taken pages begin: all those with keys >> shift above prefix, and `need` of those with it.
+// Where the taken pages begin: all those with keys above `high`, and the first `need` of those with keys from `low` to `high`.
 struct Border {
-  Key prefix;
-  int shift;
+  Key low, high;
   uint32_t need;
 };
 
-__device__ __forceinline__ Key warp_max(Key v) {
-  const uint32_t high = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(v >> 32));
-  const uint32_t low = __reduce_max_sync(0xffffffffu, high == v >> 32 ? static_cast<uint32_t>(v) : 0u);
-  return static_cast<Key>(high) << 32 | low;
-}
-
 struct Shared {
   alignas(16) uint32_t bins[3][kBins];
-  Key most[kWarps], least[kWarps];  // least: of the complements
-  uint32_t warps[kWarps];
-  uint32_t bound;  // the largest sum of a page's terms without their signs, as bits
+  // of every warp of the cluster: the most that a page's terms without their signs add up to, as bits; upper halves of keys
+  uint32_t bound[kMostBlocks * kWarps], most[kMostBlocks * kWarps], least[kMostBlocks * kWarps];
+  uint32_t warps[2][kWarps];
 };
 
-// The border of the `need` largest of keys [from, to), which are more than that; called by all threads of the block.
-__device__ __forceinline__ Border find_border(const Key* keys, int from, int to, uint32_t need, Shared& sh) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  Key most = 0, least = 0;
-  for (int i = from + threadIdx.x; i < to; i += kThreads) {
-    most = max(most, keys[i]);
-    least = max(least, ~keys[i]);
-  }
-  most = warp_max(most);
-  least = warp_max(least);
-  if (lane == 0) {
-    sh.most[warp] = most;
-    sh.least[warp] = least;
-  }
-  sh.bins[0][threadIdx.x] = 0;
-  __syncthreads();
-  for (int w = 0; w < kWarps; ++w) {
-    most = max(most, sh.most[w]);
-    least = max(least, sh.least[w]);
-  }
-  least = ~least;
-  if (need == 0) return {~0ull, 0, 0};
-  if (most == least) return {most, 0, need};
-  // Of the keys that begin with prefix (all bits from shift + bits up), the next `bits` bits are looked at.
-  int shift = max(0, 56 - __clzll(most ^ least)), bits = 8;
-  Key prefix = most >> shift >> 8;
-  for (int round = 0;; ++round) {
+// The border of the `need` largest of keys [from, to), which are more than that and lie from `least` to `most`; called by all
+// threads of the block, with bins[0] cleared.
+__device__ __forceinline__ Border find_border(const Key* keys, int from, int to, Key least, Key most, uint32_t need, Shared& sh) {
+  const int lane = threadIdx.x & 31;
+  if (need == 0) return {~0ull, ~0ull, 0};
+  for (int round = 0; least != most; ++round) {
+    const Key span = most - least;
+    const int shift = max(0, 56 - __clzll(span));  // span >> shift is below 256
     uint32_t* const bins = sh.bins[round % 3];
     sh.bins[(round + 1) % 3][threadIdx.x] = 0;  // last read two rounds ago
     for (int i = from + threadIdx.x; i < to; i += kThreads) {
-      const Key key = keys[i] >> shift;
-      if (key >> bits == prefix) atomicAdd(&bins[key & ((1u << bits) - 1)], 1u);
+      const Key place = keys[i] - least;
+      if (place <= span) atomicAdd(&bins[place >> shift], 1u);
     }
     __syncthreads();
     // every warp for itself: a lane has 8 bins, the first lane the highest
     const uint4 upper = *reinterpret_cast<const uint4*>(bins + kBins - 4 - lane * 8);
     const uint4 lower = *reinterpret_cast<const uint4*>(bins + kBins - 8 - lane * 8);
-    const uint32_t mine[8] = {upper.w, upper.z, upper.y, upper.x, lower.w, lower.z, lower.y, lower.x};
-    uint32_t here = 0;
+    uint32_t sums[8] = {upper.w, upper.z, upper.y, upper.x, lower.w, lower.z, lower.y, lower.x};  // of bins from the highest down
 #pragma unroll
-    for (int j = 0; j < 8; ++j) here += mine[j];
-    uint32_t above = here;
+    for (int j = 1; j < 8; ++j) sums[j] += sums[j - 1];
+    uint32_t above = sums[7];
     for (int d = 1; d < 32; d <<= 1) {
       const uint32_t other = __shfl_up_sync(0xffffffffu, above, d);
       above += lane >= d ? other : 0;
     }
-    above -= here;
-    const int owner = __ffs(__ballot_sync(0xffffffffu, (above < need) & (need <= above + here))) - 1;
-    uint32_t bin = 0, in_bin = 0, open = 1;
+    above -= sums[7];
+    const int owner = __ffs(__ballot_sync(0xffffffffu, (above < need) & (need <= above + sums[7]))) - 1;
+    const uint32_t rest = need - above;  // in the owner: of its bins' keys
+    uint32_t nth = 0, front = 0, through = 0xffffffffu;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint32_t hit = open & (need <= above + mine[j]);
-      bin += hit * (kBins - 1 - lane * 8 - j);
-      in_bin += hit * mine[j];
-      open -= hit;
-      above += open * mine[j];
+      const bool before = sums[j] < rest;
+      nth += before;
+      front = before ? sums[j] : front;
+      through = min(through, before ? 0xffffffffu : sums[j]);
     }
-    bin = __shfl_sync(0xffffffffu, bin, owner);
-    in_bin = __shfl_sync(0xffffffffu, in_bin, owner);
-    need -= __shfl_sync(0xffffffffu, above, owner);
-    prefix = prefix << bits | bin;
-    if (shift == 0 || in_bin == need) return {prefix, shift, need};
-    bits = min(8, shift);
-    shift -= bits;
+    const uint32_t bin = __shfl_sync(0xffffffffu, kBins - 1 - lane * 8 - nth, owner);
+    const uint32_t in_bin = __shfl_sync(0xffffffffu, through - front, owner);
+    need = __shfl_sync(0xffffffffu, rest - front, owner);
+    least += static_cast<Key>(bin) << shift;
+    most = min(most, least + ((1ull << shift) - 1));
+    if (in_bin == need) break;
   }
+  return {least, most, need};
 }
 
 // LANES: side by side on a box, 8 elements each.
@@ -257,15 +234,14 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
       for (int i = threadIdx.x; i < p.count; i += kThreads) chosen[i] = i < pages ? i : -1;
     return;
   }
-  if (threadIdx.x == 0) sh.bound = 0;
-  if (parts > 1) cluster.barrier_arrive(); else __syncthreads();
+  if (parts > 1) cluster_begun();
   const int from = p.first, to = pages - p.last;  // those that are chosen by their scores
 
   // ---- scores
   constexpr int kSides = 32 / LANES, kBatch = kAhead * kSides;  // pages of a warp's turn
   const int along = lane % LANES, side = lane / LANES, d0 = along * 8;
-  const bool mine = d0 < 2 * p.dim, high = d0 >= p.dim;
-  const int d = d0 - (high ? p.dim : 0);
+  const bool mine = d0 < 2 * p.dim, upper = d0 >= p.dim;  // upper: of the largest keys
+  const int d = d0 - (upper ? p.dim : 0);
   const int32_t* const table = p.table + static_cast<long long>(row) * p.table_width;
   const T* const boxes = static_cast<const T*>(p.boxes) + static_cast<long long>(kv) * 2 * p.dim + d0;
   const long long box_stride = static_cast<long long>(p.kv_heads) * 2 * p.dim;
@@ -287,7 +263,8 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
     float weight[8];
     uint4 largest = make_uint4(0, 0, 0, 0);  // of the lane's elements of all boxes, without their signs
     bool finite = true;
-    weigh<T>(p, row, kv * group, group, d, high, mine, weight);
+    uint32_t key_most = 0, key_least = ~0u;  // upper halves
+    weigh<T>(p, row, kv * group, group, d, upper, mine, weight);
     Key* const shared_keys = parts > 1 ? cluster.map_shared_rank(keys, 0) : keys;
     bool waited = parts == 1;
     for (; base < to; base += step) {
@@ -311,16 +288,18 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
         largest.w = larger_size(largest.w, box[u].w, T());
       }
       const int nth = add_up<LANES>(sum) * kSides + side, where = __shfl_sync(0xffffffffu, here, nth);
-      if (!waited) {  // the first block has begun: its shared memory may be written
-        cluster.barrier_wait();
+      if (!waited) {
+        cluster_wait_begun();
         waited = true;
       }
-      if (holder && base + nth < to) {
-        shared_keys[base + nth] = real(where) ? ordered(static_cast<double>(sum[0])) : 0;
-      }
+      const Key key = real(where) ? ordered(static_cast<double>(sum[0])) : 0;
+      const bool there = holder & (base + nth < to);
+      if (there) shared_keys[base + nth] = key;
+      key_most = max(key_most, there ? static_cast<uint32_t>(key >> 32) : 0u);
+      key_least = min(key_least, there ? static_cast<uint32_t>(key >> 32) : ~0u);
       finite &= fabsf(sum[0]) < INFINITY;
     }
-    if (!waited) cluster.barrier_wait();
+    if (!waited) cluster_wait_begun();
     // A sum of the largest elements' terms is no less than that of any page's.
     float x[8], most = 0.f;
     unpack<T>(largest, x);
@@ -328,50 +307,53 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
     for (int i = 0; i < 8; ++i) most = fmaf(x[i], fabsf(weight[i]), most);
     if (!finite) most = INFINITY;
     for (int off = LANES / 2; off > 0; off >>= 1) most += __shfl_xor_sync(0xffffffffu, most, off);
-    const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
-    if (lane == 0) atomicMax(parts > 1 ? cluster.map_shared_rank(&sh.bound, 0) : &sh.bound, bits);  // NaN is above infinity
+    const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most));  // NaN is above infinity
+    key_most = __reduce_max_sync(0xffffffffu, key_most);
+    key_least = __reduce_min_sync(0xffffffffu, key_least);
+    if (lane == 0) {
+      Shared& first = parts > 1 ? *cluster.map_shared_rank(&sh, 0) : sh;
+      first.bound[part * kWarps + warp] = bits;
+      first.most[part * kWarps + warp] = key_most;
+      first.least[part * kWarps + warp] = key_least;
+    }
+    if (part == 0) sh.bins[0][threadIdx.x] = 0;
   }
   if (parts > 1) cluster.sync(); else __syncthreads();
   if (part != 0) return;
 
   // ---- where the taken ones begin, and the pages that are too near to it
   const uint32_t wanted = p.count - p.first - p.last;  // of the pages [from, to), of which there are more
-  Border border = find_border(keys, from, to, wanted, sh);
+  uint32_t key_most = 0, key_least = ~0u, bound_bits = 0;
+  for (int w = lane; w < parts * kWarps; w += 32) {
+    key_most = max(key_most, sh.most[w]);
+    key_least = min(key_least, sh.least[w]);
+    bound_bits = max(bound_bits, sh.bound[w]);
+  }
+  key_most = __reduce_max_sync(0xffffffffu, key_most);
+  key_least = __reduce_min_sync(0xffffffffu, key_least);
+  const float bound = __uint_as_float(__reduce_max_sync(0xffffffffu, bound_bits));
+  Border border = find_border(keys, from, to, static_cast<Key>(key_least) << 32, static_cast<Key>(key_most) << 32 | 0xffffffffu, wanted, sh);
   if (wanted > 0) {
     // Off by at most: a rounding for each of a lane's 4 products and sums, one for their sum, 5 over lanes and one for every query head,
     // relative to the terms without their signs; and products below the smallest numbers.
-    const float bound = __uint_as_float(sh.bound);
     const double error = bound * (group + 16.0) * 0x1p-24 + 1e-40;
-    const Key lowest = border.prefix << border.shift, highest = lowest | ((1ull << border.shift) - 1);
-    const Key minus = ordered(-INFINITY);
-    const double low = lowest <= minus ? -INFINITY : number(lowest) - 2 * error;
-    const double top = highest <= minus ? -INFINITY : highest >= ordered(INFINITY) ? INFINITY : number(highest) + 2 * error;
-    const bool all = !(bound < INFINITY);
-    // 0 not taken, 1 near, 2 taken
-    const auto side_of = [&](Key key) {
-      if (all) return 1;
-      const double score = key == 0 ? -INFINITY : number(key);
-      return key != 0 && score > top ? 2 : score >= low ? 1 : 0;
-    };
+    const Key minus = ordered(-INFINITY), plus = ordered(INFINITY);  // keys below are pages that are not the cache's
+    Key low = border.low <= minus ? 0 : ordered(number(border.low) - 2 * error);
+    Key high = border.high <= minus ? minus : border.high >= plus ? ~0ull : ordered(number(border.high) + 2 * error);
+    if (!(bound < INFINITY)) low = 0, high = ~0ull;
+    // keys above `high` are taken, those from `low` on near or taken
     uint32_t counts = 0;
-    for (int i = from + threadIdx.x; i < to; i += kThreads) {
-      const int side_here = side_of(keys[i]);
-      counts += side_here == 2 ? 1u << 16 : side_here;
-    }
-    const uint32_t sums = scan(counts, sh.warps).y, near = sums & 0xffffu, taken = sums >> 16;
-    if (near + taken == wanted) {
-      // all that are near are taken: above the lowest of them nothing is left out
-      for (int i = from + threadIdx.x; i < to; i += kThreads) keys[i] = side_of(keys[i]) > 0 ? 1 : 0;
-      border = {0, 0, 0};
-    } else {
+    for (int i = from + threadIdx.x; i < to; i += kThreads) counts += keys[i] >= low ? 1u : 0u;
+    counts = sum_of_all(counts, sh.warps[0]);
+    border = {low, ~0ull, wanted};  // if all that are near are taken
+    if (counts != wanted) {
       double weight[8];
-      weigh<T>(p, row, kv * group, group, d, high, mine, weight);
+      weigh<T>(p, row, kv * group, group, d, upper, mine, weight);
       for (int base = from + warp * kBatch; base < to; base += kWarps * kBatch) {
         const bool inside = lane < kBatch && base + lane < to;
         const Key old = inside ? keys[base + lane] : 0;
-        const int side_here = inside ? side_of(old) : 0;
-        Key key = side_here == 2 ? ~0ull : 0;
-        if (__any_sync(0xffffffffu, side_here == 1)) {
+        const bool near = inside & (old >= low) & (old <= high);
+        if (__any_sync(0xffffffffu, near)) {
           const int at = look_up(base);
           uint4 box[kAhead];
           request(at, box);
@@ -385,29 +367,28 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
             for (int i = 0; i < 8; ++i) sum[u] = fma(static_cast<double>(x[i]), weight[i], sum[u]);
           }
           const int nth = add_up<LANES>(sum) * kSides + side, where = __shfl_sync(0xffffffffu, at, nth);
-          const int side_there = __shfl_sync(0xffffffffu, side_here, nth);
-          if (holder && base + nth < to && side_there == 1) keys[base + nth] = real(where) ? ordered(sum[0]) : 0;
+          const bool near_there = __shfl_sync(0xffffffffu, near, nth);
+          if (holder && base + nth < to && near_there) keys[base + nth] = real(where) ? ordered(sum[0]) : 0;
         }
-        __syncwarp();
-        if (inside && side_here != 1) keys[base + lane] = key;
+        if (inside && !near) keys[base + lane] = old > high ? ~0ull : 0;
       }
+      sh.bins[0][threadIdx.x] = 0;
       __syncthreads();
-      border = find_border(keys, from, to, wanted, sh);
+      border = find_border(keys, from, to, 0, ~0ull, wanted, sh);
     }
-    __syncthreads();
   }
 
   // ---- the chosen pages in order: every thread a run of them
   const int each = (pages + kThreads - 1) / kThreads, begin = threadIdx.x * each, end = min(pages, begin + each);
   // above in the lower half, equal in the upper one; keys outside [from, to) are whatever they are
   const auto kind = [&](int i) {
-    const Key key = keys[i] >> border.shift;
+    const Key key = keys[i];
     const bool forced = (i < from) | (i >= to);
-    return forced | (key > border.prefix) ? 1u : key == border.prefix ? 1u << 16 : 0u;
+    return forced | (key > border.high) ? 1u : key >= border.low ? 1u << 16 : 0u;
   };
   uint32_t counts = 0;
   for (int i = begin; i < end; ++i) counts += kind(i);
-  const uint32_t front = scan(counts, sh.warps).x;
+  const uint32_t front = sum_in_front(counts, sh.warps[1]);
   uint32_t higher = front & 0xffffu, same = front >> 16;
   for (int i = begin; i < end; ++i) {
     const uint32_t here = kind(i), is_above = here & 1u, is_equal = here >> 16;
@@ -428,7 +409,7 @@ int launch(const SelectParams& p, cudaStream_t stream) {
   // two blocks an SM, but a warp's turn of pages for every warp
   const long long segments = static_cast<long long>(p.rows) * p.kv_heads;
   int parts = 1;
-  while (parts < 8 && segments * parts * 2 <= 2 * kNumSMs && p.table_width >= parts * 2 * kWarps * kAhead / 2) parts *= 2;
+  while (parts < kMostBlocks && segments * parts * 2 <= 2 * kNumSMs && p.table_width >= parts * 2 * kWarps * kAhead / 2) parts *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(segments * parts));
   cfg.blockDim = dim3(kThreads);
