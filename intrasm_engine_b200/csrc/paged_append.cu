@@ -7,9 +7,9 @@
 // in fp32, and rounded once.  boxes (optional) holds the smallest and largest key of every page and head in each dimension: of a
 // page that is written to they are formed anew from all its positions up to the last new one.
 //
-// A block does one page's new tokens of one key head and its query heads, so that a box has one writer.  A thread's item is 16
-// bytes, or the two 16-byte pieces that are turned into each other; keys are done with a fixed piece of the head to a thread,
-// which keeps the smallest and largest of its own, and meet those of the positions that the page held before in shared memory.
+// A block does one page's new tokens of one key head and its query heads, so that a box has one writer; with many tokens the query
+// heads have blocks of their own.  An item is 16 bytes, or the two 16-byte pieces that are turned into each other.  What the
+// page held before is requested ahead of all else; new keys pass through shared memory on their way into the box.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -19,6 +19,9 @@ namespace paged {
 namespace {
 
 constexpr int kThreads = 128;
+constexpr int kWarps = kThreads / 32;
+constexpr int kKept = 32;       // new keys that are kept in shared memory: of pages with more of them the box reads the cache
+constexpr int kQueryHeads = 2;  // of a block that has nothing but query heads
 
 enum Turn {
   kHalves,    // pairs (i, i + rotary / 2), rotary a multiple of 16: two pieces of 8 elements at once
@@ -73,17 +76,6 @@ __device__ __forceinline__ uint4 load16(const void* p) {
   return v;
 }
 
-// Where the tokens of sequence i begin among the rows.
-__device__ __forceinline__ int begin_of(const AppendParams& p, int i) {
-  return p.cu_tokens ? min(max(p.cu_tokens[i], 0), p.tokens) : i;
-}
-
-// Blocks are laid out by what a sequence needs at most: the n tokens of a sequence touch up to n / page + 2 pages, and
-// floor(begin / page) + 2 i blocks are enough for all the sequences in front.
-__device__ __forceinline__ int first_block(const AppendParams& p, int i) {
-  return p.cu_tokens ? (begin_of(p, i) >> p.page_shift) + 2 * i : i;
-}
-
 __device__ __forceinline__ float turned(float a, float b, float c, float s) { return fmaf(a, c, b * s); }
 
 // Items of a head's row: pieces that are turned, then pieces that are copied.
@@ -99,6 +91,9 @@ template <typename T, Turn kTurn>
 struct Item {
   uint4 a, b;  // the piece, or both (kElements: one element each)
   float c[kTurn == kHalves ? 8 : kTurn == kNeighbors ? 4 : 1], s[kTurn == kHalves ? 8 : kTurn == kNeighbors ? 4 : 1];
+
+  __device__ __forceinline__ void load_copy(const T* from, int item) { a = load16(from + item * 8); }
+  __device__ __forceinline__ void store_copy(T* to, int item) const { *reinterpret_cast<uint4*>(to + item * 8) = a; }
 
   // Item `item` of the row at `from`; the angles of its position at cos and sin.
   __device__ __forceinline__ void load(const AppendParams& p, const T* from, const float* cos, const float* sin, int item) {
@@ -122,11 +117,11 @@ struct Item {
     } else if constexpr (kTurn == kNeighbors) {
       a = load16(from + item * 8);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (item * 4 + i < half) {
-          c[i] = cos[item * 4 + i];
-          s[i] = sin[item * 4 + i];
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int pair = min(item * 4 + i, max(half - 1, 0));
+        c[i] = half > 0 ? cos[pair] : 1.f;
+        s[i] = half > 0 ? sin[pair] : 0.f;
+      }
     } else {
       T *x = reinterpret_cast<T*>(&a), *y = reinterpret_cast<T*>(&b);
       if (item < half) {
@@ -140,23 +135,20 @@ struct Item {
     }
   }
 
-  // Turned, to the row at `to`; a and b are what is written.
-  __device__ __forceinline__ void store(const AppendParams& p, T* to, int item) {
+  __device__ __forceinline__ void turn(const AppendParams& p, int item) {
     const int half = p.rotary / 2;
     T *x = reinterpret_cast<T*>(&a), *y = reinterpret_cast<T*>(&b);
     if constexpr (kTurn == kNeighbors) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (item * 4 + i < half) {
-          const float one = as_float(x[2 * i]), two = as_float(x[2 * i + 1]);
-          x[2 * i] = rounded<T>(turned(one, two, c[i], -s[i]));
-          x[2 * i + 1] = rounded<T>(turned(two, one, c[i], s[i]));
-        }
-      *reinterpret_cast<uint4*>(to + item * 8) = a;
+      for (int i = 0; i < 4; ++i) {
+        const float one = as_float(x[2 * i]), two = as_float(x[2 * i + 1]);
+        const bool turns = item * 4 + i < half;
+        x[2 * i] = turns ? rounded<T>(turned(one, two, c[i], -s[i])) : x[2 * i];
+        x[2 * i + 1] = turns ? rounded<T>(turned(two, one, c[i], s[i])) : x[2 * i + 1];
+      }
     } else {
       constexpr int kElementsOf = kTurn == kHalves ? 8 : 1;
-      const bool turns = item < half / kElementsOf;
-      if (turns) {
+      if (item < half / kElementsOf) {
 #pragma unroll
         for (int i = 0; i < kElementsOf; ++i) {
           const float one = as_float(x[i]), two = as_float(y[i]);
@@ -164,201 +156,224 @@ struct Item {
           y[i] = rounded<T>(turned(two, one, c[i], s[i]));
         }
       }
+    }
+  }
+
+  // To the row at `to`.
+  __device__ __forceinline__ void store(const AppendParams& p, T* to, int item) const {
+    const int half = p.rotary / 2;
+    if constexpr (kTurn == kNeighbors) {
+      *reinterpret_cast<uint4*>(to + item * 8) = a;
+    } else {
+      constexpr int kElementsOf = kTurn == kHalves ? 8 : 1;
+      const bool turns = item < half / kElementsOf;
       T* const first = turns ? to + item * kElementsOf : to + p.rotary + (item - half / kElementsOf) * kElementsOf;
       if constexpr (kTurn == kHalves) {
         *reinterpret_cast<uint4*>(first) = a;
         if (turns) *reinterpret_cast<uint4*>(first + half) = b;
       } else {
-        *first = x[0];
-        if (turns) first[half] = y[0];
+        *first = *reinterpret_cast<const T*>(&a);
+        if (turns) first[half] = *reinterpret_cast<const T*>(&b);
       }
     }
   }
 };
 
+// The new tokens that a block has.
+struct Span {
+  int sequence, begin, n, length, nth;  // nth: of the pages that the sequence's new tokens touch
+};
+
+// Blocks in a row have the pages of one sequence after the other: n new tokens touch up to (n + page - 2) / page + 1 of them.
+// False where there is no such block.
+__device__ __forceinline__ bool find_span(const AppendParams& p, int block, Span& found) {
+  __shared__ Span shared;
+  __shared__ int sums[kWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (p.cu_tokens == nullptr) {
+    if (block >= p.batch) return false;
+    found = {block, block, 1, p.lengths[block], 0};
+    return true;
+  }
+  int front = 0;
+  for (int s0 = 0; s0 < p.batch; s0 += kThreads) {
+    const int s = s0 + threadIdx.x;
+    int begin = 0, n = 0, length = 0;
+    if (s < p.batch) {
+      begin = min(max(p.cu_tokens[s], 0), p.tokens);
+      n = max(0, min(max(p.cu_tokens[s + 1], 0), p.tokens) - begin);
+      length = p.lengths[s];
+    }
+    const int mine = n > 0 ? ((n + (1 << p.page_shift) - 2) >> p.page_shift) + 1 : 0;
+    int sum = mine;
+    for (int d = 1; d < 32; d <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, sum, d);
+      sum += lane >= d ? other : 0;
+    }
+    if (lane == 31) sums[warp] = sum;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      sum += w < warp ? sums[w] : 0;
+      all += sums[w];
+    }
+    const int first = front + sum - mine;
+    if (first <= block && block < first + mine) shared = {s, begin, n, length, block - first};
+    front += all;
+    __syncthreads();
+    if (block < front) {
+      found = shared;
+      return true;
+    }
+  }
+  return false;
+}
+
 // kAhead: items that a thread has on their way.  With few tokens there is one for a thread and blocks side by side hide the
-// latency (8 an SM); with many, two.
+// latency; with many, two.
 template <typename T, Turn kTurn, int kAhead>
-__global__ void __launch_bounds__(kThreads, kAhead == 1 ? 6 : 4) append_kernel(const __grid_constant__ AppendParams p) {
-  __shared__ uint4 box_parts[2][kThreads][1 + (kTurn == kHalves)];  // smallest and largest of a thread's pieces of new keys
-  __shared__ uint4 old_parts[2][kThreads];                          // ... of what the page held before
+__global__ void __launch_bounds__(kThreads, kAhead == 1 ? 8 : 4) append_kernel(const __grid_constant__ AppendParams p) {
+  __shared__ alignas(16) T kept[kKept][kMaxHeadDim];
+  __shared__ uint4 parts[2][kThreads];  // smallest and largest of a thread's pieces of keys
   grid_dependency_wait();
   grid_launch_dependents();
   const int block = blockIdx.x / p.kv_heads, blocks = gridDim.x / p.kv_heads, kv = blockIdx.x % p.kv_heads;
   const int group = p.heads / p.kv_heads, page = 1 << p.page_shift, pieces = p.dim / 8;
-  T* const q_out = static_cast<T*>(p.q_out) + static_cast<long long>(kv) * group * p.dim;
-  const auto clear = [&](int row) {  // the head group's queries of a token without a place
+  // what this block has of the head group: keys and values, query heads [head0, head0 + heads) of it
+  const bool alone = gridDim.y == 1, keys_too = blockIdx.y == 0;
+  const int head0 = alone || keys_too ? 0 : (blockIdx.y - 1) * kQueryHeads;
+  const int heads = alone ? group : keys_too ? 0 : min(kQueryHeads, group - head0);
+  const T* const q = static_cast<const T*>(p.q.data) + (kv * group + head0) * p.q.head;
+  T* const q_out = static_cast<T*>(p.q_out) + static_cast<long long>(kv * group + head0) * p.dim;
+  const auto clear = [&](int row) {  // the queries of a token without a place
     uint4* to = reinterpret_cast<uint4*>(q_out + static_cast<long long>(row) * p.heads * p.dim);
-    for (int x = threadIdx.x; x < group * pieces; x += kThreads) to[x] = make_uint4(0, 0, 0, 0);
+    for (int x = threadIdx.x; x < heads * pieces; x += kThreads) to[x] = make_uint4(0, 0, 0, 0);
   };
-  for (int row = begin_of(p, p.batch) + block; row < p.tokens; row += blocks) clear(row);
-  if (p.batch == 0) return;
+  const int used = p.cu_tokens ? min(max(p.cu_tokens[p.batch], 0), p.tokens) : p.tokens;  // rows of some sequence
 
-  int i = block;
-  if (p.cu_tokens != nullptr) {  // the last sequence whose blocks begin here or in front
-    i = -1;
-    for (int s = 0; s < p.batch; s += kThreads)
-      i += __syncthreads_count(s + static_cast<int>(threadIdx.x) < p.batch && first_block(p, s + threadIdx.x) <= block);
-    if (i < 0) return;
-  }
-  const int begin = begin_of(p, i), n = begin_of(p, i + 1) - begin;
-  if (n <= 0) return;
-  const int length = p.lengths[i], start = length - n;  // the first new token's position
-  const int nth = (max(start, 0) >> p.page_shift) + block - first_block(p, i);
+  Span span;
+  const bool any_span = find_span(p, block, span);
+  for (int row = used + block; row < p.tokens; row += blocks) clear(row);
+  if (!any_span) return;
+  const int start = span.length - span.n;  // the first new token's position
+  const int nth = (max(start, 0) >> p.page_shift) + span.nth;
   const long long page_begin = static_cast<long long>(nth) << p.page_shift;
   const int from = static_cast<int>(max(static_cast<long long>(start), page_begin));
-  const int to = static_cast<int>(min(static_cast<long long>(length), page_begin + page));
-  if (block == first_block(p, i))
-    for (int j = 0; j < min(n, -start); ++j) clear(begin + j);
+  const int to = static_cast<int>(min(static_cast<long long>(span.length), page_begin + page));
+  if (span.nth == 0)
+    for (int j = 0; j < min(span.n, -start); ++j) clear(span.begin + j);
   if (from >= to) return;
-  const int at = nth < p.table_width ? p.table[static_cast<long long>(i) * p.table_width + nth] : -1;
-  const bool known = at >= 0 && at < p.num_pages;
-  const int until = !known ? from : p.rotary > 0 ? max(from, min(to, p.rope_rows)) : to;  // [from, until) have a place
-  const int row0 = begin + from - start;  // the row of position `from`
-  for (int position = until; position < to; ++position) clear(row0 + position - from);
-  if (from >= until) return;
-  const int tokens = until - from, half = p.rotary / 2, items = items_of<kTurn>(p.dim, p.rotary), slot0 = from % page;
+  const int at = nth < p.table_width ? p.table[static_cast<long long>(span.sequence) * p.table_width + nth] : -1;
+  const int row0 = span.begin + from - start, half = p.rotary / 2, items = items_of<kTurn>(p.dim, p.rotary), slot0 = from % page;
   const float* const cos = p.cos + static_cast<long long>(from) * half;
   const float* const sin = p.sin + static_cast<long long>(from) * half;
-  T* const k_to = static_cast<T*>(p.k_cache) + at * p.k_page + static_cast<long long>(kv) * page * p.dim;
-  T* const v_to = static_cast<T*>(p.v_cache) + at * p.v_page + (static_cast<long long>(kv) * page + slot0) * p.dim;
 
-  // what the page held before: a piece of the head to a thread; the first ones are requested ahead of all else
+  // a token's items: of the key, the value, the queries
+  const int of_keys = keys_too ? items : 0, of_values = keys_too ? pieces : 0, of_token = of_keys + of_values + heads * items;
+  const T* const k = static_cast<const T*>(p.k.data) + kv * p.k.head;
+  const T* const v = static_cast<const T*>(p.v.data) + kv * p.v.head;
+  struct Place {
+    int t, head, item;  // head: -2 the key's, -1 the value's
+  };
+  const auto place_of = [&](int x) {
+    Place w;
+    w.t = x / of_token;
+    int y = x - w.t * of_token;
+    w.head = y < of_keys ? -2 : y < of_keys + of_values ? -1 : (y - of_keys - of_values) / items;
+    w.item = w.head == -2 ? y : w.head == -1 ? y - of_keys : y - of_keys - of_values - w.head * items;
+    return w;
+  };
+  Item<T, kTurn> some[kAhead];
+  Place place[kAhead];
+  const int positions = p.rotary > 0 ? max(0, min(to, p.rope_rows) - from) : to - from;  // that have angles
+  const auto request = [&](int x0) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int x = x0 + u * kThreads;
+      if (x >= positions * of_token) break;
+      place[u] = place_of(x);
+      const long long row = row0 + place[u].t, angles = static_cast<long long>(place[u].t) * half;
+      if (place[u].head == -1) some[u].load_copy(v + row * p.v.row, place[u].item);
+      else some[u].load(p, place[u].head == -2 ? k + row * p.k.row : q + row * p.q.row + place[u].head * p.q.head, cos + angles,
+                        sin + angles, place[u].item);
+    }
+  };
+  request(threadIdx.x);  // does not wait for the page
+  const bool known = at >= 0 && at < p.num_pages;
+  const int tokens = known ? positions : 0;
+  for (int t = tokens; t < to - from; ++t) clear(row0 + t);
+  if (tokens == 0) return;
+  T* const k_page = static_cast<T*>(p.k_cache) + at * p.k_page + static_cast<long long>(kv) * page * p.dim;
+  T* const v_page = static_cast<T*>(p.v_cache) + at * p.v_page + static_cast<long long>(kv) * page * p.dim;
+
+  // what the page held before: a piece of the head to a thread
   constexpr int kOldAhead = 4;
-  const int old_rows = kThreads / pieces, old_row = threadIdx.x / pieces;
-  const bool any_old = p.boxes != nullptr && kTurn != kElements && old_row < min(old_rows, slot0);
-  const T* const old_keys = k_to + threadIdx.x % pieces * 8;
+  const int rows = kThreads / pieces, mine = threadIdx.x / pieces, piece = threadIdx.x % pieces;
+  const bool boxed = p.boxes != nullptr && keys_too;
+  const T* const old_keys = k_page + piece * 8;
   uint4 old[kOldAhead];
   const auto request_old = [&](int slot) {
 #pragma unroll
     for (int u = 0; u < kOldAhead; ++u) {
-      const int mine = slot + u * old_rows;
-      old[u] = load16(old_keys + (mine < slot0 ? mine : old_row) * p.dim);
+      old[u] = make_uint4(0, 0, 0, 0);
+      load_if(old[u], old_keys + (slot + u * rows) * p.dim, boxed && mine < rows && slot + u * rows < slot0);
     }
   };
-  if (any_old) request_old(old_row);
-  // keys: a piece of the head to a thread
-  const int key_rows = kThreads / items, key_row = threadIdx.x / items, key_item = threadIdx.x % items;
-  uint4 lo[2], hi[2];
-  bool any = false;
-  if (key_row < key_rows)
-    for (int t0 = key_row; t0 < tokens; t0 += kAhead * key_rows) {
-      Item<T, kTurn> some[kAhead];
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int t = t0 + u * key_rows;
-        if (t < tokens)
-          some[u].load(p, static_cast<const T*>(p.k.data) + (row0 + t) * p.k.row + kv * p.k.head, cos + static_cast<long long>(t) * half,
-                       sin + static_cast<long long>(t) * half, key_item);
-      }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int t = t0 + u * key_rows;
-        if (t >= tokens) break;
-        some[u].store(p, k_to + (slot0 + t) * p.dim, key_item);
-        lo[0] = any ? smaller<T>(lo[0], some[u].a) : some[u].a;
-        hi[0] = any ? larger<T>(hi[0], some[u].a) : some[u].a;
-        if (kTurn == kHalves) {
-          lo[1] = any ? smaller<T>(lo[1], some[u].b) : some[u].b;
-          hi[1] = any ? larger<T>(hi[1], some[u].b) : some[u].b;
-        }
-        any = true;
-      }
-    }
-  if (kTurn != kElements && p.boxes != nullptr) {
-#pragma unroll
-    for (int e = 0; e < 1 + (kTurn == kHalves); ++e) {
-      box_parts[0][threadIdx.x][e] = lo[e];
-      box_parts[1][threadIdx.x][e] = hi[e];
-    }
-  }
-  // queries and values; where there are few, other warps have them than the keys
-  const int queries = tokens * group * items;
-  for (int x0 = (threadIdx.x + kThreads - 32) % kThreads; x0 < queries; x0 += kAhead * kThreads) {
-    Item<T, kTurn> some[kAhead];
-    int item[kAhead];
-    T* to_row[kAhead];
+  request_old(mine);
+
+  const bool keep = boxed && tokens <= kKept;
+  for (int x0 = threadIdx.x; x0 < tokens * of_token; x0 += kAhead * kThreads) {
+    if (x0 != threadIdx.x) request(x0);
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int x = x0 + u * kThreads;
-      if (x >= queries) break;
-      const int head_row = x / items, t = head_row / group, g = head_row - t * group;
-      item[u] = x - head_row * items;
-      to_row[u] = q_out + (static_cast<long long>(row0 + t) * p.heads + g) * p.dim;
-      some[u].load(p, static_cast<const T*>(p.q.data) + (row0 + t) * p.q.row + (kv * group + g) * p.q.head,
-                   cos + static_cast<long long>(t) * half, sin + static_cast<long long>(t) * half, item[u]);
+      if (x0 + u * kThreads >= tokens * of_token) break;
+      const Place& w = place[u];
+      if (w.head == -1) {
+        some[u].store_copy(v_page + (slot0 + w.t) * p.dim, w.item);
+        continue;
+      }
+      some[u].turn(p, w.item);
+      some[u].store(p, w.head == -2 ? k_page + (slot0 + w.t) * p.dim : q_out + (static_cast<long long>(row0 + w.t) * p.heads + w.head) * p.dim,
+                    w.item);
+      if (keep && w.head == -2) some[u].store(p, kept[w.t], w.item);
     }
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (x0 + u * kThreads < queries) some[u].store(p, to_row[u], item[u]);
   }
-  for (int x0 = (threadIdx.x + kThreads - 96) % kThreads; x0 < tokens * pieces; x0 += 4 * kThreads) {
-    uint4 some[4];
-    T* to_piece[4];
+  if (!boxed) return;
+  __syncthreads();  // the new keys are in shared memory, or in the cache
+  uint4 lo, hi;
+  bool any = false;
+  const auto join = [&](const uint4& key) {
+    lo = any ? smaller<T>(lo, key) : key;
+    hi = any ? larger<T>(hi, key) : key;
+    any = true;
+  };
+  if (mine < rows) {
+    for (int slot = mine; slot < slot0;) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int x = x0 + u * kThreads;
-      if (x >= tokens * pieces) break;
-      const int t = x / pieces, d = (x - t * pieces) * 8;
-      to_piece[u] = v_to + t * p.dim + d;
-      some[u] = load16(static_cast<const T*>(p.v.data) + (row0 + t) * p.v.row + kv * p.v.head + d);
+      for (int u = 0; u < kOldAhead; ++u)
+        if (slot + u * rows < slot0) join(old[u]);
+      slot += kOldAhead * rows;
+      if (slot < slot0) request_old(slot);
     }
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (x0 + u * kThreads < tokens * pieces) *reinterpret_cast<uint4*>(to_piece[u]) = some[u];
+    for (int t = mine; t < tokens; t += rows)
+      join(keep ? *reinterpret_cast<const uint4*>(&kept[t][piece * 8]) : load16(old_keys + (slot0 + t) * p.dim));
   }
-  if (p.boxes == nullptr) return;
+  parts[0][threadIdx.x] = lo;
+  parts[1][threadIdx.x] = hi;
+  __syncthreads();
+  // a thread for two elements, the smallest or the largest; rows of threads without a key are the last ones
+  const int filled = min(rows, max(slot0, tokens));
   uint32_t* const box = reinterpret_cast<uint32_t*>(static_cast<T*>(p.boxes) + (static_cast<long long>(at) * p.kv_heads + kv) * 2 * p.dim);
-  if constexpr (kTurn == kElements) {
-    __syncthreads();  // the block's keys have been written
-    for (int d = threadIdx.x; d < p.dim / 2; d += kThreads) {
-      const uint32_t* const keys = reinterpret_cast<const uint32_t*>(k_to) + d;
-      uint32_t low = *keys, high = low;
-      for (int t = 1; t < slot0 + tokens; ++t) {
-        const uint32_t key = keys[t * (p.dim / 2)];
-        low = smaller<T>(low, key);
-        high = larger<T>(high, key);
-      }
-      box[d] = low;
-      box[p.dim / 2 + d] = high;
+  for (int x = threadIdx.x; x < p.dim; x += kThreads) {
+    const int high = x >= p.dim / 2, word = x - high * (p.dim / 2);  // of four to a piece
+    const uint32_t* const from_parts = reinterpret_cast<const uint32_t*>(parts[high]) + word;
+    uint32_t value = from_parts[0];
+    for (int r = 1; r < filled; ++r) {
+      const uint32_t other = from_parts[r * pieces * 4];
+      value = high ? larger<T>(value, other) : smaller<T>(value, other);
     }
-  } else {
-    if (any_old) {
-      uint4 old_lo = old[0], old_hi = old[0];
-      for (int slot = old_row;;) {
-#pragma unroll
-        for (int u = 0; u < kOldAhead; ++u) {
-          old_lo = smaller<T>(old_lo, old[u]);
-          old_hi = larger<T>(old_hi, old[u]);
-        }
-        slot += kOldAhead * old_rows;
-        if (slot >= slot0) break;
-        request_old(slot);
-      }
-      old_parts[0][threadIdx.x] = old_lo;
-      old_parts[1][threadIdx.x] = old_hi;
-    }
-    __syncthreads();
-    // a thread for two elements, the smallest or the largest
-    for (int x = threadIdx.x; x < p.dim; x += kThreads) {
-      const int high = x >= p.dim / 2, d = (x - high * (p.dim / 2)) * 2;
-      int item = d / 8, piece = 0;
-      if (kTurn == kHalves) {
-        piece = d >= half && d < p.rotary;
-        item = d < p.rotary ? (d - piece * half) / 8 : half / 8 + (d - p.rotary) / 8;
-      }
-      const auto part = [&](const uint4& v) { return (&v.x)[d % 8 / 2]; };
-      uint32_t value = part(box_parts[high][item][piece]);
-      for (int r = 1; r < min(key_rows, tokens); ++r) {
-        const uint32_t other = part(box_parts[high][r * items + item][piece]);
-        value = high ? larger<T>(value, other) : smaller<T>(value, other);
-      }
-      for (int r = 0; r < min(old_rows, slot0); ++r) {
-        const uint32_t other = part(old_parts[high][r * pieces + d / 8]);
-        value = high ? larger<T>(value, other) : smaller<T>(value, other);
-      }
-      box[x] = value;
-    }
+    box[x] = value;
   }
 }
 
@@ -369,7 +384,8 @@ int launch(const AppendParams& p, bool interleaved, unsigned blocks, cudaStream_
   const auto kern = interleaved ? (few ? append_kernel<T, kNeighbors, 1> : append_kernel<T, kNeighbors, 2>)
                     : in_pieces ? (few ? append_kernel<T, kHalves, 1> : append_kernel<T, kHalves, 2>)
                                 : (few ? append_kernel<T, kElements, 1> : append_kernel<T, kElements, 2>);
-  return launch_overlapped(kern, dim3(blocks), dim3(kThreads), 0, stream, p);
+  const int group = p.heads / p.kv_heads;
+  return launch_overlapped(kern, dim3(blocks, few ? 1 : 1 + (group + kQueryHeads - 1) / kQueryHeads), dim3(kThreads), 0, stream, p);
 }
 
 }  // namespace
@@ -422,7 +438,9 @@ extern "C" int iex_paged_append(int tokens, int batch, int heads, int kv_heads, 
   p.table = block_table;
   p.lengths = lengths;
   p.cu_tokens = cu_tokens;
-  const long long blocks = (cu_tokens ? (tokens >> p.page_shift) + 2ll * batch + 1 : batch) * kv_heads;
+  // n tokens touch no more than n pages, nor than n / page + 2
+  const long long pages = cu_tokens ? std::min<long long>(tokens, (tokens >> p.page_shift) + 2ll * batch) : batch;
+  const long long blocks = std::max(1ll, pages) * kv_heads;
   if (blocks > 0x7fffffffll) return IEX_ERR_TOO_LARGE;
   return bf16 ? launch<__nv_bfloat16>(p, interleaved != 0, static_cast<unsigned>(blocks), static_cast<cudaStream_t>(stream))
               : launch<__half>(p, interleaved != 0, static_cast<unsigned>(blocks), static_cast<cudaStream_t>(stream));
