@@ -31,12 +31,17 @@ enum Turn {
 
 struct AppendParams {
   int tokens, batch, heads, kv_heads, dim, rope_rows, rotary, num_pages, page_shift, table_width;
+  uint32_t by_items, by_pieces, by_units;  // inverses for divided()
   Rows q, k, v;
   const float *cos, *sin;
   void *q_out, *k_cache, *v_cache, *boxes;
   long long k_page, v_page;
   const int32_t *table, *lengths, *cu_tokens;
 };
+
+// x / d for x * d below 2^16, with inverse_of(d); a division takes a tenth of what such a block lives.
+inline uint32_t inverse_of(int d) { return 65536u / static_cast<uint32_t>(d) + 1; }
+__device__ __forceinline__ int divided(int x, uint32_t inverse) { return static_cast<int>(static_cast<uint32_t>(x) * inverse >> 16); }
 
 template <typename T>
 struct Pair;
@@ -80,104 +85,126 @@ __device__ __forceinline__ float turned(float a, float b, float c, float s) { re
 
 // Items of a head's row: pieces that are turned, then pieces that are copied.
 template <Turn kTurn>
-__device__ __forceinline__ int items_of(int dim, int rotary) {
+__host__ __device__ __forceinline__ int items_of(int dim, int rotary) {
   if (kTurn == kHalves) return rotary / 16 + (dim - rotary) / 8;
   if (kTurn == kNeighbors) return dim / 8;
   return rotary / 2 + dim - rotary;
 }
 
-// An item on its way: what is loaded of it ahead of the items before it being stored.
+// The angles of an item at a position, and what they make of it.
 template <typename T, Turn kTurn>
-struct Item {
-  uint4 a, b;  // the piece, or both (kElements: one element each)
-  float c[kTurn == kHalves ? 8 : kTurn == kNeighbors ? 4 : 1], s[kTurn == kHalves ? 8 : kTurn == kNeighbors ? 4 : 1];
+struct Angles {
+  static constexpr int kPairs = kTurn == kHalves ? 8 : kTurn == kNeighbors ? 4 : 1;
+  float c[kPairs], s[kPairs];
+  int pairs;  // of the item
 
-  __device__ __forceinline__ void load_copy(const T* from, int item) { a = load16(from + item * 8); }
-  __device__ __forceinline__ void store_copy(T* to, int item) const { *reinterpret_cast<uint4*>(to + item * 8) = a; }
-
-  // Item `item` of the row at `from`; the angles of its position at cos and sin.
-  __device__ __forceinline__ void load(const AppendParams& p, const T* from, const float* cos, const float* sin, int item) {
+  __device__ __forceinline__ void load(const AppendParams& p, const float* cos, const float* sin, int item) {
     const int half = p.rotary / 2;
+    pairs = min(kPairs, max(0, half - item * kPairs));
     if constexpr (kTurn == kHalves) {
-      if (item < half / 8) {
-        const int d = item * 8;
-        a = load16(from + d);
-        b = load16(from + half + d);
+      uint4 v[4] = {};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint4 vc = load16(cos + d + 4 * i), vs = load16(sin + d + 4 * i);
-          c[4 * i] = __uint_as_float(vc.x), c[4 * i + 1] = __uint_as_float(vc.y);
-          c[4 * i + 2] = __uint_as_float(vc.z), c[4 * i + 3] = __uint_as_float(vc.w);
-          s[4 * i] = __uint_as_float(vs.x), s[4 * i + 1] = __uint_as_float(vs.y);
-          s[4 * i + 2] = __uint_as_float(vs.z), s[4 * i + 3] = __uint_as_float(vs.w);
-        }
-      } else {
-        a = load16(from + p.rotary + (item - half / 8) * 8);
+      for (int i = 0; i < 2; ++i) {
+        load_if(v[i], cos + item * 8 + 4 * i, pairs > 0);
+        load_if(v[2 + i], sin + item * 8 + 4 * i, pairs > 0);
+        c[4 * i] = __uint_as_float(v[i].x), c[4 * i + 1] = __uint_as_float(v[i].y);
+        c[4 * i + 2] = __uint_as_float(v[i].z), c[4 * i + 3] = __uint_as_float(v[i].w);
+        s[4 * i] = __uint_as_float(v[2 + i].x), s[4 * i + 1] = __uint_as_float(v[2 + i].y);
+        s[4 * i + 2] = __uint_as_float(v[2 + i].z), s[4 * i + 3] = __uint_as_float(v[2 + i].w);
       }
-    } else if constexpr (kTurn == kNeighbors) {
-      a = load16(from + item * 8);
+    } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int pair = min(item * 4 + i, max(half - 1, 0));
+      for (int i = 0; i < kPairs; ++i) {
+        const int pair = min(item * kPairs + i, half - 1);
         c[i] = half > 0 ? cos[pair] : 1.f;
         s[i] = half > 0 ? sin[pair] : 0.f;
       }
-    } else {
-      T *x = reinterpret_cast<T*>(&a), *y = reinterpret_cast<T*>(&b);
-      if (item < half) {
-        x[0] = from[item];
-        y[0] = from[half + item];
-        c[0] = cos[item];
-        s[0] = sin[item];
-      } else {
-        x[0] = from[half + item];
-      }
     }
   }
+};
 
-  __device__ __forceinline__ void turn(const AppendParams& p, int item) {
+template <typename T, Turn kTurn>
+struct Item {
+  uint4 a, b;  // the piece, or both (kElements: one element each)
+
+  // Item `item` of the row at `from`, where there is one.
+  __device__ __forceinline__ void load(const AppendParams& p, const T* from, int item, int pairs, bool there) {
     const int half = p.rotary / 2;
+    if constexpr (kTurn == kHalves) {
+      load_if(a, from + (pairs > 0 ? item * 8 : p.rotary + (item - half / 8) * 8), there);
+      load_if(b, from + half + item * 8, there && pairs > 0);
+    } else if constexpr (kTurn == kNeighbors) {
+      load_if(a, from + item * 8, there);
+    } else if (there) {
+      *reinterpret_cast<T*>(&a) = from[pairs > 0 ? item : half + item];
+      if (pairs > 0) *reinterpret_cast<T*>(&b) = from[half + item];
+    }
+  }
+  __device__ __forceinline__ void turn(const Angles<T, kTurn>& angles) {
     T *x = reinterpret_cast<T*>(&a), *y = reinterpret_cast<T*>(&b);
     if constexpr (kTurn == kNeighbors) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float one = as_float(x[2 * i]), two = as_float(x[2 * i + 1]);
-        const bool turns = item * 4 + i < half;
-        x[2 * i] = turns ? rounded<T>(turned(one, two, c[i], -s[i])) : x[2 * i];
-        x[2 * i + 1] = turns ? rounded<T>(turned(two, one, c[i], s[i])) : x[2 * i + 1];
+        const bool turns = i < angles.pairs;
+        x[2 * i] = turns ? rounded<T>(turned(one, two, angles.c[i], -angles.s[i])) : x[2 * i];
+        x[2 * i + 1] = turns ? rounded<T>(turned(two, one, angles.c[i], angles.s[i])) : x[2 * i + 1];
       }
-    } else {
-      constexpr int kElementsOf = kTurn == kHalves ? 8 : 1;
-      if (item < half / kElementsOf) {
+    } else if (angles.pairs > 0) {
 #pragma unroll
-        for (int i = 0; i < kElementsOf; ++i) {
-          const float one = as_float(x[i]), two = as_float(y[i]);
-          x[i] = rounded<T>(turned(one, two, c[i], -s[i]));
-          y[i] = rounded<T>(turned(two, one, c[i], s[i]));
-        }
+      for (int i = 0; i < Angles<T, kTurn>::kPairs; ++i) {
+        const float one = as_float(x[i]), two = as_float(y[i]);
+        x[i] = rounded<T>(turned(one, two, angles.c[i], -angles.s[i]));
+        y[i] = rounded<T>(turned(two, one, angles.c[i], angles.s[i]));
       }
     }
   }
-
   // To the row at `to`.
-  __device__ __forceinline__ void store(const AppendParams& p, T* to, int item) const {
+  __device__ __forceinline__ void store(const AppendParams& p, T* to, int item, int pairs) const {
     const int half = p.rotary / 2;
-    if constexpr (kTurn == kNeighbors) {
+    if constexpr (kTurn == kHalves) {
+      *reinterpret_cast<uint4*>(to + (pairs > 0 ? item * 8 : p.rotary + (item - half / 8) * 8)) = a;
+      if (pairs > 0) *reinterpret_cast<uint4*>(to + half + item * 8) = b;
+    } else if constexpr (kTurn == kNeighbors) {
       *reinterpret_cast<uint4*>(to + item * 8) = a;
     } else {
-      constexpr int kElementsOf = kTurn == kHalves ? 8 : 1;
-      const bool turns = item < half / kElementsOf;
-      T* const first = turns ? to + item * kElementsOf : to + p.rotary + (item - half / kElementsOf) * kElementsOf;
-      if constexpr (kTurn == kHalves) {
-        *reinterpret_cast<uint4*>(first) = a;
-        if (turns) *reinterpret_cast<uint4*>(first + half) = b;
-      } else {
-        *first = *reinterpret_cast<const T*>(&a);
-        if (turns) first[half] = *reinterpret_cast<const T*>(&b);
-      }
+      to[pairs > 0 ? item : half + item] = *reinterpret_cast<const T*>(&a);
+      if (pairs > 0) to[half + item] = *reinterpret_cast<const T*>(&b);
     }
   }
 };
+
+// `heads` heads of `tokens` rows turned, kHeads of them by one thread, which share the angles.  `thread`: which of the block's this one
+// counts as; kept (or null): a second place for the first head.
+template <typename T, Turn kTurn, int kHeads>
+__device__ __forceinline__ void turn_rows(const AppendParams& p, int thread, int tokens, int heads, uint32_t by_units, const T* x, long long x_row,
+                                          long long x_head, T* out, long long out_row, const float* cos, const float* sin,
+                                          T (*kept)[kMaxHeadDim]) {
+  const int items = items_of<kTurn>(p.dim, p.rotary), units = (heads + kHeads - 1) / kHeads * items;
+  if (units == 0) return;
+  const bool few = units <= kThreads;
+  const int rows = few ? divided(kThreads, by_units) : 1, row = few ? divided(thread, by_units) : 0, half = p.rotary / 2;
+  if (row >= rows) return;
+  for (int y = thread - row * units; y < units; y += kThreads) {
+    const int set = few ? divided(y, p.by_items) : y / items, item = y - set * items;
+#pragma unroll 1
+    for (int t = row; t < tokens; t += rows) {
+      Angles<T, kTurn> angles;
+      Item<T, kTurn> some[kHeads];
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h)
+        some[h].load(p, x + t * x_row + (set * kHeads + h) * x_head, item, min(1, max(0, half - item * Angles<T, kTurn>::kPairs)),
+                     set * kHeads + h < heads);
+      angles.load(p, cos + static_cast<long long>(t) * half, sin + static_cast<long long>(t) * half, item);
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h) {
+        some[h].turn(angles);
+        if (set * kHeads + h < heads) some[h].store(p, out + t * out_row + (set * kHeads + h) * p.dim, item, angles.pairs);
+      }
+      if (kept != nullptr) some[0].store(p, kept[t], item, angles.pairs);
+    }
+  }
+}
 
 // The new tokens that a block has.
 struct Span {
@@ -230,15 +257,13 @@ __device__ __forceinline__ bool find_span(const AppendParams& p, int block, Span
   return false;
 }
 
-// kAhead: items that a thread has on their way.  With few tokens there is one for a thread and blocks side by side hide the
-// latency; with many, two.
-template <typename T, Turn kTurn, int kAhead>
-__global__ void __launch_bounds__(kThreads, kAhead == 1 ? 8 : 4) append_kernel(const __grid_constant__ AppendParams p) {
+template <typename T, Turn kTurn>
+__global__ void __launch_bounds__(kThreads, 8) append_kernel(const __grid_constant__ AppendParams p) {
   __shared__ alignas(16) T kept[kKept][kMaxHeadDim];
   __shared__ uint4 parts[2][kThreads];  // smallest and largest of a thread's pieces of keys
   grid_dependency_wait();
   grid_launch_dependents();
-  const int block = blockIdx.x / p.kv_heads, blocks = gridDim.x / p.kv_heads, kv = blockIdx.x % p.kv_heads;
+  const int block = blockIdx.x, blocks = gridDim.x, kv = blockIdx.z;
   const int group = p.heads / p.kv_heads, page = 1 << p.page_shift, pieces = p.dim / 8;
   // what this block has of the head group: keys and values, query heads [head0, head0 + heads) of it
   const bool alone = gridDim.y == 1, keys_too = blockIdx.y == 0;
@@ -265,52 +290,29 @@ __global__ void __launch_bounds__(kThreads, kAhead == 1 ? 8 : 4) append_kernel(c
     for (int j = 0; j < min(span.n, -start); ++j) clear(span.begin + j);
   if (from >= to) return;
   const int at = nth < p.table_width ? p.table[static_cast<long long>(span.sequence) * p.table_width + nth] : -1;
-  const int row0 = span.begin + from - start, half = p.rotary / 2, items = items_of<kTurn>(p.dim, p.rotary), slot0 = from % page;
+  const int row0 = span.begin + from - start, half = p.rotary / 2, slot0 = from & (page - 1);
   const float* const cos = p.cos + static_cast<long long>(from) * half;
   const float* const sin = p.sin + static_cast<long long>(from) * half;
-
-  // a token's items: of the key, the value, the queries
-  const int of_keys = keys_too ? items : 0, of_values = keys_too ? pieces : 0, of_token = of_keys + of_values + heads * items;
-  const T* const k = static_cast<const T*>(p.k.data) + kv * p.k.head;
-  const T* const v = static_cast<const T*>(p.v.data) + kv * p.v.head;
-  struct Place {
-    int t, head, item;  // head: -2 the key's, -1 the value's
-  };
-  const auto place_of = [&](int x) {
-    Place w;
-    w.t = x / of_token;
-    int y = x - w.t * of_token;
-    w.head = y < of_keys ? -2 : y < of_keys + of_values ? -1 : (y - of_keys - of_values) / items;
-    w.item = w.head == -2 ? y : w.head == -1 ? y - of_keys : y - of_keys - of_values - w.head * items;
-    return w;
-  };
-  Item<T, kTurn> some[kAhead];
-  Place place[kAhead];
   const int positions = p.rotary > 0 ? max(0, min(to, p.rope_rows) - from) : to - from;  // that have angles
-  const auto request = [&](int x0) {
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int x = x0 + u * kThreads;
-      if (x >= positions * of_token) break;
-      place[u] = place_of(x);
-      const long long row = row0 + place[u].t, angles = static_cast<long long>(place[u].t) * half;
-      if (place[u].head == -1) some[u].load_copy(v + row * p.v.row, place[u].item);
-      else some[u].load(p, place[u].head == -2 ? k + row * p.k.row : q + row * p.q.row + place[u].head * p.q.head, cos + angles,
-                        sin + angles, place[u].item);
-    }
-  };
-  request(threadIdx.x);  // does not wait for the page
+
+  // Queries do not wait for the page.  Where there are few, other warps have them than the keys.
+  turn_rows<T, kTurn, kQueryHeads>(p, (threadIdx.x + kThreads - 32) % kThreads, positions, heads, p.by_units, q + row0 * p.q.row, p.q.row, p.q.head,
+                                   q_out + static_cast<long long>(row0) * p.heads * p.dim, static_cast<long long>(p.heads) * p.dim, cos,
+                                   sin, nullptr);
   const bool known = at >= 0 && at < p.num_pages;
   const int tokens = known ? positions : 0;
-  for (int t = tokens; t < to - from; ++t) clear(row0 + t);
-  if (tokens == 0) return;
+  if (tokens < to - from) {
+    if (!known) __syncthreads();  // they have been written
+    for (int t = tokens; t < to - from; ++t) clear(row0 + t);
+  }
+  if (tokens == 0 || !keys_too) return;
   T* const k_page = static_cast<T*>(p.k_cache) + at * p.k_page + static_cast<long long>(kv) * page * p.dim;
   T* const v_page = static_cast<T*>(p.v_cache) + at * p.v_page + static_cast<long long>(kv) * page * p.dim;
 
   // what the page held before: a piece of the head to a thread
   constexpr int kOldAhead = 4;
-  const int rows = kThreads / pieces, mine = threadIdx.x / pieces, piece = threadIdx.x % pieces;
-  const bool boxed = p.boxes != nullptr && keys_too;
+  const int rows = divided(kThreads, p.by_pieces), mine = divided(threadIdx.x, p.by_pieces), piece = threadIdx.x - mine * pieces;
+  const bool boxed = p.boxes != nullptr;
   const T* const old_keys = k_page + piece * 8;
   uint4 old[kOldAhead];
   const auto request_old = [&](int slot) {
@@ -323,22 +325,19 @@ __global__ void __launch_bounds__(kThreads, kAhead == 1 ? 8 : 4) append_kernel(c
   request_old(mine);
 
   const bool keep = boxed && tokens <= kKept;
-  for (int x0 = threadIdx.x; x0 < tokens * of_token; x0 += kAhead * kThreads) {
-    if (x0 != threadIdx.x) request(x0);
+  turn_rows<T, kTurn, 1>(p, threadIdx.x, tokens, 1, p.by_items, static_cast<const T*>(p.k.data) + row0 * p.k.row + kv * p.k.head, p.k.row, 0,
+                         k_page + slot0 * p.dim, p.dim, cos, sin, keep ? kept : nullptr);
+  const int vector = (threadIdx.x + kThreads - 96) % kThreads, v_row = divided(vector, p.by_pieces), d = (vector - v_row * pieces) * 8;
+  const T* const v = static_cast<const T*>(p.v.data) + row0 * p.v.row + kv * p.v.head + d;
+  if (v_row < rows)
+    for (int t0 = v_row; t0 < tokens; t0 += 4 * rows) {
+      uint4 some[4];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (x0 + u * kThreads >= tokens * of_token) break;
-      const Place& w = place[u];
-      if (w.head == -1) {
-        some[u].store_copy(v_page + (slot0 + w.t) * p.dim, w.item);
-        continue;
-      }
-      some[u].turn(p, w.item);
-      some[u].store(p, w.head == -2 ? k_page + (slot0 + w.t) * p.dim : q_out + (static_cast<long long>(row0 + w.t) * p.heads + w.head) * p.dim,
-                    w.item);
-      if (keep && w.head == -2) some[u].store(p, kept[w.t], w.item);
+      for (int u = 0; u < 4; ++u) load_if(some[u], v + (t0 + u * rows) * p.v.row, t0 + u * rows < tokens);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (t0 + u * rows < tokens) *reinterpret_cast<uint4*>(v_page + (slot0 + t0 + u * rows) * p.dim + d) = some[u];
     }
-  }
   if (!boxed) return;
   __syncthreads();  // the new keys are in shared memory, or in the cache
   uint4 lo, hi;
@@ -377,15 +376,23 @@ __global__ void __launch_bounds__(kThreads, kAhead == 1 ? 8 : 4) append_kernel(c
   }
 }
 
+template <typename T, Turn kTurn>
+int launch(AppendParams p, int blocks, cudaStream_t stream) {
+  const bool few = p.tokens <= 4ll * p.batch;  // a block's threads have next to nothing to do
+  const int group = p.heads / p.kv_heads, items = items_of<kTurn>(p.dim, p.rotary);
+  const int heads = few ? group : std::min(group, kQueryHeads);  // of a block
+  p.by_items = inverse_of(items);
+  p.by_pieces = inverse_of(p.dim / 8);
+  p.by_units = inverse_of((heads + kQueryHeads - 1) / kQueryHeads * items);
+  const dim3 grid(blocks, few ? 1 : 1 + (group + kQueryHeads - 1) / kQueryHeads, p.kv_heads);
+  return launch_overlapped(append_kernel<T, kTurn>, grid, dim3(kThreads), 0, stream, p);
+}
+
 template <typename T>
-int launch(const AppendParams& p, bool interleaved, unsigned blocks, cudaStream_t stream) {
+int launch(const AppendParams& p, bool interleaved, int blocks, cudaStream_t stream) {
+  if (interleaved) return launch<T, kNeighbors>(p, blocks, stream);
   const bool in_pieces = p.rotary % 16 == 0 && aligned16(p.cos) && aligned16(p.sin);
-  const bool few = p.tokens <= 4ll * p.batch;
-  const auto kern = interleaved ? (few ? append_kernel<T, kNeighbors, 1> : append_kernel<T, kNeighbors, 2>)
-                    : in_pieces ? (few ? append_kernel<T, kHalves, 1> : append_kernel<T, kHalves, 2>)
-                                : (few ? append_kernel<T, kElements, 1> : append_kernel<T, kElements, 2>);
-  const int group = p.heads / p.kv_heads;
-  return launch_overlapped(kern, dim3(blocks, few ? 1 : 1 + (group + kQueryHeads - 1) / kQueryHeads), dim3(kThreads), 0, stream, p);
+  return in_pieces ? launch<T, kHalves>(p, blocks, stream) : launch<T, kElements>(p, blocks, stream);
 }
 
 }  // namespace
@@ -403,6 +410,7 @@ extern "C" int iex_paged_append(int tokens, int batch, int heads, int kv_heads, 
   if (tokens < 0 || batch < 0 || num_pages < 0 || table_width < 0 || rope_rows < 0 || rotary < 0) return IEX_ERR_BAD_ARG;
   if (!heads_ok(heads, kv_heads, head_dim) || !page_size_ok(page_size) || rotary % 2 != 0 || rotary > head_dim)
     return IEX_ERR_UNSUPPORTED;
+  if (kv_heads > 65535 || heads / kv_heads > 65535) return IEX_ERR_TOO_LARGE;  // a grid's second and third dimension
   if (tokens == 0) return IEX_OK;
   if (!q || !k || !v || !q_out || (batch > 0 && !lengths) || (rotary > 0 && (!cos || !sin)) ||
       (batch > 0 && table_width > 0 && !block_table) || (num_pages > 0 && (!k_cache || !v_cache)) ||
@@ -440,8 +448,7 @@ extern "C" int iex_paged_append(int tokens, int batch, int heads, int kv_heads, 
   p.cu_tokens = cu_tokens;
   // n tokens touch no more than n pages, nor than n / page + 2
   const long long pages = cu_tokens ? std::min<long long>(tokens, (tokens >> p.page_shift) + 2ll * batch) : batch;
-  const long long blocks = std::max(1ll, pages) * kv_heads;
-  if (blocks > 0x7fffffffll) return IEX_ERR_TOO_LARGE;
-  return bf16 ? launch<__nv_bfloat16>(p, interleaved != 0, static_cast<unsigned>(blocks), static_cast<cudaStream_t>(stream))
-              : launch<__half>(p, interleaved != 0, static_cast<unsigned>(blocks), static_cast<cudaStream_t>(stream));
+  const int blocks = static_cast<int>(std::max(1ll, pages));
+  return bf16 ? launch<__nv_bfloat16>(p, interleaved != 0, blocks, static_cast<cudaStream_t>(stream))
+              : launch<__half>(p, interleaved != 0, blocks, static_cast<cudaStream_t>(stream));
 }
