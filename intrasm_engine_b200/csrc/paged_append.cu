@@ -11,6 +11,7 @@
 // heads have blocks of their own.  An item is 16 bytes, or the two 16-byte pieces that are turned into each other.  What the
 // page held before is requested ahead of all else; new keys pass through shared memory on their way into the box.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -18,8 +19,6 @@ namespace iex {
 namespace paged {
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int kWarps = kThreads / 32;
 constexpr int kKept = 32;       // new keys that are kept in shared memory: of pages with more of them the box reads the cache
 constexpr int kQueryHeads = 2;  // of a block that has nothing but query heads
 
@@ -176,7 +175,7 @@ struct Item {
 
 // `heads` heads of `tokens` rows turned, kHeads of them by one thread, which share the angles.  `thread`: which of the block's this one
 // counts as; kept (or null): a second place for the first head.
-template <typename T, Turn kTurn, int kHeads>
+template <typename T, Turn kTurn, int kThreads, int kHeads>
 __device__ __forceinline__ void turn_rows(const AppendParams& p, int thread, int tokens, int heads, uint32_t by_units, const T* x, long long x_row,
                                           long long x_head, T* out, long long out_row, const float* cos, const float* sin,
                                           T (*kept)[kMaxHeadDim]) {
@@ -212,12 +211,15 @@ struct Span {
 };
 
 // Blocks in a row have the pages of one sequence after the other: n new tokens touch up to (n + page - 2) / page + 1 of them.
-// False where there is no such block.
-__device__ __forceinline__ bool find_span(const AppendParams& p, int block, Span& found) {
+// False where there is no such block.  used: the rows of the sequences.
+template <int kThreads>
+__device__ __forceinline__ bool find_span(const AppendParams& p, int block, Span& found, int& used) {
+  constexpr int kWarps = kThreads / 32;
   __shared__ Span shared;
-  __shared__ int sums[kWarps];
+  __shared__ int sums[kWarps], last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (p.cu_tokens == nullptr) {
+    used = p.tokens;
     if (block >= p.batch) return false;
     found = {block, block, 1, p.lengths[block], 0};
     return true;
@@ -228,8 +230,10 @@ __device__ __forceinline__ bool find_span(const AppendParams& p, int block, Span
     int begin = 0, n = 0, length = 0;
     if (s < p.batch) {
       begin = min(max(p.cu_tokens[s], 0), p.tokens);
-      n = max(0, min(max(p.cu_tokens[s + 1], 0), p.tokens) - begin);
+      const int next = min(max(p.cu_tokens[s + 1], 0), p.tokens);
+      n = max(0, next - begin);
       length = p.lengths[s];
+      if (s == p.batch - 1) last = next;
     }
     const int mine = n > 0 ? ((n + (1 << p.page_shift) - 2) >> p.page_shift) + 1 : 0;
     int sum = mine;
@@ -249,16 +253,20 @@ __device__ __forceinline__ bool find_span(const AppendParams& p, int block, Span
     if (first <= block && block < first + mine) shared = {s, begin, n, length, block - first};
     front += all;
     __syncthreads();
-    if (block < front) {
-      found = shared;
-      return true;
+    const bool here = block < front;
+    if (here) found = shared;
+    if (here || s0 + kThreads >= p.batch) {
+      used = s0 + kThreads >= p.batch ? last : min(max(p.cu_tokens[p.batch], 0), p.tokens);
+      return here;
     }
   }
+  used = min(max(p.cu_tokens[0], 0), p.tokens);  // no sequences
   return false;
 }
 
-template <typename T, Turn kTurn>
-__global__ void __launch_bounds__(kThreads, 8) append_kernel(const __grid_constant__ AppendParams p) {
+// kThreads: 128, or 64 where a block has few tokens and what counts is how many blocks are under way at once.
+template <typename T, Turn kTurn, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) append_kernel(const __grid_constant__ AppendParams p) {
   __shared__ alignas(16) T kept[kKept][kMaxHeadDim];
   __shared__ uint4 parts[2][kThreads];  // smallest and largest of a thread's pieces of keys
   grid_dependency_wait();
@@ -275,10 +283,9 @@ __global__ void __launch_bounds__(kThreads, 8) append_kernel(const __grid_consta
     uint4* to = reinterpret_cast<uint4*>(q_out + static_cast<long long>(row) * p.heads * p.dim);
     for (int x = threadIdx.x; x < heads * pieces; x += kThreads) to[x] = make_uint4(0, 0, 0, 0);
   };
-  const int used = p.cu_tokens ? min(max(p.cu_tokens[p.batch], 0), p.tokens) : p.tokens;  // rows of some sequence
-
   Span span;
-  const bool any_span = find_span(p, block, span);
+  int used;
+  const bool any_span = find_span<kThreads>(p, block, span, used);
   for (int row = used + block; row < p.tokens; row += blocks) clear(row);
   if (!any_span) return;
   const int start = span.length - span.n;  // the first new token's position
@@ -296,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 8) append_kernel(const __grid_consta
   const int positions = p.rotary > 0 ? max(0, min(to, p.rope_rows) - from) : to - from;  // that have angles
 
   // Queries do not wait for the page.  Where there are few, other warps have them than the keys.
-  turn_rows<T, kTurn, kQueryHeads>(p, (threadIdx.x + kThreads - 32) % kThreads, positions, heads, p.by_units, q + row0 * p.q.row, p.q.row, p.q.head,
+  turn_rows<T, kTurn, kThreads, kQueryHeads>(p, (threadIdx.x + kThreads - 32) % kThreads, positions, heads, p.by_units, q + row0 * p.q.row, p.q.row, p.q.head,
                                    q_out + static_cast<long long>(row0) * p.heads * p.dim, static_cast<long long>(p.heads) * p.dim, cos,
                                    sin, nullptr);
   const bool known = at >= 0 && at < p.num_pages;
@@ -310,24 +317,23 @@ __global__ void __launch_bounds__(kThreads, 8) append_kernel(const __grid_consta
   T* const v_page = static_cast<T*>(p.v_cache) + at * p.v_page + static_cast<long long>(kv) * page * p.dim;
 
   // what the page held before: a piece of the head to a thread
-  constexpr int kOldAhead = 4;
+  constexpr int kOldAhead = 512 / kThreads;
   const int rows = divided(kThreads, p.by_pieces), mine = divided(threadIdx.x, p.by_pieces), piece = threadIdx.x - mine * pieces;
   const bool boxed = p.boxes != nullptr;
   const T* const old_keys = k_page + piece * 8;
   uint4 old[kOldAhead];
-  const auto request_old = [&](int slot) {
+  const bool any_old = boxed && mine < rows && mine < slot0;
+  const auto request_old = [&](int slot) {  // those behind the last one: one of the others again
 #pragma unroll
-    for (int u = 0; u < kOldAhead; ++u) {
-      old[u] = make_uint4(0, 0, 0, 0);
-      load_if(old[u], old_keys + (slot + u * rows) * p.dim, boxed && mine < rows && slot + u * rows < slot0);
-    }
+    for (int u = 0; u < kOldAhead; ++u)
+      load_if(old[u], old_keys + (slot + u * rows < slot0 ? slot + u * rows : mine) * p.dim, any_old);
   };
   request_old(mine);
 
   const bool keep = boxed && tokens <= kKept;
-  turn_rows<T, kTurn, 1>(p, threadIdx.x, tokens, 1, p.by_items, static_cast<const T*>(p.k.data) + row0 * p.k.row + kv * p.k.head, p.k.row, 0,
+  turn_rows<T, kTurn, kThreads, 1>(p, threadIdx.x, tokens, 1, p.by_items, static_cast<const T*>(p.k.data) + row0 * p.k.row + kv * p.k.head, p.k.row, 0,
                          k_page + slot0 * p.dim, p.dim, cos, sin, keep ? kept : nullptr);
-  const int vector = (threadIdx.x + kThreads - 96) % kThreads, v_row = divided(vector, p.by_pieces), d = (vector - v_row * pieces) * 8;
+  const int vector = (threadIdx.x + 16) % kThreads, v_row = divided(vector, p.by_pieces), d = (vector - v_row * pieces) * 8;
   const T* const v = static_cast<const T*>(p.v.data) + row0 * p.v.row + kv * p.v.head + d;
   if (v_row < rows)
     for (int t0 = v_row; t0 < tokens; t0 += 4 * rows) {
@@ -340,24 +346,26 @@ __global__ void __launch_bounds__(kThreads, 8) append_kernel(const __grid_consta
     }
   if (!boxed) return;
   __syncthreads();  // the new keys are in shared memory, or in the cache
-  uint4 lo, hi;
-  bool any = false;
-  const auto join = [&](const uint4& key) {
-    lo = any ? smaller<T>(lo, key) : key;
-    hi = any ? larger<T>(hi, key) : key;
-    any = true;
-  };
-  if (mine < rows) {
-    for (int slot = mine; slot < slot0;) {
+  constexpr uint32_t kInfinity = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;  // two of them
+  uint4 lo = make_uint4(kInfinity, kInfinity, kInfinity, kInfinity), hi = lo;
+  hi.x = hi.y = hi.z = hi.w = kInfinity | 0x80008000u;
+  if (any_old)
+    for (int slot = mine;;) {
 #pragma unroll
-      for (int u = 0; u < kOldAhead; ++u)
-        if (slot + u * rows < slot0) join(old[u]);
+      for (int u = 0; u < kOldAhead; ++u) {
+        lo = smaller<T>(lo, old[u]);
+        hi = larger<T>(hi, old[u]);
+      }
       slot += kOldAhead * rows;
-      if (slot < slot0) request_old(slot);
+      if (slot >= slot0) break;
+      request_old(slot);
     }
-    for (int t = mine; t < tokens; t += rows)
-      join(keep ? *reinterpret_cast<const uint4*>(&kept[t][piece * 8]) : load16(old_keys + (slot0 + t) * p.dim));
-  }
+  if (mine < rows)
+    for (int t = mine; t < tokens; t += rows) {
+      const uint4 key = keep ? *reinterpret_cast<const uint4*>(&kept[t][piece * 8]) : load16(old_keys + (slot0 + t) * p.dim);
+      lo = smaller<T>(lo, key);
+      hi = larger<T>(hi, key);
+    }
   parts[0][threadIdx.x] = lo;
   parts[1][threadIdx.x] = hi;
   __syncthreads();
@@ -378,14 +386,15 @@ __global__ void __launch_bounds__(kThreads, 8) append_kernel(const __grid_consta
 
 template <typename T, Turn kTurn>
 int launch(AppendParams p, int blocks, cudaStream_t stream) {
-  const bool few = p.tokens <= 4ll * p.batch;  // a block's threads have next to nothing to do
+  const bool few = p.tokens <= 4ll * p.batch;
   const int group = p.heads / p.kv_heads, items = items_of<kTurn>(p.dim, p.rotary);
   const int heads = few ? group : std::min(group, kQueryHeads);  // of a block
   p.by_items = inverse_of(items);
   p.by_pieces = inverse_of(p.dim / 8);
   p.by_units = inverse_of((heads + kQueryHeads - 1) / kQueryHeads * items);
   const dim3 grid(blocks, few ? 1 : 1 + (group + kQueryHeads - 1) / kQueryHeads, p.kv_heads);
-  return launch_overlapped(append_kernel<T, kTurn>, grid, dim3(kThreads), 0, stream, p);
+  return few ? launch_overlapped(append_kernel<T, kTurn, 64>, grid, dim3(64), 0, stream, p)
+             : launch_overlapped(append_kernel<T, kTurn, 128>, grid, dim3(128), 0, stream, p);
 }
 
 template <typename T>
