@@ -31,7 +31,7 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kAhead = 8;         // boxes that a lane has on their way
-constexpr int kMaxPages = 16384;  // keys of 8 bytes in shared memory
+constexpr int kMaxPages = 16384;  // 12 bytes of shared memory each
 constexpr int kBins = 256;
 constexpr int kMostBlocks = 8;  // of a cluster
 static_assert(kThreads == kBins, "a thread clears a bin");
@@ -46,12 +46,18 @@ struct SelectParams {
 
 using Key = unsigned long long;
 
-// Doubles as whole numbers of the same order, all above 0; both zeros are one number, NaN is above all.
+// Scores as whole numbers of the same order, all above 0; both zeros are one number, NaN is above all.  And the other way round, for numbers.
 __device__ __forceinline__ Key ordered(double score) {
-  if (score != score) return ~0ull;
   const long long bits = __double_as_longlong(score + 0.0);
-  return static_cast<Key>(bits) ^ (bits < 0 ? ~0ull : 1ull << 63);
+  const Key key = static_cast<Key>(bits) ^ (bits < 0 ? ~0ull : 1ull << 63);
+  return score != score ? ~0ull : key;
 }
+__device__ __forceinline__ uint32_t ordered(float score) {
+  const int bits = __float_as_int(score + 0.f);
+  const uint32_t key = static_cast<uint32_t>(bits) ^ (bits < 0 ? ~0u : 1u << 31);
+  return score != score ? ~0u : key;
+}
+__device__ __forceinline__ float number(uint32_t key) { return __uint_as_float(key >> 31 ? key ^ 1u << 31 : ~key); }
 
 template <typename T>
 __device__ __forceinline__ void unpack(const uint4& v, float (&to)[8]) {
@@ -70,8 +76,8 @@ __device__ __forceinline__ uint32_t larger_size(uint32_t a, uint32_t b, __nv_bfl
   return reinterpret_cast<const uint32_t&>(v);
 }
 
-// The sum of v over all threads in front of this one.  `warps` has not been read since the last barrier.
-__device__ __forceinline__ uint32_t sum_in_front(uint32_t v, uint32_t* warps) {
+// The sums of v over all threads in front of this one and over all.  `warps` has not been read since the last barrier.
+__device__ __forceinline__ uint2 add_in_order(uint32_t v, uint32_t* warps) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t sum = v;
   for (int d = 1; d < 32; d <<= 1) {
@@ -80,19 +86,8 @@ __device__ __forceinline__ uint32_t sum_in_front(uint32_t v, uint32_t* warps) {
   }
   if (lane == 31) warps[warp] = sum;
   __syncthreads();
-  return sum - v + __reduce_add_sync(0xffffffffu, lane < warp ? warps[lane] : 0);
-}
-// The sum of v over all threads, likewise.
-__device__ __forceinline__ uint32_t sum_of_all(uint32_t v, uint32_t* warps) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t sum = __reduce_add_sync(0xffffffffu, v);
-  if (lane == 0) warps[warp] = sum;
-  __syncthreads();
-  return __reduce_add_sync(0xffffffffu, lane < kWarps ? warps[lane] : 0);
-}
-
-__device__ __forceinline__ double number(Key key) {  // the other way round, for numbers
-  return __longlong_as_double(static_cast<long long>(key >> 63 ? key ^ 1ull << 63 : ~key));
+  const uint32_t of_warp = lane < kWarps ? warps[lane] : 0;
+  return make_uint2(sum - v + __reduce_add_sync(0xffffffffu, lane < warp ? of_warp : 0), __reduce_add_sync(0xffffffffu, of_warp));
 }
 
 // The positive part, NaN if x is.  No branches in what follows: lanes would go their own ways element by element (weighing took 6000
@@ -156,30 +151,35 @@ __device__ __forceinline__ int add_up(Number (&sum)[kAhead]) {
 }
 
 // Where the taken pages begin: all those with keys above `high`, and the first `need` of those with keys from `low` to `high`.
+template <typename K>
 struct Border {
-  Key low, high;
+  K low, high;
   uint32_t need;
 };
 
 struct Shared {
   alignas(16) uint32_t bins[3][kBins];
-  // of every warp of the cluster: the most that a page's terms without their signs add up to, as bits; upper halves of keys
+  // of every warp of the cluster: the most that a page's terms without their signs add up to, as bits; keys
   uint32_t bound[kMostBlocks * kWarps], most[kMostBlocks * kWarps], least[kMostBlocks * kWarps];
   uint32_t warps[2][kWarps];
 };
 
+__device__ __forceinline__ int leading_zeros(uint32_t v) { return __clz(v); }
+__device__ __forceinline__ int leading_zeros(Key v) { return __clzll(v); }
+
 // The border of the `need` largest of keys [from, to), which are more than that and lie from `least` to `most`; called by all
 // threads of the block, with bins[0] cleared.
-__device__ __forceinline__ Border find_border(const Key* keys, int from, int to, Key least, Key most, uint32_t need, Shared& sh) {
+template <typename K>
+__device__ __forceinline__ Border<K> find_border(const K* keys, int from, int to, K least, K most, uint32_t need, Shared& sh) {
   const int lane = threadIdx.x & 31;
-  if (need == 0) return {~0ull, ~0ull, 0};
+  if (need == 0) return {static_cast<K>(~K(0)), static_cast<K>(~K(0)), 0};
   for (int round = 0; least != most; ++round) {
-    const Key span = most - least;
-    const int shift = max(0, 56 - __clzll(span));  // span >> shift is below 256
+    const K span = most - least;
+    const int shift = max(0, static_cast<int>(8 * sizeof(K)) - 8 - leading_zeros(span));  // span >> shift is below 256
     uint32_t* const bins = sh.bins[round % 3];
     sh.bins[(round + 1) % 3][threadIdx.x] = 0;  // last read two rounds ago
     for (int i = from + threadIdx.x; i < to; i += kThreads) {
-      const Key place = keys[i] - least;
+      const K place = keys[i] - least;
       if (place <= span) atomicAdd(&bins[place >> shift], 1u);
     }
     __syncthreads();
@@ -208,8 +208,8 @@ __device__ __forceinline__ Border find_border(const Key* keys, int from, int to,
     const uint32_t bin = __shfl_sync(0xffffffffu, kBins - 1 - lane * 8 - nth, owner);
     const uint32_t in_bin = __shfl_sync(0xffffffffu, through - front, owner);
     need = __shfl_sync(0xffffffffu, rest - front, owner);
-    least += static_cast<Key>(bin) << shift;
-    most = min(most, least + ((1ull << shift) - 1));
+    least += static_cast<K>(bin) << shift;
+    most = min(most, least + ((K(1) << shift) - 1));
     if (in_bin == need) break;
   }
   return {least, most, need};
@@ -218,7 +218,8 @@ __device__ __forceinline__ Border find_border(const Key* keys, int from, int to,
 // LANES: side by side on a box, 8 elements each.
 template <typename T, int LANES>
 __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant__ SelectParams p) {
-  extern __shared__ Key keys[];  // of all pages; the first block's are used
+  extern __shared__ Key keys64[];  // of all pages, of which the scores in 64 bits are needed; the first block's are used
+  uint32_t* const keys = reinterpret_cast<uint32_t*>(keys64 + p.table_width);  // of all pages, in 32 bits
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = cluster.num_blocks(), part = cluster.block_rank(), segment = blockIdx.x / parts;
@@ -263,9 +264,9 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
     float weight[8];
     uint4 largest = make_uint4(0, 0, 0, 0);  // of the lane's elements of all boxes, without their signs
     bool finite = true;
-    uint32_t key_most = 0, key_least = ~0u;  // upper halves
+    uint32_t key_most = 0, key_least = ~0u;
     weigh<T>(p, row, kv * group, group, d, upper, mine, weight);
-    Key* const shared_keys = parts > 1 ? cluster.map_shared_rank(keys, 0) : keys;
+    uint32_t* const shared_keys = parts > 1 ? cluster.map_shared_rank(keys, 0) : keys;
     bool waited = parts == 1;
     for (; base < to; base += step) {
       uint4 box[kAhead];
@@ -292,11 +293,11 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
         cluster_wait_begun();
         waited = true;
       }
-      const Key key = real(where) ? ordered(static_cast<double>(sum[0])) : 0;
+      const uint32_t key = real(where) ? ordered(sum[0]) : 0;
       const bool there = holder & (base + nth < to);
       if (there) shared_keys[base + nth] = key;
-      key_most = max(key_most, there ? static_cast<uint32_t>(key >> 32) : 0u);
-      key_least = min(key_least, there ? static_cast<uint32_t>(key >> 32) : ~0u);
+      key_most = max(key_most, there ? key : 0u);
+      key_least = min(key_least, there ? key : ~0u);
       finite &= fabsf(sum[0]) < INFINITY;
     }
     if (!waited) cluster_wait_begun();
@@ -332,67 +333,74 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
   key_most = __reduce_max_sync(0xffffffffu, key_most);
   key_least = __reduce_min_sync(0xffffffffu, key_least);
   const float bound = __uint_as_float(__reduce_max_sync(0xffffffffu, bound_bits));
-  Border border = find_border(keys, from, to, static_cast<Key>(key_least) << 32, static_cast<Key>(key_most) << 32 | 0xffffffffu, wanted, sh);
-  if (wanted > 0) {
-    // Off by at most: a rounding for each of a lane's 4 products and sums, one for their sum, 5 over lanes and one for every query head,
-    // relative to the terms without their signs; and products below the smallest numbers.
-    const double error = bound * (group + 16.0) * 0x1p-24 + 1e-40;
-    const Key minus = ordered(-INFINITY), plus = ordered(INFINITY);  // keys below are pages that are not the cache's
-    Key low = border.low <= minus ? 0 : ordered(number(border.low) - 2 * error);
-    Key high = border.high <= minus ? minus : border.high >= plus ? ~0ull : ordered(number(border.high) + 2 * error);
-    if (!(bound < INFINITY)) low = 0, high = ~0ull;
-    // keys above `high` are taken, those from `low` on near or taken
-    uint32_t counts = 0;
-    for (int i = from + threadIdx.x; i < to; i += kThreads) counts += keys[i] >= low ? 1u : 0u;
-    counts = sum_of_all(counts, sh.warps[0]);
-    border = {low, ~0ull, wanted};  // if all that are near are taken
-    if (counts != wanted) {
-      double weight[8];
-      weigh<T>(p, row, kv * group, group, d, upper, mine, weight);
-      for (int base = from + warp * kBatch; base < to; base += kWarps * kBatch) {
-        const bool inside = lane < kBatch && base + lane < to;
-        const Key old = inside ? keys[base + lane] : 0;
-        const bool near = inside & (old >= low) & (old <= high);
-        if (__any_sync(0xffffffffu, near)) {
-          const int at = look_up(base);
-          uint4 box[kAhead];
-          request(at, box);
-          double sum[kAhead];
-#pragma unroll
-          for (int u = 0; u < kAhead; ++u) {
-            float x[8];
-            unpack<T>(box[u], x);
-            sum[u] = 0.0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum[u] = fma(static_cast<double>(x[i]), weight[i], sum[u]);
-          }
-          const int nth = add_up<LANES>(sum) * kSides + side, where = __shfl_sync(0xffffffffu, at, nth);
-          const bool near_there = __shfl_sync(0xffffffffu, near, nth);
-          if (holder && base + nth < to && near_there) keys[base + nth] = real(where) ? ordered(sum[0]) : 0;
-        }
-        if (inside && !near) keys[base + lane] = old > high ? ~0ull : 0;
-      }
-      sh.bins[0][threadIdx.x] = 0;
-      __syncthreads();
-      border = find_border(keys, from, to, 0, ~0ull, wanted, sh);
-    }
-  }
+  const Border<uint32_t> border = find_border(keys, from, to, key_least, key_most, wanted, sh);
+  // Off by at most: a rounding for each of a lane's 4 products and sums, one for their sum, 5 over lanes and one for every query head,
+  // relative to the terms without their signs; and products below the smallest numbers.  The border is off by no more than a page's score.
+  const float twice = __fmaf_ru(bound, (group + 16.f) * 0x1p-23f, 1e-40f);
+  const uint32_t minus = ordered(-INFINITY), plus = ordered(INFINITY);  // keys below are pages that are not the cache's
+  uint32_t low = border.low <= minus ? 0 : ordered(__fsub_rd(number(border.low), twice));
+  uint32_t high = border.high <= minus ? minus : border.high >= plus ? ~0u : ordered(__fadd_ru(number(border.high), twice));
+  if (!(bound < INFINITY)) low = 0, high = ~0u;
+  if (wanted == 0) low = high = ~0u;
 
   // ---- the chosen pages in order: every thread a run of them
   const int each = (pages + kThreads - 1) / kThreads, begin = threadIdx.x * each, end = min(pages, begin + each);
+  {
+    // keys above `high` are taken, those from `low` on near or taken: if they are no more than are wanted, these are they
+    const auto taken = [&](int i) { return (i < from) | (i >= to) | ((keys[i] >= low) & (wanted != 0)); };
+    uint32_t mine_taken = 0;
+    for (int i = begin; i < end; ++i) mine_taken += taken(i);
+    const uint2 counts = add_in_order(mine_taken, sh.warps[0]);
+    if (counts.y == p.count) {
+      int32_t* next = chosen + counts.x;
+      for (int i = begin; i < end; ++i)
+        if (taken(i)) *next++ = i;
+      return;
+    }
+  }
+  {
+    double weight[8];
+    weigh<T>(p, row, kv * group, group, d, upper, mine, weight);
+    for (int base = from + warp * kBatch; base < to; base += kWarps * kBatch) {
+      const bool inside = lane < kBatch && base + lane < to;
+      const uint32_t old = inside ? keys[base + lane] : 0;
+      const bool near = inside & (old >= low) & (old <= high);
+      if (__any_sync(0xffffffffu, near)) {
+        const int at = look_up(base);
+        uint4 box[kAhead];
+        request(at, box);
+        double sum[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          float x[8];
+          unpack<T>(box[u], x);
+          sum[u] = 0.0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum[u] = fma(static_cast<double>(x[i]), weight[i], sum[u]);
+        }
+        const int nth = add_up<LANES>(sum) * kSides + side, where = __shfl_sync(0xffffffffu, at, nth);
+        const bool near_there = __shfl_sync(0xffffffffu, near, nth);
+        if (holder && base + nth < to && near_there) keys64[base + nth] = real(where) ? ordered(sum[0]) : 0;
+      }
+      if (inside && !near) keys64[base + lane] = old > high ? ~0ull : 0;
+    }
+  }
+  sh.bins[0][threadIdx.x] = 0;
+  __syncthreads();
+  const Border<Key> exact = find_border(keys64, from, to, Key(0), ~Key(0), wanted, sh);
   // above in the lower half, equal in the upper one; keys outside [from, to) are whatever they are
   const auto kind = [&](int i) {
-    const Key key = keys[i];
+    const Key key = keys64[i];
     const bool forced = (i < from) | (i >= to);
-    return forced | (key > border.high) ? 1u : key >= border.low ? 1u << 16 : 0u;
+    return forced | (key > exact.high) ? 1u : key >= exact.low ? 1u << 16 : 0u;
   };
   uint32_t counts = 0;
   for (int i = begin; i < end; ++i) counts += kind(i);
-  const uint32_t front = sum_in_front(counts, sh.warps[1]);
+  const uint32_t front = add_in_order(counts, sh.warps[1]).x;
   uint32_t higher = front & 0xffffu, same = front >> 16;
   for (int i = begin; i < end; ++i) {
     const uint32_t here = kind(i), is_above = here & 1u, is_equal = here >> 16;
-    if (is_above | (is_equal & (same < border.need))) chosen[higher + min(same, border.need)] = i;
+    if (is_above | (is_equal & (same < exact.need))) chosen[higher + min(same, exact.need)] = i;
     higher += is_above;
     same += is_equal;
   }
@@ -401,7 +409,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
 template <typename T, int LANES>
 int launch(const SelectParams& p, cudaStream_t stream) {
   const auto kern = select_kernel<T, LANES>;
-  const size_t smem = static_cast<size_t>(std::max(p.table_width, 1)) * sizeof(Key);
+  const size_t smem = static_cast<size_t>(std::max(p.table_width, 1)) * (sizeof(Key) + sizeof(uint32_t));
   if (smem > 40 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return static_cast<int>(e);
