@@ -57,14 +57,14 @@ __device__ __forceinline__ void load_if(uint4& v, const void* p, bool there) {
       : "l"(p), "r"(static_cast<int>(there))
       : "memory");
 }
-// The same for what this SM reads once.
-__device__ __forceinline__ void load_once_if(uint4& v, const void* p, bool there) {
+// The same for what this SM reads once, where `index` is not negative.
+__device__ __forceinline__ void load_once_if(uint4& v, const void* p, int index) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
+      "setp.ge.s32 p, %5, 0;\n\t"
       "@p ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
       : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
-      : "l"(p), "r"(static_cast<int>(there))
+      : "l"(p), "r"(index)
       : "memory");
 }
 

@@ -202,7 +202,7 @@ struct Walk {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
             load_once_if(kr[r][i][h], k_lane + c.k + 8 * r * p.dim + i * 64 + h * 32,
-                         g + 8 * r < c.valid && i * 64 + h * 32 + q * 8 < p.dim);
+                         g + 8 * r < c.valid && i * 64 + h * 32 + q * 8 < p.dim ? 0 : -1);
     };
     const auto request_v = [&](const Chunk& c) {
       if (c.valid < kChunk) clear(vr);
@@ -211,7 +211,7 @@ struct Walk {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
           const int t = (r & 1) + (r & 2) * 4;
-          load_once_if(vr[r][i], v_lane + c.v + t * p.dim + i * 64, 2 * q + t < c.valid && i * 64 + g * 8 < p.dim);
+          load_once_if(vr[r][i], v_lane + c.v + t * p.dim + i * 64, 2 * q + t < c.valid && i * 64 + g * 8 < p.dim ? 0 : -1);
         }
     };
 

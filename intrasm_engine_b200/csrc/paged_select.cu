@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
     for (int u = 0; u < kAhead; ++u) {
       const int where = __shfl_sync(0xffffffffu, at, u * kSides + side);
       box[u] = make_uint4(0, 0, 0, 0);
-      load_once_if(box[u], boxes + where * box_stride, mine && real(where));
+      load_once_if(box[u], boxes + where * box_stride, mine && real(where) ? 0 : -1);
     }
   };
   const bool holder = along % (LANES / kAhead) == 0;  // one lane for each box that is added up
