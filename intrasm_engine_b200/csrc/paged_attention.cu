@@ -508,45 +508,51 @@ __global__ void __launch_bounds__(32 * warps_of(PIECES, NT), 1) attention_kernel
   __syncthreads();
   grid_launch_dependents();
 
-  // ---- parts of one segment that several warps have
-  int opened = -1, opened_until = 0;
-  for (int from = 0; from < 2 * kWarps;) {
-    const int segment = segment_of[from / 2][from % 2];
-    if (segment < 0) {
-      ++from;
-      continue;
-    }
-    int until = from + 1, last = from;  // parts [from, last] of the segment, some of them empty
-    for (; until < 2 * kWarps; ++until) {
-      const int other = segment_of[until / 2][until % 2];
-      if (other >= 0 && other != segment) break;
-      if (other >= 0) last = until;
-    }
+  // ---- parts of one segment that several warps have; every warp for itself finds the segments, and joins some of their query heads
+  static_assert(2 * kWarps <= 32, "a lane for each part");
+  const int segment_here = lane < 2 * kWarps ? segment_of[lane / 2][lane % 2] : -1;
+  const uint32_t parts_there = __ballot_sync(0xffffffffu, segment_here >= 0), in_front = parts_there & ((1u << lane) - 1);
+  const int segment_before = __shfl_sync(0xffffffffu, segment_here, in_front != 0 ? 31 - __clz(in_front) : lane);
+  uint32_t starts = __ballot_sync(0xffffffffu, segment_here >= 0 && (in_front == 0 || segment_before != segment_here));
+  int opened = -1, opened_until = 0, turn = warp;  // the first query head that this warp joins
+  while (starts != 0) {
+    const int from = __ffs(starts) - 1, segment = __shfl_sync(0xffffffffu, segment_here, from);
+    starts &= starts - 1;
+    const uint32_t behind = starts != 0 ? ~0u << (__ffs(starts) - 1) : 0u;
+    const uint32_t members = parts_there & (~0u << from) & ~behind;
+    const int last = 31 - __clz(members);
     const bool begins = from % 2 == 1, finished = last % 2 == 0 && ends[last / 2];
     const int seg_row = segment / per_row, seg_part = segment - seg_row * per_row, kv = seg_part / p.parts;
-    const int head0 = kv * group + (seg_part - kv * p.parts) * kHeads, here = min(kHeads, (kv + 1) * group - head0);
-    const int vectors = p.dim / 4;
-    for (int x = threadIdx.x; x < here * vectors; x += kThreads) {
-      const int h = x / vectors, d = (x - h * vectors) * 4;
-      const auto there = [&](int i) { return segment_of[i / 2][i % 2] >= 0; };
-      const Joined j = join(
-          from, last + 1, [&](int i) { return there(i) ? stats_of_warps[i * kHeads + h] : make_float2(-INFINITY, 0.f); },
-          [&](int i) {
-            return there(i) ? *reinterpret_cast<const float4*>(parts_of_warps + (i * kHeads + h) * kPitch + d) : float4{};
-          });
+    const int head0 = kv * group + (seg_part - kv * p.parts) * kHeads, here = min(kHeads, (kv + 1) * group - head0), d = lane * 4;
+    for (; turn < here; turn += kWarps) {
+      const int h = turn;
+      float high = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+      for (uint32_t m = members; m != 0; m &= m - 1) high = fmaxf(high, stats_of_warps[(__ffs(m) - 1) * kHeads + h].x);
+      const float base = high == -INFINITY ? 0.f : high;
+      for (uint32_t m = members; m != 0; m &= m - 1) {
+        const int i = (__ffs(m) - 1) * kHeads + h;
+        const float2 s = stats_of_warps[i];
+        const float4 v = d < p.dim ? *reinterpret_cast<const float4*>(parts_of_warps + i * kPitch + d) : float4{};
+        const float weight = exp2f(s.x - base);
+        sum += s.y * weight;
+        o[0] += v.x * weight;
+        o[1] += v.y * weight;
+        o[2] += v.z * weight;
+        o[3] += v.w * weight;
+      }
       if (begins && finished) {
-        write4<T>(p, seg_row, head0 + h, d, j.sum, j.o[0], j.o[1], j.o[2], j.o[3]);
+        if (d < p.dim) write4<T>(p, seg_row, head0 + h, d, sum, o[0], o[1], o[2], o[3]);
       } else {
         const long long slot = (static_cast<long long>(blockIdx.x) * 2 + begins) * kHeads + h;
-        *reinterpret_cast<float4*>(p.product + slot * kDim + d) = make_float4(j.o[0], j.o[1], j.o[2], j.o[3]);
-        if (d == 0) p.stats[slot] = make_float2(j.high, j.sum);
+        if (d < p.dim) *reinterpret_cast<float4*>(p.product + slot * kDim + d) = make_float4(o[0], o[1], o[2], o[3]);
+        if (lane == 0) p.stats[slot] = make_float2(high, sum);
       }
     }
+    turn -= here;
     if (begins && !finished) {
       opened = segment;
       opened_until = last_block[from / 2];
     }
-    from = until;
   }
   if (threadIdx.x == 0) p.open[blockIdx.x] = make_int2(opened, opened_until);
 }
