@@ -423,6 +423,7 @@ __global__ void __launch_bounds__(32 * warps_of(PIECES, NT), 1) attention_kernel
   __shared__ long long before[kThreads + 1];  // units (of one segment) of the rows in front of a thread's
   __shared__ long long warp_sums[kWarps];
   __shared__ int segment_of[kWarps][2], last_block[kWarps], ends[kWarps];
+  __shared__ int2 place_of[kWarps][2];  // of the segment: row, part of it
   float2* const stats_of_warps = reinterpret_cast<float2*>(parts_of_warps + 2 * kWarps * kHeads * kPitch);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int per_row = p.kv_heads * p.parts, group = p.heads / p.kv_heads;
@@ -449,9 +450,14 @@ __global__ void __launch_bounds__(32 * warps_of(PIECES, NT), 1) attention_kernel
     __syncthreads();
   }
   const long long total = before[kThreads] * per_row;
-  const long long workers = min(static_cast<long long>(gridDim.x) * kWarps, (total + kMinUnits - 1) / kMinUnits);
-  const long long worker = static_cast<long long>(blockIdx.x) * kWarps + warp;
-  const long long begin = worker < workers ? total * worker / workers : 0, end = worker < workers ? total * (worker + 1) / workers : 0;
+  const int workers = static_cast<int>(min(static_cast<long long>(gridDim.x) * kWarps, (total + kMinUnits - 1) / kMinUnits));
+  const int worker = blockIdx.x * kWarps + warp;
+  const bool small = total < 1 << 20;  // products with numbers of workers fit 32 bits
+  const auto share = [&](int w) {      // where the units of worker w begin
+    return small ? static_cast<long long>(static_cast<uint32_t>(total) * static_cast<uint32_t>(w) / static_cast<uint32_t>(workers))
+                 : total * w / workers;
+  };
+  const long long begin = worker < workers ? share(worker) : 0, end = worker < workers ? share(worker + 1) : 0;
 
   // rows that hold nothing
   for (int r = blockIdx.x; r < p.rows; r += gridDim.x)
@@ -464,16 +470,15 @@ __global__ void __launch_bounds__(32 * warps_of(PIECES, NT), 1) attention_kernel
   int row = 0, part_of_row = 0, chunks = 0;  // the segment
   long long at = begin, segment_begin = begin;
   if (begin < end) {
-    int lo = 0, hi = kThreads;  // the last thread whose rows begin at or in front of `begin`
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (before[mid] * per_row <= begin) lo = mid; else hi = mid;
-    }
+    int lo = -1;  // the last thread whose rows begin at or in front of `begin`
+#pragma unroll
+    for (int t = 0; t < kThreads; t += 32) lo += __popc(__ballot_sync(0xffffffffu, before[t + lane] * per_row <= begin));
     row = lo * rows_each;
     long long rest = begin - before[lo] * per_row;
     for (chunks = chunks_of(p, row); rest >= static_cast<long long>(units_of(chunks)) * per_row; chunks = chunks_of(p, ++row))
       rest -= static_cast<long long>(units_of(chunks)) * per_row;
-    part_of_row = static_cast<int>(rest / units_of(chunks));
+    part_of_row = small ? static_cast<int>(static_cast<uint32_t>(rest) / static_cast<uint32_t>(units_of(chunks)))
+                        : static_cast<int>(rest / units_of(chunks));
     segment_begin = begin - (rest - static_cast<long long>(part_of_row) * units_of(chunks));
   }
   while (at < end) {
@@ -492,9 +497,10 @@ __global__ void __launch_bounds__(32 * warps_of(PIECES, NT), 1) attention_kernel
         walk.keep(parts_of_warps + (warp * 2 + slot) * kHeads * kPitch, stats_of_warps + (warp * 2 + slot) * kHeads);
         if (lane == 0) {
           segment_of[warp][slot] = row * per_row + part_of_row;
+          place_of[warp][slot] = make_int2(row, part_of_row);
           if (slot == 0) ends[warp] = stop == chunks;
           // the block whose warp has the segment's last unit
-          else last_block[warp] = static_cast<int>(((segment_begin + units_of(chunks)) * workers - 1) / total / kWarps);
+          else last_block[warp] = static_cast<int>(((segment_begin + units_of(chunks)) * workers - 1) / total) / kWarps;
         }
       }
     }
@@ -514,17 +520,28 @@ __global__ void __launch_bounds__(32 * warps_of(PIECES, NT), 1) attention_kernel
   const uint32_t parts_there = __ballot_sync(0xffffffffu, segment_here >= 0), in_front = parts_there & ((1u << lane) - 1);
   const int segment_before = __shfl_sync(0xffffffffu, segment_here, in_front != 0 ? 31 - __clz(in_front) : lane);
   uint32_t starts = __ballot_sync(0xffffffffu, segment_here >= 0 && (in_front == 0 || segment_before != segment_here));
+  const int most_heads = min(kHeads, group);
   int opened = -1, opened_until = 0, turn = warp;  // the first query head that this warp joins
   while (starts != 0) {
-    const int from = __ffs(starts) - 1, segment = __shfl_sync(0xffffffffu, segment_here, from);
+    const int from = __ffs(starts) - 1;
     starts &= starts - 1;
     const uint32_t behind = starts != 0 ? ~0u << (__ffs(starts) - 1) : 0u;
     const uint32_t members = parts_there & (~0u << from) & ~behind;
     const int last = 31 - __clz(members);
     const bool begins = from % 2 == 1, finished = last % 2 == 0 && ends[last / 2];
-    const int seg_row = segment / per_row, seg_part = segment - seg_row * per_row, kv = seg_part / p.parts;
-    const int head0 = kv * group + (seg_part - kv * p.parts) * kHeads, here = min(kHeads, (kv + 1) * group - head0), d = lane * 4;
-    for (; turn < here; turn += kWarps) {
+    if (begins && !finished) {
+      opened = segment_of[from / 2][1];
+      opened_until = last_block[from / 2];
+    }
+    if (turn >= most_heads) {
+      turn -= most_heads;
+      continue;
+    }
+    const int2 place = place_of[from / 2][from % 2];
+    const int seg_row = place.x, kv = p.parts == 1 ? place.y : place.y / p.parts, d = lane * 4;
+    const int head0 = kv * group + (place.y - kv * p.parts) * kHeads, here = min(kHeads, (kv + 1) * group - head0);
+    for (; turn < most_heads; turn += kWarps) {
+      if (turn >= here) continue;
       const int h = turn;
       float high = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
       for (uint32_t m = members; m != 0; m &= m - 1) high = fmaxf(high, stats_of_warps[(__ffs(m) - 1) * kHeads + h].x);
@@ -548,11 +565,7 @@ __global__ void __launch_bounds__(32 * warps_of(PIECES, NT), 1) attention_kernel
         if (lane == 0) p.stats[slot] = make_float2(high, sum);
       }
     }
-    turn -= here;
-    if (begins && !finished) {
-      opened = segment;
-      opened_until = last_block[from / 2];
-    }
+    turn -= most_heads;
   }
   if (threadIdx.x == 0) p.open[blockIdx.x] = make_int2(opened, opened_until);
 }
@@ -623,7 +636,7 @@ __global__ void __launch_bounds__(32 * kClusterWarps, 1) cluster_kernel(const __
 template <typename T, int PIECES, int NT>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ AttentionParams p) {
   constexpr int kHeads = 8 * NT, kDim = 64 * PIECES, kJoinWarps = kJoinThreads / 32;
-  __shared__ float highs[kJoinWarps], sums[kJoinWarps];
+  __shared__ float2 stats[kJoinWarps];
   __shared__ float4 products[kJoinWarps][32];
   grid_dependency_wait();
   grid_launch_dependents();
@@ -635,41 +648,28 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   if (head0 + h >= (kv + 1) * group) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = lane * 4;
   const int n = open.y - static_cast<int>(blockIdx.x) + 1;
-  const auto slot = [&](int i) { return (static_cast<long long>(blockIdx.x + i) * 2 + (i == 0)) * kHeads + h; };
-  float high = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += kJoinThreads) high = fmaxf(high, p.stats[slot(i)].x);
-  for (int s = 16; s > 0; s >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, s));
-  if (lane == 0) highs[warp] = high;
-  __syncthreads();
-  for (int w = 0; w < kJoinWarps; ++w) high = fmaxf(high, highs[w]);
-  const float base = high == -INFINITY ? 0.f : high;
-  float sum = 0.f;
+  // every warp joins a quarter of the parts, and the first one the quarters
+  float high = -INFINITY, sum = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i = warp; i < n; i += kJoinWarps) {
-    const float2 s = p.stats[slot(i)];
-    const float weight = exp2f(s.x - base);
-    sum += s.y * weight;
-    if (d < p.dim) {
-      const float4 v = *reinterpret_cast<const float4*>(p.product + slot(i) * kDim + d);
-      o.x += v.x * weight;
-      o.y += v.y * weight;
-      o.z += v.z * weight;
-      o.w += v.w * weight;
-    }
+    const long long slot = (static_cast<long long>(blockIdx.x + i) * 2 + (i == 0)) * kHeads + h;
+    const float2 s = p.stats[slot];
+    const float4 v = *reinterpret_cast<const float4*>(p.product + slot * kDim + (d < p.dim ? d : 0));
+    const float next = fmaxf(high, s.x), base = next == -INFINITY ? 0.f : next;
+    const float old = exp2f(high - base), weight = exp2f(s.x - base);
+    high = next;
+    sum = sum * old + s.y * weight;
+    o.x = o.x * old + v.x * weight;
+    o.y = o.y * old + v.y * weight;
+    o.z = o.z * old + v.z * weight;
+    o.w = o.w * old + v.w * weight;
   }
-  if (lane == 0) sums[warp] = sum;
+  if (lane == 0) stats[warp] = make_float2(high, sum);
   products[warp][lane] = o;
   __syncthreads();
   if (warp != 0 || d >= p.dim) return;
-  for (int w = 1; w < kJoinWarps; ++w) {
-    const float4 v = products[w][lane];
-    sum += sums[w];
-    o.x += v.x;
-    o.y += v.y;
-    o.z += v.z;
-    o.w += v.w;
-  }
-  write4<T>(p, row, head0 + h, d, sum, o.x, o.y, o.z, o.w);
+  const Joined j = join(0, kJoinWarps, [&](int i) { return stats[i]; }, [&](int i) { return products[i][lane]; });
+  write4<T>(p, row, head0 + h, d, j.sum, j.o[0], j.o[1], j.o[2], j.o[3]);
 }
 
 // Query heads of a segment: 8, or 16 where a key head has more than 8.
@@ -683,15 +683,18 @@ size_t product_bytes(int heads, int head_dim) {
 
 // Blocks of a cluster for each segment, or 0 for attention_kernel; from the most that the rows could hold.
 //
-// A launch of attention_kernel, with join_kernel behind it, costs about kSaved us more than a cluster kernel's, which in turn leaves SMs
-// idle and is as uneven as the rows.
-int cluster_blocks(long long segments, long long most_chunks, int head_dim) {
-  constexpr double kSaved = 4.0, kRate = 6.5e6;  // bytes a us
+// attention_kernel with join_kernel behind it takes 13 us before anything is read (how the work is shared out, joining twice), a
+// cluster 6; but it keeps all SMs busy until the end, where clusters leave some idle and last as long as the longest row.
+// Rows are taken to hold kFill of the most on average, with listed pages all.  Measured, attention_kernel / clusters, us: 1 row of 500, 32
+// heads 14.9 / 5.9; 4 rows up to 4096, 8 key heads 17.4 / 15.9; 16 rows of 32 listed pages of 64 29.0 / 27.7; 1 row of 16384, 8 key heads
+// 20.1 / 26.2; 32 rows up to 8192, one key head 27.2 / 33.0.
+int cluster_blocks(long long segments, long long most_chunks, int head_dim, bool listed) {
+  constexpr double kSaved = 7.0, kFill = 0.65, kRate = 6.5e6;  // us, -, bytes a us
   if (segments > kNumSMs) return 0;
   int blocks = 1;
   while (blocks < kMostBlocks && segments * blocks * 2 <= kNumSMs && most_chunks > blocks * kClusterWarps) blocks *= 2;
   const double us = segments * static_cast<double>(most_chunks) * kChunk * head_dim * 4 / kRate;
-  return us * (static_cast<double>(kNumSMs) / (segments * blocks) - 1.0) < kSaved ? blocks : 0;
+  return us * (static_cast<double>(kNumSMs) / (segments * blocks) - (listed ? 1.0 : kFill)) < kSaved ? blocks : 0;
 }
 
 template <typename Kernel>
@@ -761,7 +764,7 @@ extern "C" size_t iex_paged_attention_workspace_bytes(int rows, int heads, int k
   using namespace iex::paged;
   if (rows <= 0 || table_width < 0 || count < 0 || !iex_paged_attention_supported(heads, kv_heads, head_dim, page_size)) return 0;
   const Extent e = extent(rows, heads, kv_heads, page_size, table_width, listed != 0, count);
-  if (cluster_blocks(e.segments, e.chunks, head_dim) > 0) return 0;
+  if (cluster_blocks(e.segments, e.chunks, head_dim, listed != 0) > 0) return 0;
   const int n = segment_heads(heads, kv_heads);
   return open_bytes() + stats_bytes(n) + product_bytes(n, head_dim);
 }
@@ -795,7 +798,7 @@ extern "C" int iex_paged_attention(int rows, int heads, int kv_heads, int head_d
   p.table_width = table_width;
   p.count = count;
   p.parts = (heads / kv_heads + segment - 1) / segment;
-  p.blocks = cluster_blocks(e.segments, e.chunks, head_dim);
+  p.blocks = cluster_blocks(e.segments, e.chunks, head_dim, pages != nullptr);
   p.q = {q, q_row, q_head};
   p.k_cache = k_cache;
   p.v_cache = v_cache;
