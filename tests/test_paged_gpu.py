@@ -92,6 +92,30 @@ def test_what_is_not_finite_reaches_the_rows_that_hold_it():
     assert clean[2, :3].all() and not clean[2, 3].any()
 
 
+@pytest.mark.parametrize("dtype", U.DTYPES)
+def test_infinite_values_among_many_rows(dtype):
+    """More segments than there are blocks; what is infinite is at the largest score, at a small one, and twice of opposite signs."""
+    lengths = [300] * 30 + [17] * 30
+    q, k, v, table, held = case(lengths, 8, 8, 64, 32, dtype)
+    ref, bound = U.attention(q, k, v, table, lengths)
+    scores = torch.stack([k[table[7].long()[:10], 2].reshape(-1, 64)[:300].float() @ q[7, 2].float()])[0]
+    best, worst = int(scores.argmax()), int(scores.argmin())
+    def put(row, head, position, element, value):
+        v[int(table[row, position // 32]), head, position % 32, element] = value
+    put(7, 2, best, 5, float("inf"))
+    put(7, 2, worst, 6, float("-inf"))
+    put(40, 1, 3, 0, float("inf"))
+    put(40, 1, 16, 0, float("-inf"))
+    put(40, 1, 16, 1, float("-inf"))
+    got = paged.paged_attention(q, k, v, table, held).cpu().double()
+    assert got[7, 2, 5] == float("inf") and got[7, 2, 6] == float("-inf")
+    assert torch.isnan(got[40, 1, 0]) and got[40, 1, 1] == float("-inf")
+    keep = torch.isfinite(got)
+    assert int((~keep).sum()) == 4
+    bound = bound + U.unit(dtype) * (ref.abs() + bound) + 1e-7
+    assert ((got - ref).abs() <= bound)[keep].all()
+
+
 def test_scores_of_minus_infinity_weigh_nothing():
     q, k, v, table, held = case([150, 40], 2, 1, 64, 16, BF16)
     q.fill_(1.0)
@@ -190,6 +214,63 @@ def test_attention_over_listed_pages(heads, kv_heads, dim, page, dtype):
     U.check_attention(paged.paged_attention(q, k, v, table, held, pages=every), q, k, v, table, lengths)
 
 
+@pytest.mark.parametrize("rows,kv_heads,group,dim,dtype", [(700, 1, 1, 64, F16), (1500, 3, 2, 128, BF16), (9000, 32, 1, 64, F16), (900, 2, 9, 72, BF16)])
+def test_attention_of_many_rows_that_share_a_table(rows, kv_heads, group, dim, dtype):
+    """More rows than a block has threads, and, in the third case, more work than 32 bits of products hold."""
+    gen = torch.Generator(device=DEV).manual_seed(rows)
+    page, width = 16, 9
+    k, v = (torch.randn(width + 2, kv_heads, page, dim, device=DEV, generator=gen).to(dtype) for _ in range(2))
+    pages = torch.randperm(width + 2, device=DEV, generator=gen)[:width].to(torch.int32)
+    table = pages.expand(rows, width).contiguous()
+    held = torch.randint(0, width * page + 1, (rows,), device=DEV, generator=gen).to(torch.int32)
+    held[::7] = 0
+    q = torch.randn(rows, kv_heads * group, dim, device=DEV, generator=gen).to(dtype)
+    got = paged.paged_attention(q, k, v, table, held).double()
+    keys, values = (t[pages.long()].transpose(0, 1).reshape(kv_heads, width * page, dim).double() for t in (k, v))
+    scores = torch.einsum("rhgd,hsd->rhgs", q.double().view(rows, kv_heads, group, dim), keys) * dim ** -0.5
+    seen = (torch.arange(width * page, device=DEV) < held[:, None])[:, None, None]
+    weights = torch.softmax(scores.masked_fill(~seen, -1e30), -1) * seen
+    ref = torch.einsum("rhgs,hsd->rhgd", weights, values).reshape(q.shape)
+    size = torch.einsum("rhgs,hsd->rhgd", weights, values.abs()).reshape(q.shape)
+    # scores below 40 without their signs: exponents off by 2 (dim + 3) 2^-23 40, above the line and below (paged_util.attention)
+    loss = 2 * (2 * (dim + 3) * 2.0 ** -23 * 40) + 2.0 ** -16 + width * page * 2.0 ** -23
+    assert float(torch.einsum("rhgd,hsd->rhgs", q.double().abs().view(rows, kv_heads, group, dim), keys.abs()).max()) * dim ** -0.5 < 40
+    assert ((got - ref).abs() <= loss * size + U.unit(dtype) * (ref.abs() + loss * size) + 1e-7).all()
+    assert not got[held == 0].any()
+
+
+def test_attention_of_sequences_with_a_common_beginning():
+    lengths = [100, 77, 64]
+    q, k, v, table, held = case(lengths, 4, 2, 64, 16, F16)
+    table[1, :3] = table[0, :3]
+    table[2, :4] = table[0, :4]
+    U.check_attention(paged.paged_attention(q, k, v, table, held), q, k, v, table, lengths)
+
+
+def test_attention_does_not_depend_on_what_scratch_memory_held():
+    for lengths, heads, kv_heads in (([3000, 200, 0, 1500], 16, 4), ([200] * 200, 8, 8), ([500], 32, 32)):
+        q, k, v, table, held = case(lengths, heads, kv_heads, 128, 64, BF16)
+        ref = paged.paged_attention(q, k, v, table, held)
+        for value in (float("nan"), float("inf"), -1.0):
+            junk = [torch.full((1 << 18,), value, device=DEV) for _ in range(24)]
+            del junk
+            assert torch.equal(paged.paged_attention(q, k, v, table, held), ref)
+
+
+def test_operators_on_another_device_than_the_current_one():
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    lengths = [700, 90]
+    q, k, v, table, held = case(lengths, 8, 2, 64, 32, F16)
+    boxes = U.boxes_of(k, table, lengths, 32)
+    one = paged.paged_attention(q, k, v, table, held), paged.paged_select(q, boxes, table, held, 32, 4)
+    other = [t.to("cuda:1") for t in (q, k, v, table, held, boxes)]
+    two = paged.paged_attention(*other[:5]), paged.paged_select(other[0], other[5], other[3], other[4], 32, 4)
+    assert all(torch.equal(a, b.to(DEV)) for a, b in zip(one, two))
+    with pytest.raises(RuntimeError):
+        paged.paged_attention(q, *other[1:5])
+
+
 def test_attention_refuses():
     q, k, v, table, held = case([50, 20], 4, 2, 64, 16, F16)
     def refused(q=q, k=k, v=v, table=table, held=held, **kwargs):
@@ -281,6 +362,36 @@ def test_selection_of_scores_that_are_not_finite():
     for count in (1, 2, 3, 4, 5, 97, 98, 99):
         got = paged.paged_select(q, boxes, table, held, 16, count, 0, 0)
         assert torch.equal(got.cpu(), U.select(q, boxes, table, lengths, 16, count, 0, 0)), count
+
+
+def test_selection_by_queries_that_are_not_finite():
+    lengths = [1600] * 4
+    q, k, v, table, held = case(lengths, 4, 2, 64, 16, F16)
+    boxes = U.boxes_of(k, table, lengths, 16)
+    q[0, 0, 3] = float("nan")
+    q[1, 3, 5] = float("inf")
+    q[2, 1, :] = float("-inf")
+    q[3] *= 20000.0
+    for count in (2, 9, 99):
+        got = paged.paged_select(q, boxes, table, held, 16, count)
+        assert torch.equal(got.cpu(), U.select(q, boxes, table, lengths, 16, count, 1, 1)), count
+
+
+@pytest.mark.parametrize("dtype", U.DTYPES)
+def test_selection_of_whole_numbers(dtype):
+    """Scores that are often equal, of both signs, at random sizes: the border is in the middle of equal ones."""
+    import random
+    rng = random.Random(21)
+    for turn in range(25):
+        kv_heads, group, dim = rng.choice([1, 2, 5]), rng.choice([1, 3, 4, 9]), 8 * rng.randint(1, 16)
+        lengths = [rng.randint(0, 6000) for _ in range(rng.randint(1, 4))]
+        q, k, v, table, held = case(lengths, kv_heads * group, kv_heads, dim, 16, dtype, seed=turn)
+        boxes = (U.boxes_of(k, table, lengths, 16) * rng.choice([1.0, 2.0])).round()
+        q = (q * rng.choice([0.0, 1.0, 2.0])).round()
+        count, first = rng.randint(2, 60), rng.randint(0, 1)
+        last = rng.randint(0, count - first)
+        got = paged.paged_select(q, boxes, table, held, 16, count, first, last)
+        assert torch.equal(got.cpu(), U.select(q, boxes, table, lengths, 16, count, first, last)), turn
 
 
 def test_selection_is_bounded_and_refuses():
