@@ -1,6 +1,7 @@
 /*
  * iex_b200 — C ABI of the B200 (sm_100a) implementation of intrasm_engine's hot path:
- * CSR SpMM, SDDMM, the dense fp16 linear and the fused sparse||dense layer.
+ * CSR SpMM, SDDMM, the dense fp16 linear and the fused sparse||dense layer; and of a paged
+ * key-value cache for decoding beside it.
  *
  * Plain pointers and sizes only.  All pointers are device pointers unless a comment says
  * "host".  `stream` is a cudaStream_t passed as void* (NULL = the legacy default stream).
