@@ -119,6 +119,11 @@ __device__ __forceinline__ int chunks_of(const AttentionParams& p, int row) {
   return min(p.count, pages) << (p.page_shift - 4);
 }
 
+// A page of a row: its place in the cache and in the row of the table.
+struct PageOfLane {
+  int at, nth;
+};
+
 // What a warp has of a segment: of its chunks [first, stop), for the 8 NT query heads from head0.
 //   PIECES: of 64 elements of a head; NT: groups of 8 query heads
 template <typename T, int PIECES, int NT>
@@ -126,9 +131,10 @@ struct Walk {
   static constexpr int kHeads = 8 * NT, kDim = 64 * PIECES, kPitch = kDim + 4;
   float o[NT][PIECES][4][4], top[NT][2], sum[NT][2];
 
-  // `scratch`: kHeads x kPitch of shared memory that is this warp's; `here`: query heads that there are
+  // `scratch`: kHeads x kPitch of shared memory that is this warp's; `here`: query heads that there are; `early`: the lane's page of the
+  // first 32, looked up before the row's length was known
   __device__ __forceinline__ void run(const AttentionParams& p, int row, int kv, int head0, int here, int first, int stop, int chunks,
-                                      float* scratch) {
+                                      float* scratch, const PageOfLane* early = nullptr) {
     const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3, page = 1 << p.page_shift, sub_shift = p.page_shift - 4;
     const long long head_stride = static_cast<long long>(page) * p.dim;
     const uint4 none = make_uint4(0, 0, 0, 0);
@@ -231,7 +237,13 @@ struct Walk {
       }
       clear_k();
       clear(vr);
-      look_up(first >> sub_shift);
+      if (early != nullptr && first >> sub_shift < 32) {
+        entry0 = 0;
+        page_nth = early->nth;
+        page_at = lane < (chunks + (1 << sub_shift) - 1) >> sub_shift && page_nth < held_pages && early->at < p.num_pages ? early->at : -1;
+      } else {
+        look_up(first >> sub_shift);
+      }
       Chunk now = locate(first);
       request_k(now);
       request_v(now);
@@ -587,6 +599,11 @@ __global__ void __launch_bounds__(32 * kClusterWarps, 1) cluster_kernel(const __
   const int head0 = kv * group + (part - kv * p.parts) * kHeads, here = min(kHeads, (kv + 1) * group - head0);
   grid_dependency_wait();
   grid_launch_dependents();
+  // the first 32 pages, beside the length
+  const int lane = threadIdx.x & 31;
+  PageOfLane early{-1, lane};
+  if (p.pages != nullptr) early.nth = lane < p.count ? p.pages[(static_cast<long long>(row) * p.kv_heads + kv) * p.count + lane] : -1;
+  if (early.nth >= 0 && early.nth < p.table_width) early.at = p.table[static_cast<long long>(row) * p.table_width + early.nth];
   const int chunks = chunks_of(p, row), vectors = p.dim / 4;
   if (chunks == 0) {
     for (int x = threadIdx.x; rank == 0 && x < here * vectors; x += kThreads)
@@ -600,7 +617,7 @@ __global__ void __launch_bounds__(32 * kClusterWarps, 1) cluster_kernel(const __
     W walk;
     float* const mine = parts_of_warps + warp * kHeads * kPitch;
     walk.run(p, row, kv, head0, here, static_cast<int>(static_cast<long long>(chunks) * worker / workers),
-             static_cast<int>(static_cast<long long>(chunks) * (worker + 1) / workers), chunks, mine);
+             static_cast<int>(static_cast<long long>(chunks) * (worker + 1) / workers), chunks, mine, &early);
     walk.keep(mine, stats_of_warps[warp]);
   }
   __syncthreads();

@@ -32,9 +32,8 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kAhead = 8;         // boxes that a lane has on their way
 constexpr int kMaxPages = 16384;  // 12 bytes of shared memory each
-constexpr int kBins = 256;
-constexpr int kMostBlocks = 8;  // of a cluster
-static_assert(kThreads == kBins, "a thread clears a bin");
+constexpr int kBits = 10, kBins = 1 << kBits;  // of a round
+constexpr int kMostBlocks = 8;                 // of a cluster
 
 struct SelectParams {
   int rows, heads, kv_heads, dim, num_pages, page_shift, table_width, count, first, last;
@@ -158,7 +157,7 @@ struct Border {
 };
 
 struct Shared {
-  alignas(16) uint32_t bins[3][kBins];
+  uint32_t bins[3][kBins], groups[3][32];  // keys in a bin, in 32 bins
   // of every warp of the cluster: the most that a page's terms without their signs add up to, as bits; keys
   uint32_t bound[kMostBlocks * kWarps], most[kMostBlocks * kWarps], least[kMostBlocks * kWarps];
   uint32_t warps[2][kWarps];
@@ -167,47 +166,51 @@ struct Shared {
 __device__ __forceinline__ int leading_zeros(uint32_t v) { return __clz(v); }
 __device__ __forceinline__ int leading_zeros(Key v) { return __clzll(v); }
 
+__device__ __forceinline__ void clear_bins(Shared& sh, int which) {
+#pragma unroll
+  for (int i = 0; i < kBins; i += kThreads) sh.bins[which][i + threadIdx.x] = 0;
+  if (threadIdx.x < 32) sh.groups[which][threadIdx.x] = 0;
+}
+
+// Which of 32 numbers, one a lane, the need-th key is in, counted from the last lane down; need becomes its place in there.
+__device__ __forceinline__ int find_lane(uint32_t mine, uint32_t& need, uint32_t& in_lane) {
+  const int lane = threadIdx.x & 31;
+  uint32_t above = mine;
+  for (int d = 1; d < 32; d <<= 1) {
+    const uint32_t other = __shfl_down_sync(0xffffffffu, above, d);
+    above += lane + d < 32 ? other : 0;
+  }
+  above -= mine;
+  const int owner = __ffs(__ballot_sync(0xffffffffu, (above < need) & (need <= above + mine))) - 1;
+  in_lane = __shfl_sync(0xffffffffu, mine, owner);
+  need -= __shfl_sync(0xffffffffu, above, owner);
+  return owner;
+}
+
 // The border of the `need` largest of keys [from, to), which are more than that and lie from `least` to `most`; called by all
-// threads of the block, with bins[0] cleared.
+// threads of the block, with the first bins cleared.
 template <typename K>
 __device__ __forceinline__ Border<K> find_border(const K* keys, int from, int to, K least, K most, uint32_t need, Shared& sh) {
   const int lane = threadIdx.x & 31;
   if (need == 0) return {static_cast<K>(~K(0)), static_cast<K>(~K(0)), 0};
   for (int round = 0; least != most; ++round) {
     const K span = most - least;
-    const int shift = max(0, static_cast<int>(8 * sizeof(K)) - 8 - leading_zeros(span));  // span >> shift is below 256
+    const int shift = max(0, static_cast<int>(8 * sizeof(K)) - kBits - leading_zeros(span));  // span >> shift is below kBins
     uint32_t* const bins = sh.bins[round % 3];
-    sh.bins[(round + 1) % 3][threadIdx.x] = 0;  // last read two rounds ago
+    uint32_t* const groups = sh.groups[round % 3];
+    clear_bins(sh, (round + 1) % 3);  // last read two rounds ago
     for (int i = from + threadIdx.x; i < to; i += kThreads) {
       const K place = keys[i] - least;
-      if (place <= span) atomicAdd(&bins[place >> shift], 1u);
+      if (place <= span) {
+        atomicAdd(&bins[place >> shift], 1u);
+        atomicAdd(&groups[place >> shift >> 5], 1u);
+      }
     }
     __syncthreads();
-    // every warp for itself: a lane has 8 bins, the first lane the highest
-    const uint4 upper = *reinterpret_cast<const uint4*>(bins + kBins - 4 - lane * 8);
-    const uint4 lower = *reinterpret_cast<const uint4*>(bins + kBins - 8 - lane * 8);
-    uint32_t sums[8] = {upper.w, upper.z, upper.y, upper.x, lower.w, lower.z, lower.y, lower.x};  // of bins from the highest down
-#pragma unroll
-    for (int j = 1; j < 8; ++j) sums[j] += sums[j - 1];
-    uint32_t above = sums[7];
-    for (int d = 1; d < 32; d <<= 1) {
-      const uint32_t other = __shfl_up_sync(0xffffffffu, above, d);
-      above += lane >= d ? other : 0;
-    }
-    above -= sums[7];
-    const int owner = __ffs(__ballot_sync(0xffffffffu, (above < need) & (need <= above + sums[7]))) - 1;
-    const uint32_t rest = need - above;  // in the owner: of its bins' keys
-    uint32_t nth = 0, front = 0, through = 0xffffffffu;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const bool before = sums[j] < rest;
-      nth += before;
-      front = before ? sums[j] : front;
-      through = min(through, before ? 0xffffffffu : sums[j]);
-    }
-    const uint32_t bin = __shfl_sync(0xffffffffu, kBins - 1 - lane * 8 - nth, owner);
-    const uint32_t in_bin = __shfl_sync(0xffffffffu, through - front, owner);
-    need = __shfl_sync(0xffffffffu, rest - front, owner);
+    // every warp for itself
+    uint32_t in_bin;
+    const int first = find_lane(groups[lane], need, in_bin) * 32;
+    const int bin = first + find_lane(bins[first + lane], need, in_bin);
     least += static_cast<K>(bin) << shift;
     most = min(most, least + ((K(1) << shift) - 1));
     if (in_bin == need) break;
@@ -227,7 +230,17 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
   const int row = segment / p.kv_heads, kv = segment - row * p.kv_heads, group = p.heads / p.kv_heads;
   grid_dependency_wait();
   grid_launch_dependents();
+  constexpr int kSides = 32 / LANES, kBatch = kAhead * kSides;  // pages of a warp's turn
+  const int along = lane % LANES, side = lane / LANES, d0 = along * 8;
+  const bool mine = d0 < 2 * p.dim, upper = d0 >= p.dim;  // upper: of the largest keys
+  const int d = d0 - (upper ? p.dim : 0);
+  const int32_t* const table = p.table + static_cast<long long>(row) * p.table_width;
+  const int from = min(p.first, p.table_width), base0 = from + (part * kWarps + warp) * kBatch;
+  // what does not depend on the length is requested beside it
+  const int at0 = base0 + lane < p.table_width && lane < kBatch ? table[base0 + lane] : -1;
   const int length = held(p.lengths, row, p.table_width, p.page_shift);
+  float weight[8];
+  weigh<T>(p, row, kv * group, group, d, upper, mine, weight);
   const int pages = (length + (1 << p.page_shift) - 1) >> p.page_shift;
   int32_t* const chosen = p.chosen + static_cast<long long>(segment) * p.count;
   if (pages <= p.count) {
@@ -236,14 +249,9 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
     return;
   }
   if (parts > 1) cluster_begun();
-  const int from = p.first, to = pages - p.last;  // those that are chosen by their scores
+  const int to = pages - p.last;  // [from, to): those that are chosen by their scores
 
   // ---- scores
-  constexpr int kSides = 32 / LANES, kBatch = kAhead * kSides;  // pages of a warp's turn
-  const int along = lane % LANES, side = lane / LANES, d0 = along * 8;
-  const bool mine = d0 < 2 * p.dim, upper = d0 >= p.dim;  // upper: of the largest keys
-  const int d = d0 - (upper ? p.dim : 0);
-  const int32_t* const table = p.table + static_cast<long long>(row) * p.table_width;
   const T* const boxes = static_cast<const T*>(p.boxes) + static_cast<long long>(kv) * 2 * p.dim + d0;
   const long long box_stride = static_cast<long long>(p.kv_heads) * 2 * p.dim;
   const auto look_up = [&](int base) { return base + lane < to && lane < kBatch ? table[base + lane] : -1; };
@@ -259,13 +267,11 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
   const bool holder = along % (LANES / kAhead) == 0;  // one lane for each box that is added up
   {
     const int step = parts * kWarps * kBatch;
-    int base = from + (part * kWarps + warp) * kBatch;
-    int at = look_up(base);
-    float weight[8];
+    int base = base0;
+    int at = base + lane < to ? at0 : -1;
     uint4 largest = make_uint4(0, 0, 0, 0);  // of the lane's elements of all boxes, without their signs
     bool finite = true;
     uint32_t key_most = 0, key_least = ~0u;
-    weigh<T>(p, row, kv * group, group, d, upper, mine, weight);
     uint32_t* const shared_keys = parts > 1 ? cluster.map_shared_rank(keys, 0) : keys;
     bool waited = parts == 1;
     for (; base < to; base += step) {
@@ -317,7 +323,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
       first.most[part * kWarps + warp] = key_most;
       first.least[part * kWarps + warp] = key_least;
     }
-    if (part == 0) sh.bins[0][threadIdx.x] = 0;
+    if (part == 0) clear_bins(sh, 0);
   }
   if (parts > 1) cluster.sync(); else __syncthreads();
   if (part != 0) return;
@@ -385,7 +391,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
       if (inside && !near) keys64[base + lane] = old > high ? ~0ull : 0;
     }
   }
-  sh.bins[0][threadIdx.x] = 0;
+  clear_bins(sh, 0);
   __syncthreads();
   const Border<Key> exact = find_border(keys64, from, to, Key(0), ~Key(0), wanted, sh);
   // above in the lower half, equal in the upper one; keys outside [from, to) are whatever they are
