@@ -561,10 +561,12 @@ IEX_API int iex_paged_append(int tokens, int batch, int heads, int kv_heads, int
  * of the table, the first min(count, pages held) entries; entries that are no held page are
  * skipped, one that is there twice counts twice.
  * workspace (or NULL where iex_paged_attention_workspace_bytes is 0; listed: whether there are
- * pages) is scratch of one call: calls that may run at the same time need one each. */
+ * pages) is scratch of one call: calls that may run at the same time need one each.  Up to 512 MB
+ * where rows list so much that the pages of the cache are sorted by who reads them. */
 IEX_API int iex_paged_attention_supported(int heads, int kv_heads, int head_dim, int page_size);
 IEX_API size_t iex_paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim,
-                                                   int page_size, int table_width, int listed, int count);
+                                                   int num_pages, int page_size, int table_width,
+                                                   int listed, int count);
 IEX_API int iex_paged_attention(int rows, int heads, int kv_heads, int head_dim, int bf16,
                                 const void* q, long long q_row, long long q_head,
                                 const void* k_cache, long long k_page, const void* v_cache,

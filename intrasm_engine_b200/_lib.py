@@ -152,8 +152,8 @@ SIGNATURES = {
                                  c_ll, c_ptr, c_ll, c_ptr, c_int, c_int, c_ptr, c_int, c_ptr, c_ptr, c_ptr]),
     # heads kv_heads dim page_size
     "iex_paged_attention_supported": (c_int, [c_int, c_int, c_int, c_int]),
-    # rows heads kv_heads dim page_size table_width listed count
-    "iex_paged_attention_workspace_bytes": (c_size, [c_int] * 8),
+    # rows heads kv_heads dim num_pages page_size table_width listed count
+    "iex_paged_attention_workspace_bytes": (c_size, [c_int] * 9),
     # rows heads kv_heads dim bf16 q+strides k_cache k_page v_cache v_page num_pages page_size table table_width lengths
     # pages count scale out workspace workspace_bytes stream
     "iex_paged_attention": (c_int, [c_int] * 5 + [c_ptr, c_ll, c_ll, c_ptr, c_ll, c_ptr, c_ll, c_int, c_int, c_ptr, c_int,

@@ -46,8 +46,8 @@ struct Rows {
 };
 
 // 16 bytes, where `there`; else v stays as it is.  Not invariant (".nc"): the kernel in front, which may still run when this one
-// starts, can have written what is read, and loads that claim otherwise may be moved ahead of the wait for it.  A predicate and
-// not a branch: behind one, the loads of a row of them were waited for one by one (4 of them 6400 cycles, without it 900).
+// starts, can have written what is read, and loads that claim otherwise may be moved ahead of the wait for it.  A predicate, so
+// that a row of such loads has no branches between them.
 __device__ __forceinline__ void load_if(uint4& v, const void* p, bool there) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"

@@ -9,7 +9,8 @@
 // warps of one block per SM, whatever the rows' lengths, a segment's start counted as kStart chunks; a warp that has a whole segment
 // writes its rows, the others leave maximum, sum and product, which the block joins through shared memory and, where a segment reaches over
 // several blocks, join_kernel joins from the workspace, in order.  Where there are few segments (cluster_kernel): a cluster of blocks for
-// each, joined through distributed shared memory, without workspace or second launch.
+// each, joined through distributed shared memory, without workspace or second launch.  Where many rows list the same pages:
+// paged_shared.cu.
 //
 // A chunk: keys and values come straight from global memory into registers, 16 bytes a lane, the next chunk's keys requested
 // when this one's scores are formed and its values after the product; the lengths of what a warp has on its way (8 KB) and nothing else covers
@@ -26,7 +27,8 @@
 
 #include <cooperative_groups.h>
 
-#include "paged.cuh"
+#include "paged_mma.cuh"
+#include "paged_shared.cuh"
 
 namespace iex {
 namespace paged {
@@ -56,45 +58,6 @@ struct AttentionParams {
   float* product;  // [blocks][2][heads of a segment][dim bucket]  ... 0: began in front of the block, 1: begins in it
 };
 
-template <typename T>
-struct Half2;
-template <>
-struct Half2<__half> {
-  static constexpr float kBias = 15.f;  // weights are 2^15 times as large
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return reinterpret_cast<const uint32_t&>(v);
-  }
-  static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(reinterpret_cast<const __half2&>(v)); }
-};
-template <>
-struct Half2<__nv_bfloat16> {
-  static constexpr float kBias = 0.f;
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return reinterpret_cast<const uint32_t&>(v);
-  }
-  static __device__ __forceinline__ float2 unpack(uint32_t v) {
-    return __bfloat1622float2(reinterpret_cast<const __nv_bfloat162&>(v));
-  }
-};
-
-template <typename T>
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma<__half>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                            uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                                   uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 // The 8 x 8 matrix of 16-bit elements that the warp holds, transposed.
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
   uint32_t t;
@@ -776,10 +739,12 @@ extern "C" int iex_paged_attention_supported(int heads, int kv_heads, int head_d
   return iex::paged::heads_ok(heads, kv_heads, head_dim) && iex::paged::page_size_ok(page_size) ? 1 : 0;
 }
 
-extern "C" size_t iex_paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim, int page_size,
+extern "C" size_t iex_paged_attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim, int num_pages, int page_size,
                                                       int table_width, int listed, int count) {
   using namespace iex::paged;
-  if (rows <= 0 || table_width < 0 || count < 0 || !iex_paged_attention_supported(heads, kv_heads, head_dim, page_size)) return 0;
+  if (rows <= 0 || num_pages < 0 || table_width < 0 || count < 0 || !iex_paged_attention_supported(heads, kv_heads, head_dim, page_size)) return 0;
+  if (listed)
+    if (const size_t bytes = shared_workspace_bytes(rows, heads, kv_heads, head_dim, num_pages, page_size, table_width, count)) return bytes;
   const Extent e = extent(rows, heads, kv_heads, page_size, table_width, listed != 0, count);
   if (cluster_blocks(e.segments, e.chunks, head_dim, listed != 0) > 0) return 0;
   const int n = segment_heads(heads, kv_heads);
@@ -801,8 +766,15 @@ extern "C" int iex_paged_attention(int rows, int heads, int kv_heads, int head_d
       !iex::aligned16(k_cache) || !iex::aligned16(v_cache) || !iex::aligned16(workspace))
     return IEX_ERR_UNSUPPORTED;
   if (static_cast<long long>(rows) * heads > 0x7fffffffll) return IEX_ERR_TOO_LARGE;
-  const size_t need = iex_paged_attention_workspace_bytes(rows, heads, kv_heads, head_dim, page_size, table_width, pages != nullptr, count);
+  const size_t need =
+      iex_paged_attention_workspace_bytes(rows, heads, kv_heads, head_dim, num_pages, page_size, table_width, pages != nullptr, count);
   if (need > 0 && (!workspace || workspace_bytes < need)) return IEX_ERR_BAD_ARG;
+  const float scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  if (pages != nullptr && shared_workspace_bytes(rows, heads, kv_heads, head_dim, num_pages, page_size, table_width, count) > 0) {
+    SharedCall c{rows, heads, kv_heads, head_dim, num_pages, log2_of(page_size), table_width, count, {q, q_row, q_head},
+                 k_cache, v_cache, k_page, v_page, block_table, lengths, pages, scale_log2, out};
+    return shared_attention(c, bf16 != 0, workspace, static_cast<cudaStream_t>(stream));
+  }
   const int segment = segment_heads(heads, kv_heads);
   const Extent e = extent(rows, heads, kv_heads, page_size, table_width, pages != nullptr, count);
   AttentionParams p{};
@@ -824,7 +796,7 @@ extern "C" int iex_paged_attention(int rows, int heads, int kv_heads, int head_d
   p.table = block_table;
   p.lengths = lengths;
   p.pages = pages;
-  p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  p.scale_log2 = scale_log2;
   p.out = out;
   if (need > 0) {
     char* const ws = static_cast<char*>(workspace);

@@ -171,7 +171,7 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
   at::Tensor out = empty(q, {rows, heads, kc.dim});
   if (rows == 0) return out;
   const Operand qo(q);
-  const size_t bytes = iex_paged_attention_workspace_bytes(rows, heads, kc.kv_heads, kc.dim, kc.page_size, block_table.size(1),
+  const size_t bytes = iex_paged_attention_workspace_bytes(rows, heads, kc.kv_heads, kc.dim, kc.pages, kc.page_size, block_table.size(1),
                                                            pages.has_value(), count);
   at::Tensor workspace;
   if (bytes > 0) workspace = empty_bytes(q, bytes);

@@ -239,6 +239,98 @@ def test_attention_of_many_rows_that_share_a_table(rows, kv_heads, group, dim, d
     assert not got[held == 0].any()
 
 
+# rows that list pages of one sequence: where enough of them do, a page is read once for many
+SHARED = [
+    # rows, heads, kv_heads, dim, page, longest, count
+    (300, 36, 4, 80, 128, 31 * 128 - 9, 9),
+    (300, 16, 2, 104, 256, 12 * 256 - 200, 5),
+    (400, 32, 32, 64, 16, 60 * 16, 16),
+    (512, 32, 2, 128, 256, 20 * 256 - 1, 8),
+    (128, 16, 4, 128, 64, 40 * 64 - 5, 8),
+    (400, 4, 4, 64, 16, 60 * 16, 16),
+    (150, 27, 3, 80, 64, 30 * 64 + 1, 9),
+    (140, 10, 2, 128, 128, 20 * 128 - 70, 6),
+    (90, 32, 2, 104, 256, 12 * 256 - 200, 5),
+    (300, 8, 8, 40, 32, 33 * 32 + 7, 20),
+]
+
+
+def shared_case(rows, heads, kv_heads, dim, page, longest, count, dtype, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    k, v, table = U.make_cache(gen, [longest], kv_heads, dim, page, dtype)
+    table = table.expand(rows, -1).contiguous()
+    q = torch.randn(rows, heads, dim, generator=gen).to(dtype).to(DEV)
+    # a piece of a prompt at the end, rows anywhere, and idle ones
+    lengths = [longest - rows // 2 + 1 + i for i in range(rows // 2)]
+    lengths += [int(torch.randint(0, longest + 1, (1,), generator=gen)) for _ in range(rows - len(lengths))]
+    lengths[-1], lengths[rows // 2], lengths[3] = 0, 1, longest
+    lists = torch.full((rows, kv_heads, count), -1, dtype=torch.int32)
+    for i, n in enumerate(lengths):
+        held = (n + page - 1) // page
+        for h in range(kv_heads):
+            some = torch.randperm(held, generator=gen)[:count].sort().values
+            lists[i, h, :len(some)] = some.int()
+    return q, k, v, table, lengths, lists
+
+
+def takes_shared_pages(q, k, table, lists):
+    from intrasm_engine_b200 import _lib
+    need = _lib.lib.iex_paged_attention_workspace_bytes(q.size(0), q.size(1), k.size(1), q.size(2), k.size(0), k.size(2), table.size(1), 1,
+                                                        lists.size(2))
+    return need > 4 << 20  # the other kernels need less
+
+
+@pytest.mark.parametrize("dtype", U.DTYPES)
+@pytest.mark.parametrize("rows,heads,kv_heads,dim,page,longest,count", SHARED)
+def test_attention_over_pages_that_rows_share(rows, heads, kv_heads, dim, page, longest, count, dtype):
+    q, k, v, table, lengths, lists = shared_case(rows, heads, kv_heads, dim, page, longest, count, dtype)
+    assert rows * heads < 8192 or takes_shared_pages(q, k, table, lists)
+    got = paged.paged_attention(q, k, v, table, ints(lengths), pages=lists.to(DEV))
+    U.check_attention(got, q, k, v, table, lengths, pages=lists)
+    assert not got[-1].any()
+    # any order, a page twice, entries that are no page, lengths and tables that are none
+    rough = lists.clone()
+    rough[0, 0] = rough[0, 0].flip(0)
+    rough[1, :, 1] = rough[1, :, 0]
+    rough[2, 0, 0], rough[2, 0, 1] = -7, 2 ** 31 - 1
+    rough[4] = rough[4, :, :1]
+    wild, holes = list(lengths), table.clone()
+    wild[6] = -3
+    holes[7, 0], holes[8, :] = -1, k.size(0)
+    got = paged.paged_attention(q, k, v, holes, ints(wild), pages=rough.to(DEV))
+    U.check_attention(got, q, k, v, holes, wild, pages=rough)
+    assert torch.equal(got, paged.paged_attention(q, k, v, holes, ints(wild), pages=rough.to(DEV)))
+
+
+@pytest.mark.parametrize("dtype", U.DTYPES)
+def test_shared_pages_keep_what_is_not_finite_to_the_rows_that_see_it(dtype):
+    q, k, v, table, lengths, lists = shared_case(128, 16, 4, 128, 64, 40 * 64 - 5, 8, dtype, seed=3)
+    assert takes_shared_pages(q, k, table, lists)
+    ref, bound = U.attention(q, k, v, table, lengths, pages=lists)
+    last = (lengths[3] - 1) // 64
+    lists[:64, :, 0] = last  # the piece of a prompt: all rows list the last page, of which they see more and more
+    lists[:64] = lists[:64].sort(-1).values
+    for i in range(64):
+        for h in range(4):
+            seen = torch.unique(lists[i, h])
+            seen = torch.cat([seen, torch.full((8 - len(seen),), -1, dtype=torch.int32)])
+            lists[i, h] = seen
+    ref, bound = U.attention(q, k, v, table, lengths, pages=lists)
+    spot = lengths[3] - 1 - last * 64 - 20            # seen by rows from some on
+    v[int(table[0, last]), 1, spot, 9] = float("inf")
+    k[int(table[0, last]), 2, spot, 5] = float("nan")
+    got = paged.paged_attention(q, k, v, table, ints(lengths), pages=lists.to(DEV)).cpu().double()
+    expected = torch.isfinite(got)
+    sees = torch.tensor([any(int(x) == last for x in lists[i, 1]) and n > last * 64 + spot for i, n in enumerate(lengths)])
+    assert (got[sees][:, 4:8, 9] == float("inf")).all() and torch.isnan(got[sees][:, 8:12]).all() and 10 < int(sees.sum()) < 64
+    expected[sees, 4:8, 9] = True
+    expected[sees, 8:12] = True
+    assert expected.all()
+    keep = torch.isfinite(got)
+    bound = bound + U.unit(dtype) * (ref.abs() + bound) + 1e-7
+    assert ((got - ref).abs() <= bound)[keep].all()
+
+
 def test_attention_of_sequences_with_a_common_beginning():
     lengths = [100, 77, 64]
     q, k, v, table, held = case(lengths, 4, 2, 64, 16, F16)
