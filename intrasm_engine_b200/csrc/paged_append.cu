@@ -221,7 +221,7 @@ __device__ __forceinline__ bool find_span(const AppendParams& p, int block, Span
   if (p.cu_tokens == nullptr) {
     used = p.tokens;
     if (block >= p.batch) return false;
-    found = {block, block, 1, p.lengths[block], 0};
+    found = {block, block, 1, max(p.lengths[block], 0), 0};
     return true;
   }
   int front = 0;
@@ -232,7 +232,7 @@ __device__ __forceinline__ bool find_span(const AppendParams& p, int block, Span
       begin = min(max(p.cu_tokens[s], 0), p.tokens);
       const int next = min(max(p.cu_tokens[s + 1], 0), p.tokens);
       n = max(0, next - begin);
-      length = p.lengths[s];
+      length = max(p.lengths[s], 0);
       if (s == p.batch - 1) last = next;
     }
     const int mine = n > 0 ? ((n + (1 << p.page_shift) - 2) >> p.page_shift) + 1 : 0;

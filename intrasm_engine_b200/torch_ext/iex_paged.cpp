@@ -73,7 +73,7 @@ void check_table(const at::Tensor& block_table, const at::Tensor& lengths) {
   TORCH_CHECK(block_table.dim() == 2 && lengths.dim() == 1 && block_table.size(0) == lengths.size(0),
               "block_table must be [rows, pages] and lengths [rows]");
   TORCH_CHECK(block_table.is_contiguous() && lengths.is_contiguous(), "block_table and lengths must be contiguous tensors");
-  TORCH_CHECK(block_table.size(1) <= kMostInt, "block_table is too wide");
+  TORCH_CHECK(block_table.size(0) <= kMostInt && block_table.size(1) <= kMostInt, "block_table is too large");
 }
 
 // A cache that is written: what was saved of it before is seen to have changed.
@@ -166,7 +166,7 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
     count = pages->size(2);
   }
   const double factor = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(kc.dim));
-  TORCH_CHECK(std::isfinite(factor), "scale must be finite");
+  TORCH_CHECK(std::isfinite(static_cast<float>(factor)), "scale must be finite in 32 bits");
   c10::cuda::CUDAGuard guard(q.device());
   at::Tensor out = empty(q, {rows, heads, kc.dim});
   if (rows == 0) return out;

@@ -331,6 +331,47 @@ def test_shared_pages_keep_what_is_not_finite_to_the_rows_that_see_it(dtype):
     assert ((got - ref).abs() <= bound)[keep].all()
 
 
+def test_shared_pages_in_graphs_and_whatever_scratch_memory_held():
+    cases = [shared_case(128, 16, 4, 128, 64, 40 * 64 - 5, 8, F16, seed=s) for s in (5, 6)]
+    expected, graphs = [], []
+    for q, k, v, table, lengths, lists in cases:
+        assert takes_shared_pages(q, k, table, lists)
+        held, listed = ints(lengths), lists.to(DEV)
+        expected.append(paged.paged_attention(q, k, v, table, held, pages=listed))
+        U.check_attention(expected[-1], q, k, v, table, lengths, pages=lists)
+        for value in (float("nan"), float("inf"), 0.0):
+            junk = torch.full((1 << 24,), value, device=DEV)
+            del junk
+            assert torch.equal(expected[-1], paged.paged_attention(q, k, v, table, held, pages=listed))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = paged.paged_attention(q, k, v, table, held, pages=listed)
+            out = paged.paged_attention(out, k, v, table, held, pages=listed)
+        graphs.append((graph, out, q, held, listed, paged.paged_attention(expected[-1], k, v, table, held, pages=listed)))
+    for _ in range(3):
+        for graph, out, *_, twice in graphs:
+            out.fill_(float("nan"))
+            graph.replay()
+            assert torch.equal(out, twice)
+    # two streams at once
+    streams, outs = [torch.cuda.Stream() for _ in cases], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for i, (q, k, v, table, _, _) in enumerate(cases):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(paged.paged_attention(q, k, v, table, graphs[i][3], pages=graphs[i][4]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, expected[i]) for o in outs[i])
+
+
+def test_attention_refuses_scales_that_are_not_finite_in_32_bits():
+    q, k, v, table, held = case([50, 20], 4, 2, 64, 16, F16)
+    for scale in (1e300, -1e39, float("nan")):
+        with pytest.raises(RuntimeError):
+            paged.paged_attention(q, k, v, table, held, scale=scale)
+
+
 def test_attention_of_sequences_with_a_common_beginning():
     lengths = [100, 77, 64]
     q, k, v, table, held = case(lengths, 4, 2, 64, 16, F16)
@@ -663,6 +704,20 @@ def test_append_drops_tokens_without_a_place():
     assert not paged.paged_append(q, k, v, k_cache, v_cache, table[:0], ints([]), ints([0])).any()
     assert paged.paged_append(q[:0], k[:0], v[:0], k_cache, v_cache, table[:0], ints([])).shape == (0, 2, 64)
     assert torch.equal(before[0], k_cache) and torch.equal(before[1], v_cache)
+
+
+def test_lengths_below_zero_leave_no_place():
+    gen = torch.Generator().manual_seed(5)
+    k_cache, v_cache, table = U.make_cache(gen, [64, 64], 2, 64, 16, F16, spare=0, fill=0.0)
+    before = k_cache.clone(), v_cache.clone()
+    q, k, v = (torch.randn(6, 2, 64, generator=gen).half().to(DEV) for _ in range(3))
+    for n, cu in ((2, None), (6, ints([0, 4, 6]))):
+        for low in (-2 ** 31, -2 ** 31 + 3, -1, 0):
+            junk = [torch.full_like(q[:n], float("nan")) for _ in range(4)]  # what the output's memory holds, most likely
+            del junk
+            out = paged.paged_append(q[:n], k[:n], v[:n], k_cache, v_cache, table, ints([low, low]), cu)
+            assert torch.equal(out, torch.zeros_like(out)), (n, low)
+            assert torch.equal(before[0], k_cache) and torch.equal(before[1], v_cache)
 
 
 def test_append_refuses():
