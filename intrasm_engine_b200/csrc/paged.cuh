@@ -19,8 +19,11 @@ inline bool page_size_ok(int page_size) {
   return page_size >= kMinPage && page_size <= kMaxPage && (page_size & (page_size - 1)) == 0;
 }
 inline bool heads_ok(int heads, int kv_heads, int head_dim) {
-  return kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && head_dim > 0 && head_dim % 8 == 0 && head_dim <= kMaxHeadDim;
+  return kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && head_dim > 0 && head_dim % 8 == 0 && head_dim <= kMaxHeadDim &&
+         heads <= (1 << 24) - 1;  // a row's elements are counted in 32 bits
 }
+// Positions, rounded up to whole pages, are counted in 32 bits.
+inline bool table_ok(int table_width, int page_size) { return static_cast<long long>(table_width) * page_size <= 0x7fffff00ll; }
 inline int log2_of(int power_of_two) {
   int bits = 0;
   while ((1 << bits) < power_of_two) ++bits;

@@ -419,7 +419,8 @@ extern "C" int iex_paged_append(int tokens, int batch, int heads, int kv_heads, 
   if (tokens < 0 || batch < 0 || num_pages < 0 || table_width < 0 || rope_rows < 0 || rotary < 0) return IEX_ERR_BAD_ARG;
   if (!heads_ok(heads, kv_heads, head_dim) || !page_size_ok(page_size) || rotary % 2 != 0 || rotary > head_dim)
     return IEX_ERR_UNSUPPORTED;
-  if (kv_heads > 65535 || heads / kv_heads > 65535) return IEX_ERR_TOO_LARGE;  // a grid's second and third dimension
+  if (kv_heads > 65535 || heads / kv_heads > 65535 || !table_ok(table_width, page_size))  // a grid's second and third dimension
+    return IEX_ERR_TOO_LARGE;
   if (tokens == 0) return IEX_OK;
   if (!q || !k || !v || !q_out || (batch > 0 && !lengths) || (rotary > 0 && (!cos || !sin)) ||
       (batch > 0 && table_width > 0 && !block_table) || (num_pages > 0 && (!k_cache || !v_cache)) ||

@@ -765,7 +765,7 @@ extern "C" int iex_paged_attention(int rows, int heads, int kv_heads, int head_d
   if (q_row % 8 != 0 || q_head % 8 != 0 || k_page % 8 != 0 || v_page % 8 != 0 || !iex::aligned16(q) || !iex::aligned16(out) ||
       !iex::aligned16(k_cache) || !iex::aligned16(v_cache) || !iex::aligned16(workspace))
     return IEX_ERR_UNSUPPORTED;
-  if (static_cast<long long>(rows) * heads > 0x7fffffffll) return IEX_ERR_TOO_LARGE;
+  if (static_cast<long long>(rows) * heads > 0x7fffffffll || !table_ok(table_width, page_size)) return IEX_ERR_TOO_LARGE;
   const size_t need =
       iex_paged_attention_workspace_bytes(rows, heads, kv_heads, head_dim, num_pages, page_size, table_width, pages != nullptr, count);
   if (need > 0 && (!workspace || workspace_bytes < need)) return IEX_ERR_BAD_ARG;

@@ -72,6 +72,10 @@ def test_entry_points_check_their_arguments():
                    dict(out=x + 2), dict(cache=x + 4)):
         assert attention(**kwargs) == unsupported, kwargs
 
+    for width, page in ((2 ** 23, 256), (2 ** 27, 16), (2 ** 31 - 1, 256)):
+        assert attention(width=width, page=page) == too_large
+    assert attention(heads=2 ** 24, kv=1) == unsupported
+
     def select(rows=1, heads=4, kv=2, dim=64, q=x, q_row=256, boxes=x, num=3, page=16, table=x, width=2, lengths=x, count=2,
                first=1, last=1, pages=x):
         return lib.iex_paged_select(rows, heads, kv, dim, 0, q, q_row, 64, boxes, num, page, table, width, lengths, count, first,
@@ -96,3 +100,5 @@ def test_entry_points_check_their_arguments():
     for kwargs in (dict(dim=60), dict(page=24), dict(heads=3), dict(rotary=31), dict(rotary=66), dict(q_row=260), dict(boxes=x + 8),
                    dict(k=x + 4), dict(stride=2052)):
         assert append(**kwargs) == unsupported, kwargs
+    for width, page in ((2 ** 23, 256), (2 ** 27, 16), (2 ** 31 - 1, 256)):
+        assert append(width=width, page=page) == too_large
