@@ -34,6 +34,7 @@ constexpr int kAhead = 8;         // boxes that a lane has on their way
 constexpr int kMaxPages = 16384;  // 12 bytes of shared memory each
 constexpr int kBits = 10, kBins = 1 << kBits;  // of a round
 constexpr int kMostBlocks = 8;                 // of a cluster
+constexpr uint32_t kFewNear = 32;              // pages near the border that are compared with one another: a lane each
 
 struct SelectParams {
   int rows, heads, kv_heads, dim, num_pages, page_shift, table_width, count, first, last;
@@ -161,6 +162,7 @@ struct Shared {
   // of every warp of the cluster: the most that a page's terms without their signs add up to, as bits; keys
   uint32_t bound[kMostBlocks * kWarps], most[kMostBlocks * kWarps], least[kMostBlocks * kWarps];
   uint32_t warps[2][kWarps];
+  int near[kFewNear];
 };
 
 __device__ __forceinline__ int leading_zeros(uint32_t v) { return __clz(v); }
@@ -352,15 +354,56 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
   // ---- the chosen pages in order: every thread a run of them
   const int each = (pages + kThreads - 1) / kThreads, begin = threadIdx.x * each, end = min(pages, begin + each);
   {
-    // keys above `high` are taken, those from `low` on near or taken: if they are no more than are wanted, these are they
-    const auto taken = [&](int i) { return (i < from) | (i >= to) | ((keys[i] >= low) & (wanted != 0)); };
-    uint32_t mine_taken = 0;
-    for (int i = begin; i < end; ++i) mine_taken += taken(i);
-    const uint2 counts = add_in_order(mine_taken, sh.warps[0]);
-    if (counts.y == p.count) {
-      int32_t* next = chosen + counts.x;
-      for (int i = begin; i < end; ++i)
-        if (taken(i)) *next++ = i;
+    // keys above `high` are taken (1), those from `low` on near (1 << 16)
+    const auto kind = [&](int i) {
+      const uint32_t key = keys[i];
+      return (i < from) | (i >= to) | (key > high) ? 1u : (key >= low) & (wanted != 0) ? 1u << 16 : 0u;
+    };
+    uint32_t mine_of = 0;
+    for (int i = begin; i < end; ++i) mine_of += kind(i);
+    const uint2 counts = add_in_order(mine_of, sh.warps[0]);
+    const uint32_t near = counts.y >> 16, open = p.count - (counts.y & 0xffffu);  // places for the near ones
+    if (near <= open || near <= kFewNear) {
+      uint32_t taken = ~0u, before = counts.x >> 16;  // which of the near ones are taken; near ones in front of the thread's
+      if (near > open) {
+        for (int i = begin; i < end; ++i)
+          if (kind(i) > 1u) sh.near[before++] = i;
+        before = counts.x >> 16;
+        double weight[8];
+        weigh<T>(p, row, kv * group, group, d, upper, mine, weight);
+        __syncthreads();
+        for (uint32_t e0 = warp * kSides; e0 < near; e0 += kWarps * kSides) {
+          const uint32_t e = e0 + side;
+          const int where = e < near ? table[sh.near[e]] : -1;
+          uint4 box = make_uint4(0, 0, 0, 0);
+          load_once_if(box, boxes + where * box_stride, mine && real(where) ? 0 : -1);
+          float x[8];
+          unpack<T>(box, x);
+          double sum = 0.0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum = fma(static_cast<double>(x[i]), weight[i], sum);
+#pragma unroll
+          for (int off = LANES / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+          if (along == 0 && e < near) keys64[e] = real(where) ? ordered(sum) : 0;
+        }
+        __syncthreads();
+        // every warp for itself: a lane's place among them
+        const uint32_t e = lane;
+        const Key key = e < near ? keys64[e] : 0;
+        uint32_t place = 0;
+        for (uint32_t f = 0; f < near; ++f) {
+          const Key other = keys64[f];
+          place += (other > key) | ((other == key) & (f < e));
+        }
+        taken = __ballot_sync(0xffffffffu, e < near && place < open);
+      }
+      const bool all = near <= open;
+      uint32_t at = (counts.x & 0xffffu) + (all ? before : __popc(taken & static_cast<uint32_t>((1ull << min(before, 32u)) - 1)));
+      for (int i = begin; i < end; ++i) {
+        const uint32_t here = kind(i);
+        if (here == 1u || (here > 1u && (all || (taken >> before & 1u)))) chosen[at++] = i;
+        before += here >> 16;
+      }
       return;
     }
   }

@@ -470,6 +470,33 @@ def test_selection_of_equal_scores_takes_the_lower_pages():
     assert got[0, 0].tolist() == list(range(19)) + [99]
 
 
+@pytest.mark.parametrize("same", (2, 3, 31, 32, 33, 70))
+def test_selection_with_some_equal_scores_at_the_border(same):
+    """Few pages with the score at the border are compared with one another, more of them all over again; a part of them in pairs
+    that 32 bits do not tell apart."""
+    pages, page, above = 200, 16, 9
+    gen = torch.Generator().manual_seed(same)
+    q, k, v, table, held = case([pages * page] * 4, 8, 2, 128, page, F16)
+    boxes = U.boxes_of(k, table, [pages * page] * 4, page)
+    q[...] = 1.0
+    for i in range(4):
+        order = torch.randperm(pages - 2, generator=gen)[:above + same] + 1
+        own = table[i].long()
+        boxes[own] = 0.0
+        boxes[own[order[:above].to(DEV)], :, 1] = 2.0
+        boxes[own[order[above:].to(DEV)], :, 1] = 1.0
+        if i >= 2:  # every other one adds up to 2^-38 more, beside a sum of some 500
+            boxes[own[order[above::2].to(DEV)], :, 1, 5] += 2.0 ** -10
+            boxes[own[order[above::2].to(DEV)], :, 1, 6] -= 2.0 ** -10
+            boxes[own[order[above + 1::2].to(DEV)], :, 0, 7] = -(2.0 ** -24)
+            q[i, :, 7] = 0.5
+            q[i, ::4, 7] = -2.0 ** -14
+    for taken in (1, same // 2, same - 1, same):
+        count = above + taken + 2
+        got = paged.paged_select(q, boxes, table, held, page, count)
+        assert torch.equal(got.cpu(), U.select(q, boxes, table, [pages * page] * 4, page, count, 1, 1)), taken
+
+
 def test_selection_tells_scores_apart_that_are_equal_in_32_bits():
     """Two pages whose scores differ by 2^-40 of their size."""
     q, k, v, table, held = case([160], 1, 1, 64, 16, BF16)
