@@ -42,6 +42,26 @@ __device__ __forceinline__ int held(const int32_t* lengths, int row, int table_w
 __device__ __forceinline__ void cluster_begun() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait_begun() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
+// A launch in clusters of `cluster` blocks, that may begin while the kernel in front runs (launch_overlapped).
+template <typename P>
+int launch_clusters(void (*kern)(P), unsigned blocks, int cluster, int threads, size_t smem, cudaStream_t stream, const P& p) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+  return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
+}
+
 // A matrix of rows and heads whose innermost dimension is contiguous, in elements.
 struct Rows {
   const void* data;

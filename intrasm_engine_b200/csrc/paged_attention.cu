@@ -689,21 +689,7 @@ int launch(const AttentionParams& p, double chunks, cudaStream_t stream) {
     const auto kern = cluster_kernel<T, PIECES, NT>;
     constexpr int smem = kClusterWarps * W::kHeads * W::kPitch * 4;
     if (const int st = allow_shared(kern, smem)) return st;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.rows * p.kv_heads * p.parts * p.blocks);
-    cfg.blockDim = dim3(32 * kClusterWarps);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = p.blocks;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
-    return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
+    return launch_clusters<AttentionParams>(kern, p.rows * p.kv_heads * p.parts * p.blocks, p.blocks, 32 * kClusterWarps, smem, stream, p);
   }
   constexpr int kWarps = warps_of(PIECES, NT), smem = 2 * kWarps * W::kHeads * (W::kPitch * 4 + 8);
   const int blocks = static_cast<int>(std::min<double>(kNumSMs, std::max(1.0, std::ceil(chunks / (2 * kWarps)))));

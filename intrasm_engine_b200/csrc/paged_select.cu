@@ -467,21 +467,7 @@ int launch(const SelectParams& p, cudaStream_t stream) {
   const long long segments = static_cast<long long>(p.rows) * p.kv_heads;
   int parts = 1;
   while (parts < kMostBlocks && segments * parts * 2 <= 2 * kNumSMs && p.table_width >= parts * 2 * kWarps * kAhead / 2) parts *= 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(segments * parts));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = parts;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
-  return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
+  return launch_clusters<SelectParams>(kern, static_cast<unsigned>(segments * parts), parts, kThreads, smem, stream, p);
 }
 
 template <typename T>

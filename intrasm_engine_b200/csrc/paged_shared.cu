@@ -5,9 +5,9 @@
 // Here a page is read once for up to 64 of the (entry, query head) pairs that list it: index_kernel sorts the entries of the lists
 // by page, page_kernel forms the softmax and the product of such a tile with its page, join_entries_kernel adds up each row's
 // entries in the order of its list.  What is written and read between them, a product of fp32 for every entry and query head, is
-// 2 G / page of the keys and values that would be read (G query heads to a key head).  86 us at the same sizes: 13 us of sorting
-// (one block for each key head, latency), 64 us of page_kernel (378 MB through L2, 5.9 TB/s), 20 us of joining (108 MB), with
-// their launches overlapped; 96 us instead of 420 where each of 32 key heads has its own query head.
+// 2 G / page of the keys and values that would be read (G query heads to a key head).  85 us at the same sizes: 11 us of sorting
+// (latency), 63 us of page_kernel (378 MB through L2, 6 TB/s), 18 us of joining (108 MB, 6 TB/s), with their launches overlapped; 96
+// us instead of 420 where each of 32 key heads has its own query head.
 //
 // page_kernel: keys and values of 64 positions and the queries in shared memory (rows of 16 bytes more than they have, so that
 // eight of them lie in different banks), a warp has 16 of the pairs: S = Q K^T by m16n8k16, whose accumulators are the fragments
@@ -17,6 +17,8 @@
 // reach the others (0 x Inf): rows whose product comes out not finite are summed again, position by position.
 #include <algorithm>
 
+#include <cooperative_groups.h>
+
 #include "paged_mma.cuh"
 #include "paged_shared.cuh"
 
@@ -24,9 +26,12 @@ namespace iex {
 namespace paged {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kIndexThreads = 1024;
 constexpr int kTileRows = 64, kThreads = 128, kPositions = 64;
-constexpr int kMostPages = 16384;  // counters of 8 bytes in shared memory
+constexpr int kMostPages = 16384;  // 12 bytes of shared memory each
+constexpr int kIndexBlocks = 8;    // of a cluster, at most
 constexpr int kMostGroup = 16;
 
 struct Item {
@@ -44,59 +49,83 @@ struct Params {
   float* product;  // [kv_heads][entries][group][dim]
 };
 
-// The page of an entry, or -1, and the positions of it that the row sees.
-__device__ __forceinline__ int2 look_at(const SharedCall& c, int kv, int row, int i) {
-  const int page = 1 << c.page_shift;
-  const int nth = c.pages[(static_cast<long long>(row) * c.kv_heads + kv) * c.count + i];  // an entry that counts, or not
-  const int length = held(c.lengths, row, c.table_width, c.page_shift), held_pages = (length + page - 1) >> c.page_shift;
-  if (i >= held_pages || nth < 0 || nth >= held_pages) return make_int2(-1, 0);
-  const int at = c.table[static_cast<long long>(row) * c.table_width + nth];
-  return make_int2(at >= 0 && at < c.num_pages ? at : -1, min(page, length - (nth << c.page_shift)));
-}
-
-// A block for each key head: counts the entries of every page, and writes them page by page.  In which order a page's entries come
-// makes no difference: an entry's sums depend on nothing else of its tile.
+// A cluster for each key head: counts the entries of every page, and writes them page by page.  In which order a page's entries come
+// makes no difference: an entry's sums depend on nothing else of its tile.  Lookups and writes go everywhere, 32 places a warp: one
+// block alone takes 9 us for 4096 entries, eight take 6; 26 and 10 for 16384.
 __global__ void __launch_bounds__(kIndexThreads) index_kernel(const __grid_constant__ Params p) {
-  extern __shared__ int counters[];  // of the pages: entries; then the most positions that one sees
+  extern __shared__ int counters[];  // of the pages: entries of this block; the most positions that one sees; where the next one goes
   __shared__ unsigned long long warps[32];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
   grid_dependency_wait();
   grid_launch_dependents();
   const SharedCall& c = p.c;
-  int* const most = counters + c.num_pages;
-  const int kv = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = c.heads / c.kv_heads;
+  int *const most = counters + c.num_pages, *const next = most + c.num_pages;
+  const int kv = blockIdx.x / blocks, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = c.heads / c.kv_heads;
   int2* const seen = p.seen + static_cast<long long>(kv) * p.entries;
   for (int i = threadIdx.x; i < 2 * c.num_pages; i += kIndexThreads) counters[i] = 0;
   __syncthreads();
+  const int each_block = (p.entries + blocks - 1) / blocks, first = rank * each_block + threadIdx.x;
+  const int last = min(p.entries, (rank + 1) * each_block);
+  // kAhead entries of a thread at once, in steps without branches, as they take three loads after one another
   constexpr int kAhead = 4;
-  for (int e0 = threadIdx.x; e0 < p.entries; e0 += kAhead * kIndexThreads) {
-    int2 some[kAhead];
+  const int page = 1 << c.page_shift;
+  for (int e0 = first; e0 < last; e0 += kAhead * kIndexThreads) {
+    int row[kAhead], nth[kAhead], length[kAhead], at[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const int e = min(e0 + u * kIndexThreads, p.entries - 1), row = e / c.count;
-      some[u] = look_at(c, kv, row, e - row * c.count);
+      const int e = min(e0 + u * kIndexThreads, last - 1);
+      row[u] = e / c.count;
+      const int i = e - row[u] * c.count;
+      length[u] = held(c.lengths, row[u], c.table_width, c.page_shift);
+      nth[u] = c.pages[(static_cast<long long>(row[u]) * c.kv_heads + kv) * c.count + i];
+      if (i >= (length[u] + page - 1) >> c.page_shift) length[u] = 0;  // an entry that does not count
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      at[u] = c.table[static_cast<long long>(row[u]) * c.table_width + min(max(nth[u], 0), c.table_width - 1)];
+      const bool there = nth[u] >= 0 && nth[u] < (length[u] + page - 1) >> c.page_shift;
+      length[u] = there ? min(page, length[u] - (nth[u] << c.page_shift)) : 0;
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int e = e0 + u * kIndexThreads;
-      if (e >= p.entries) break;
-      seen[e] = some[u];
-      if (some[u].x >= 0) {
-        atomicAdd(&counters[some[u].x], 1);
-        atomicMax(&most[some[u].x], some[u].y);
+      if (e >= last) break;
+      const bool there = length[u] > 0 && at[u] >= 0 && at[u] < c.num_pages;
+      seen[e] = make_int2(there ? at[u] : -1, length[u]);
+      if (there) {
+        atomicAdd(&counters[at[u]], 1);
+        atomicMax(&most[at[u]], length[u]);
       } else {
         float2* const stats = p.stats + (static_cast<long long>(kv) * p.entries + e) * group;
         for (int g = 0; g < group; ++g) stats[g] = make_float2(-INFINITY, 0.f);
       }
     }
   }
-  __syncthreads();
+  cluster.sync();
   // entries (lower half) and items (upper half) of the pages in front; a thread has a run of pages
   const int each = (c.num_pages + kIndexThreads - 1) / kIndexThreads;
   const int from = min(c.num_pages, static_cast<int>(threadIdx.x) * each), to = min(c.num_pages, from + each);
   const auto items_for = [&](int n) { return (n + p.tile_entries - 1) / p.tile_entries; };
+  struct Page {
+    int all, in_front, most;  // entries of all blocks, of those in front of this one
+  };
+  const auto count = [&](int i) {
+    Page found{0, 0, 0};
+    for (int b = 0; b < blocks; ++b) {
+      const int* const theirs = cluster.map_shared_rank(counters, b);
+      const int n = theirs[i];
+      found.all += n;
+      found.in_front += b < rank ? n : 0;
+      found.most = max(found.most, theirs[c.num_pages + i]);
+    }
+    return found;
+  };
   unsigned long long mine = 0;
-  for (int i = from; i < to; ++i)
-    mine += static_cast<unsigned long long>(items_for(counters[i])) << 32 | static_cast<unsigned>(counters[i]);
+  for (int i = from; i < to; ++i) {
+    const int n = count(i).all;
+    mine += static_cast<unsigned long long>(items_for(n)) << 32 | static_cast<unsigned>(n);
+  }
   unsigned long long sum = mine;
   for (int d = 1; d < 32; d <<= 1) {
     const unsigned long long other = __shfl_up_sync(0xffffffffu, sum, d);
@@ -110,20 +139,31 @@ __global__ void __launch_bounds__(kIndexThreads) index_kernel(const __grid_const
   int list_at = static_cast<int>(front & 0xffffffffu), item_at = static_cast<int>(front >> 32);
   Item* const items = p.items + static_cast<long long>(kv) * p.most_items;
   for (int i = from; i < to; ++i) {
-    const int n = counters[i];
-    for (int begin = 0; begin < n; begin += p.tile_entries)
-      items[item_at++] = {i, list_at + begin, min(p.tile_entries, n - begin), most[i]};
-    counters[i] = list_at;  // where the page's next entry goes
-    list_at += n;
+    const Page here = count(i);
+    if (rank == 0)
+      for (int begin = 0; begin < here.all; begin += p.tile_entries)
+        items[item_at++] = {i, list_at + begin, min(p.tile_entries, here.all - begin), here.most};
+    next[i] = list_at + here.in_front;
+    list_at += here.all;
   }
-  if (threadIdx.x == kIndexThreads - 1) p.items_of[kv] = item_at;
+  if (rank == 0 && threadIdx.x == kIndexThreads - 1) p.items_of[kv] = item_at;
   __syncthreads();
   int2* const list = p.list + static_cast<long long>(kv) * p.entries;
-#pragma unroll 4
-  for (int e = threadIdx.x; e < p.entries; e += kIndexThreads) {
-    const int2 here = seen[e];
-    if (here.x >= 0) list[atomicAdd(&counters[here.x], 1)] = make_int2(e, here.y);
+  for (int e0 = first; e0 < last; e0 += kAhead * kIndexThreads) {
+    int2 here[kAhead];
+    int to[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int e = e0 + u * kIndexThreads;
+      here[u] = e < last ? seen[e] : make_int2(-1, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) to[u] = here[u].x >= 0 ? atomicAdd(&next[here[u].x], 1) : -1;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (to[u] >= 0) list[to[u]] = make_int2(e0 + u * kIndexThreads, here[u].y);
   }
+  cluster.sync();  // others may read this block's counters until then
 }
 
 __device__ __forceinline__ uint32_t smem(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -379,7 +419,7 @@ template <typename T, int PIECES>
 int launch(const Params& p, cudaStream_t stream) {
   const SharedCall& c = p.c;
   constexpr int bytes = (kTileRows + 2 * kPositions) * (64 * PIECES + 8) * 2;
-  const int counters = 2 * c.num_pages * static_cast<int>(sizeof(int));
+  const int counters = 3 * c.num_pages * static_cast<int>(sizeof(int));
   if (counters > 40 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(index_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, counters);
     if (e != cudaSuccess) return static_cast<int>(e);
@@ -388,7 +428,10 @@ int launch(const Params& p, cudaStream_t stream) {
     const cudaError_t e = cudaFuncSetAttribute(page_kernel<T, PIECES>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return static_cast<int>(e);
   }
-  if (const int st = launch_overlapped(index_kernel, dim3(c.kv_heads), dim3(kIndexThreads), counters, stream, p)) return st;
+  // Together no more than half the SMs: 16 key heads with 8 blocks each take 7 us longer than with 4 (clusters wait for places).
+  int blocks = 1;
+  while (blocks < kIndexBlocks && p.entries > blocks * kIndexThreads / 2 && c.kv_heads * blocks * 4 <= kNumSMs) blocks *= 2;
+  if (const int st = launch_clusters<Params>(index_kernel, c.kv_heads * blocks, blocks, kIndexThreads, counters, stream, p)) return st;
   if (const int st = launch_overlapped(page_kernel<T, PIECES>, dim3(p.most_items, c.kv_heads), dim3(kThreads), bytes, stream, p)) return st;
   return launch_overlapped(join_entries_kernel<T>, dim3(c.rows * c.kv_heads), dim3(kThreads), 0, stream, p);
 }
@@ -401,19 +444,22 @@ size_t shared_workspace_bytes(int rows, int heads, int kv_heads, int head_dim, i
   if (group > kMostGroup || num_pages <= 0 || num_pages > kMostPages || count <= 0 || count > table_width || kv_heads > 65535) return 0;
   const double entries = static_cast<double>(rows) * count;
   if (entries > 1 << 18) return 0;  // one block sorts a head's
-  // us of the two ways; within a quarter of 30 measurements (rows 32 .. 4096, 1 .. 16 query heads to a key head, pages of 16 .. 256).
-  // Row by row: keys and values from L2.  Here: the sort, a product to and fro for every entry and query head, and a block's work.
+  // us of the two ways; of 30 measurements (rows 32 .. 4096, 1 .. 16 query heads to a key head, pages of 16 .. 256) all but three
+  // within a quarter.  Row by row: keys and values from L2.  Here: the sort, a product to and fro for every entry and query head,
+  // and a block's work.
   //   rows, key heads x G, dim, page, pages, listed    row by row   here
-  //   256,   8 x 4, 128,  64,  256, 16                    118        86
+  //   256,   8 x 4, 128,  64,  256, 16                    118        85
   //   256,  32 x 1, 128,  64,   64, 16                    420        96
-  //   512,  16 x 2,  64, 128,  128, 16                    470       125
+  //   512,  16 x 2,  64, 128,  128, 16                    470       120
+  //   4096,  2 x 2, 128,  64,  512, 32                    836       292
+  //   64,    8 x 4, 128,  64,  256, 16                     38        45
   //   1024,  2 x 8, 128,  64,  256, 16                    119       156
   //   256,   8 x 4, 128,  64, 4096, 16                    160       311
   const int dim = head_dim > 64 ? 128 : 64, tiles = (page_size + kPositions - 1) / kPositions;
   const double pairs = entries * heads, blocks = kv_heads * (entries / (kTileRows / group) + 0.5 * std::min<double>(num_pages, entries));
-  const double one_by_one = 12.0 + entries * kv_heads * 4 * page_size * dim * (group > 8 ? 1.25 : 1.0) / 9.0e6;
-  const double shared = 14.0 + 1.3e-3 * entries + pairs * (8.3e-6 + 1.5e-6 * head_dim) + blocks * (4.6e-3 + 8.4e-5 * tiles * dim);
-  if (one_by_one < 1.1 * shared) return 0;
+  const double one_by_one = 12.0 + entries * kv_heads * 4 * page_size * dim * (group > 8 ? 1.25 : 1.0) / 9.7e6;
+  const double shared = 15.0 + 6e-4 * entries + 1e-6 * pairs * head_dim + blocks * (6e-3 + 8.8e-5 * tiles * dim);
+  if (one_by_one < 1.05 * shared) return 0;
   const Sizes s = sizes(rows, heads, kv_heads, head_dim, num_pages, count);
   return s.all <= 512u << 20 ? s.all : 0;
 }
