@@ -66,14 +66,11 @@ __device__ __forceinline__ void unpack(const uint4& v, float (&to)[8]) {
   for (int i = 0; i < 8; ++i) to[i] = as_float(e[i]);
 }
 
-// The larger of each of two elements without their signs.
-__device__ __forceinline__ uint32_t larger_size(uint32_t a, uint32_t b, __half) {
-  const __half2 v = __hmax2(reinterpret_cast<const __half2&>(a), __habs2(reinterpret_cast<const __half2&>(b)));
-  return reinterpret_cast<const uint32_t&>(v);
-}
-__device__ __forceinline__ uint32_t larger_size(uint32_t a, uint32_t b, __nv_bfloat16) {
-  const __nv_bfloat162 v = __hmax2(reinterpret_cast<const __nv_bfloat162&>(a), __habs2(reinterpret_cast<const __nv_bfloat162&>(b)));
-  return reinterpret_cast<const uint32_t&>(v);
+// The largest of three without their signs; not NaN where one is a number.
+__device__ __forceinline__ float largest_size(float a, float b, float c) {
+  float v;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+  return v;
 }
 
 // The sums of v over all threads in front of this one and over all.  `warps` has not been read since the last barrier.
@@ -220,9 +217,10 @@ __device__ __forceinline__ Border<K> find_border(const K* keys, int from, int to
   return {least, most, need};
 }
 
-// LANES: side by side on a box, 8 elements each.
-template <typename T, int LANES>
-__global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant__ SelectParams p) {
+// LANES: side by side on a box, 8 elements each.  BLOCKS of an SM at once: 2 where there are no more (all of a lane's boxes then find
+// registers: 9.9 us for 16 rows x 8 key heads x 512 pages, with 3 11.1), else 3 (256 rows x 8 key heads x 256 pages: 43.9 us, with 2 51.7).
+template <typename T, int LANES, int BLOCKS>
+__global__ void __launch_bounds__(kThreads, BLOCKS) select_kernel(const __grid_constant__ SelectParams p) {
   extern __shared__ Key keys64[];  // of all pages, of which the scores in 64 bits are needed; the first block's are used
   uint32_t* const keys = reinterpret_cast<uint32_t*>(keys64 + p.table_width);  // of all pages, in 32 bits
   __shared__ Shared sh;
@@ -250,58 +248,73 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
       for (int i = threadIdx.x; i < p.count; i += kThreads) chosen[i] = i < pages ? i : -1;
     return;
   }
+  if (p.num_pages == 0) {  // all are alike
+    if (part == 0)
+      for (int i = threadIdx.x; i < p.count; i += kThreads) chosen[i] = i < p.count - p.last ? i : pages - p.count + i;
+    return;
+  }
   if (parts > 1) cluster_begun();
   const int to = pages - p.last;  // [from, to): those that are chosen by their scores
 
   // ---- scores
   const T* const boxes = static_cast<const T*>(p.boxes) + static_cast<long long>(kv) * 2 * p.dim + d0;
-  const long long box_stride = static_cast<long long>(p.kv_heads) * 2 * p.dim;
-  const auto look_up = [&](int base) { return base + lane < to && lane < kBatch ? table[base + lane] : -1; };
-  const auto real = [&](int where) { return where >= 0 && where < p.num_pages; };
+  const uint32_t box_stride = static_cast<uint32_t>(p.kv_heads) * 2 * p.dim;  // kv_heads is below 2^24
+  const auto box_of = [&](int where) { return boxes + static_cast<unsigned long long>(static_cast<uint32_t>(where)) * box_stride; };
+  const auto real = [&](int where) { return where < p.num_pages ? where : -1; };  // negative where it is not one of the cache's
+  const auto look_up = [&](int base) { return real(base + lane < to && lane < kBatch ? table[base + lane] : -1); };
   const auto request = [&](int at, uint4 (&box)[kAhead]) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int where = __shfl_sync(0xffffffffu, at, u * kSides + side);
       box[u] = make_uint4(0, 0, 0, 0);
-      load_once_if(box[u], boxes + where * box_stride, mine && real(where) ? 0 : -1);
+      load_once_if(box[u], box_of(where), mine ? where : -1);
     }
   };
   const bool holder = along % (LANES / kAhead) == 0;  // one lane for each box that is added up
   {
     const int step = parts * kWarps * kBatch;
     int base = base0;
-    int at = base + lane < to ? at0 : -1;
-    uint4 largest = make_uint4(0, 0, 0, 0);  // of the lane's elements of all boxes, without their signs
+    int at = real(base + lane < to ? at0 : -1);
+    float largest[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // of the lane's elements of all boxes, without their signs
     bool finite = true;
     uint32_t key_most = 0, key_least = ~0u;
     uint32_t* const shared_keys = parts > 1 ? cluster.map_shared_rank(keys, 0) : keys;
     bool waited = parts == 1;
+    // Loads without conditions (their registers need not be set first): lanes without a piece read the first one, which weighs nothing,
+    // and pages that are not the cache's are read as its first one and then not counted.  An infinite value in there makes a score that
+    // is not finite, and costs no more than that the pages are scored again.
+    const T* const own = boxes - (mine ? 0 : d0);
     for (; base < to; base += step) {
       uint4 box[kAhead];
-      request(at, box);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int where = max(__shfl_sync(0xffffffffu, at, u * kSides + side), 0);
+        box[u] = load_once(own + static_cast<unsigned long long>(static_cast<uint32_t>(where)) * box_stride);
+      }
       const int here = at;
       at = look_up(base + step);
       float sum[kAhead];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        float x[8];
-        unpack<T>(box[u], x);
-        float2 two = make_float2(0.f, 0.f);
+      for (int u = 0; u < kAhead; u += 2) {
+        float x[2][8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          two = ffma2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(weight[2 * i], weight[2 * i + 1]), two);
-        sum[u] = two.x + two.y;
-        largest.x = larger_size(largest.x, box[u].x, T());
-        largest.y = larger_size(largest.y, box[u].y, T());
-        largest.z = larger_size(largest.z, box[u].z, T());
-        largest.w = larger_size(largest.w, box[u].w, T());
+        for (int j = 0; j < 2; ++j) {
+          unpack<T>(box[u + j], x[j]);
+          float2 two = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            two = ffma2(make_float2(x[j][2 * i], x[j][2 * i + 1]), make_float2(weight[2 * i], weight[2 * i + 1]), two);
+          sum[u + j] = two.x + two.y;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) largest[i] = largest_size(largest[i], x[0][i], x[1][i]);
       }
       const int nth = add_up<LANES>(sum) * kSides + side, where = __shfl_sync(0xffffffffu, here, nth);
       if (!waited) {
         cluster_wait_begun();
         waited = true;
       }
-      const uint32_t key = real(where) ? ordered(sum[0]) : 0;
+      const uint32_t key = where >= 0 ? ordered(sum[0]) : 0;
       const bool there = holder & (base + nth < to);
       if (there) shared_keys[base + nth] = key;
       key_most = max(key_most, there ? key : 0u);
@@ -310,10 +323,9 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
     }
     if (!waited) cluster_wait_begun();
     // A sum of the largest elements' terms is no less than that of any page's.
-    float x[8], most = 0.f;
-    unpack<T>(largest, x);
+    float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) most = fmaf(x[i], fabsf(weight[i]), most);
+    for (int i = 0; i < 8; ++i) most = fmaf(largest[i], fabsf(weight[i]), most);
     if (!finite) most = INFINITY;
     for (int off = LANES / 2; off > 0; off >>= 1) most += __shfl_xor_sync(0xffffffffu, most, off);
     const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(most));  // NaN is above infinity
@@ -374,9 +386,9 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
         __syncthreads();
         for (uint32_t e0 = warp * kSides; e0 < near; e0 += kWarps * kSides) {
           const uint32_t e = e0 + side;
-          const int where = e < near ? table[sh.near[e]] : -1;
+          const int where = real(e < near ? table[sh.near[e]] : -1);
           uint4 box = make_uint4(0, 0, 0, 0);
-          load_once_if(box, boxes + where * box_stride, mine && real(where) ? 0 : -1);
+          load_once_if(box, box_of(where), mine ? where : -1);
           float x[8];
           unpack<T>(box, x);
           double sum = 0.0;
@@ -384,7 +396,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
           for (int i = 0; i < 8; ++i) sum = fma(static_cast<double>(x[i]), weight[i], sum);
 #pragma unroll
           for (int off = LANES / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-          if (along == 0 && e < near) keys64[e] = real(where) ? ordered(sum) : 0;
+          if (along == 0 && e < near) keys64[e] = where >= 0 ? ordered(sum) : 0;
         }
         __syncthreads();
         // every warp for itself: a lane's place among them
@@ -429,7 +441,7 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
         }
         const int nth = add_up<LANES>(sum) * kSides + side, where = __shfl_sync(0xffffffffu, at, nth);
         const bool near_there = __shfl_sync(0xffffffffu, near, nth);
-        if (holder && base + nth < to && near_there) keys64[base + nth] = real(where) ? ordered(sum[0]) : 0;
+        if (holder && base + nth < to && near_there) keys64[base + nth] = where >= 0 ? ordered(sum[0]) : 0;
       }
       if (inside && !near) keys64[base + lane] = old > high ? ~0ull : 0;
     }
@@ -455,19 +467,24 @@ __global__ void __launch_bounds__(kThreads) select_kernel(const __grid_constant_
   }
 }
 
-template <typename T, int LANES>
-int launch(const SelectParams& p, cudaStream_t stream) {
-  const auto kern = select_kernel<T, LANES>;
+template <typename T, int LANES, int BLOCKS>
+int launch(const SelectParams& p, int parts, cudaStream_t stream) {
+  const auto kern = select_kernel<T, LANES, BLOCKS>;
   const size_t smem = static_cast<size_t>(std::max(p.table_width, 1)) * (sizeof(Key) + sizeof(uint32_t));
   if (smem > 40 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return static_cast<int>(e);
   }
+  return launch_clusters<SelectParams>(kern, static_cast<unsigned>(p.rows) * p.kv_heads * parts, parts, kThreads, smem, stream, p);
+}
+
+template <typename T, int LANES>
+int launch(const SelectParams& p, cudaStream_t stream) {
   // two blocks an SM, but a warp's turn of pages for every warp
   const long long segments = static_cast<long long>(p.rows) * p.kv_heads;
   int parts = 1;
   while (parts < kMostBlocks && segments * parts * 2 <= 2 * kNumSMs && p.table_width >= parts * 2 * kWarps * kAhead / 2) parts *= 2;
-  return launch_clusters<SelectParams>(kern, static_cast<unsigned>(segments * parts), parts, kThreads, smem, stream, p);
+  return segments * parts <= 2 * kNumSMs ? launch<T, LANES, 2>(p, parts, stream) : launch<T, LANES, 3>(p, parts, stream);
 }
 
 template <typename T>

@@ -497,6 +497,23 @@ def test_selection_with_some_equal_scores_at_the_border(same):
         assert torch.equal(got.cpu(), U.select(q, boxes, table, [pages * page] * 4, page, count, 1, 1)), taken
 
 
+def test_selection_where_pages_are_not_the_caches():
+    lengths = [900, 30, 0, 1600, 1500]
+    q, k, v, table, held = case(lengths, 4, 2, 40, 16, F16)
+    boxes = U.boxes_of(k, table, lengths, 16)
+    table[0, 3:20], table[0, 20:23], table[3, 1::2] = -1, 2 ** 31 - 1, k.size(0)
+    table[4] = -2 ** 31
+    for first in (0.0, float("inf"), float("nan"), 65504.0):  # what the cache's first page has is nothing to them
+        boxes[0] = first
+        table[table == 0] = 1
+        for count in (2, 7, 60, 95):
+            got = paged.paged_select(q, boxes, table, held, 16, count)
+            assert torch.equal(got.cpu(), U.select(q, boxes, table, lengths, 16, count, 1, 1)), (first, count)
+    for count, first, last in ((2, 1, 1), (9, 0, 3), (20, 4, 0), (95, 1, 1)):
+        got = paged.paged_select(q, boxes[:0], table, held, 16, count, first, last)
+        assert torch.equal(got.cpu(), U.select(q, boxes[:0], table, lengths, 16, count, first, last)), count
+
+
 def test_selection_tells_scores_apart_that_are_equal_in_32_bits():
     """Two pages whose scores differ by 2^-40 of their size."""
     q, k, v, table, held = case([160], 1, 1, 64, 16, BF16)
