@@ -13,9 +13,13 @@
 // scores in 32 bits do not tell are they scored again (any score that is not finite has all of them scored again).
 //
 // A cluster of blocks per row and key head: each scores a part of the pages (lanes side by side on a box, eight boxes in flight
-// a lane) and stores the scores, as whole numbers of the same order, in the first block's shared memory, which selects: 8 bits at
+// a lane) and stores the scores, as whole numbers of the same order, in the first block's shared memory, which selects: 10 bits at
 // a time from the first one in which the largest and the smallest differ, until a digit's pages are all taken (two rounds as
-// a rule).  So many blocks that they fill the GPU, or one each where rows and key heads do.
+// a rule).  Up to 32 pages near the border are then compared with one another in 64 bits, more of them searched like all were.  So
+// many blocks that they fill the GPU, or one each where rows and key heads do.
+//
+// 1 row of 512 pages, 8 key heads of 128: 5.4 us, latency (lengths and queries, boxes, the cluster's barrier, the search); 16 rows:
+// 9.9 us (19 MB of boxes); 256 rows of 256 pages: 37 us, issue slots (70 %; 70 instructions a box and warp, half of them the search's) and 268 MB from L2.
 #include <algorithm>
 
 #include <cooperative_groups.h>
@@ -28,12 +32,12 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+constexpr int kMostWarps = 8;     // of a block
 constexpr int kAhead = 8;         // boxes that a lane has on their way
 constexpr int kMaxPages = 16384;  // 12 bytes of shared memory each
 constexpr int kBits = 10, kBins = 1 << kBits;  // of a round
 constexpr int kMostBlocks = 8;                 // of a cluster
+constexpr size_t kSmallSmem = 22 * 1024;       // of which an SM has room for 6, beside what is fixed
 constexpr uint32_t kFewNear = 32;              // pages near the border that are compared with one another: a lane each
 
 struct SelectParams {
@@ -74,6 +78,7 @@ __device__ __forceinline__ float largest_size(float a, float b, float c) {
 }
 
 // The sums of v over all threads in front of this one and over all.  `warps` has not been read since the last barrier.
+template <int THREADS>
 __device__ __forceinline__ uint2 add_in_order(uint32_t v, uint32_t* warps) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t sum = v;
@@ -83,7 +88,7 @@ __device__ __forceinline__ uint2 add_in_order(uint32_t v, uint32_t* warps) {
   }
   if (lane == 31) warps[warp] = sum;
   __syncthreads();
-  const uint32_t of_warp = lane < kWarps ? warps[lane] : 0;
+  const uint32_t of_warp = lane < THREADS / 32 ? warps[lane] : 0;
   return make_uint2(sum - v + __reduce_add_sync(0xffffffffu, lane < warp ? of_warp : 0), __reduce_add_sync(0xffffffffu, of_warp));
 }
 
@@ -157,17 +162,18 @@ struct Border {
 struct Shared {
   uint32_t bins[3][kBins], groups[3][32];  // keys in a bin, in 32 bins
   // of every warp of the cluster: the most that a page's terms without their signs add up to, as bits; keys
-  uint32_t bound[kMostBlocks * kWarps], most[kMostBlocks * kWarps], least[kMostBlocks * kWarps];
-  uint32_t warps[2][kWarps];
+  uint32_t bound[kMostBlocks * kMostWarps], most[kMostBlocks * kMostWarps], least[kMostBlocks * kMostWarps];
+  uint32_t warps[2][kMostWarps];
   int near[kFewNear];
 };
 
 __device__ __forceinline__ int leading_zeros(uint32_t v) { return __clz(v); }
 __device__ __forceinline__ int leading_zeros(Key v) { return __clzll(v); }
 
+template <int THREADS>
 __device__ __forceinline__ void clear_bins(Shared& sh, int which) {
 #pragma unroll
-  for (int i = 0; i < kBins; i += kThreads) sh.bins[which][i + threadIdx.x] = 0;
+  for (int i = 0; i < kBins; i += THREADS) sh.bins[which][i + threadIdx.x] = 0;
   if (threadIdx.x < 32) sh.groups[which][threadIdx.x] = 0;
 }
 
@@ -188,7 +194,7 @@ __device__ __forceinline__ int find_lane(uint32_t mine, uint32_t& need, uint32_t
 
 // The border of the `need` largest of keys [from, to), which are more than that and lie from `least` to `most`; called by all
 // threads of the block, with the first bins cleared.
-template <typename K>
+template <int THREADS, typename K>
 __device__ __forceinline__ Border<K> find_border(const K* keys, int from, int to, K least, K most, uint32_t need, Shared& sh) {
   const int lane = threadIdx.x & 31;
   if (need == 0) return {static_cast<K>(~K(0)), static_cast<K>(~K(0)), 0};
@@ -197,8 +203,8 @@ __device__ __forceinline__ Border<K> find_border(const K* keys, int from, int to
     const int shift = max(0, static_cast<int>(8 * sizeof(K)) - kBits - leading_zeros(span));  // span >> shift is below kBins
     uint32_t* const bins = sh.bins[round % 3];
     uint32_t* const groups = sh.groups[round % 3];
-    clear_bins(sh, (round + 1) % 3);  // last read two rounds ago
-    for (int i = from + threadIdx.x; i < to; i += kThreads) {
+    clear_bins<THREADS>(sh, (round + 1) % 3);  // last read two rounds ago
+    for (int i = from + threadIdx.x; i < to; i += THREADS) {
       const K place = keys[i] - least;
       if (place <= span) {
         atomicAdd(&bins[place >> shift], 1u);
@@ -217,10 +223,13 @@ __device__ __forceinline__ Border<K> find_border(const K* keys, int from, int to
   return {least, most, need};
 }
 
-// LANES: side by side on a box, 8 elements each.  BLOCKS of an SM at once: 2 where there are no more (all of a lane's boxes then find
-// registers: 9.9 us for 16 rows x 8 key heads x 512 pages, with 3 11.1), else 3 (256 rows x 8 key heads x 256 pages: 43.9 us, with 2 51.7).
-template <typename T, int LANES, int BLOCKS>
-__global__ void __launch_bounds__(kThreads, BLOCKS) select_kernel(const __grid_constant__ SelectParams p) {
+// LANES: side by side on a box, 8 elements each.  THREADS, BLOCKS of an SM at once: 256, 2 where there are no more blocks (all of a
+// lane's boxes then find registers: 9.9 us for 16 rows x 8 key heads x 512 pages, with a third block 11.1); else 128, 6 (what every warp does
+// for itself counts there: 256 rows x 8 key heads x 256 pages 37 us, with 256, 3 44), or 256, 3 where the scores' shared memory leaves no
+// room for 6 (the same with 4096 pages: 453 us, with 128 threads 562, with 256, 2 498).
+template <typename T, int LANES, int THREADS, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS) select_kernel(const __grid_constant__ SelectParams p) {
+  constexpr int kThreads = THREADS, kWarps = THREADS / 32;
   extern __shared__ Key keys64[];  // of all pages, of which the scores in 64 bits are needed; the first block's are used
   uint32_t* const keys = reinterpret_cast<uint32_t*>(keys64 + p.table_width);  // of all pages, in 32 bits
   __shared__ Shared sh;
@@ -337,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) select_kernel(const __grid_c
       first.most[part * kWarps + warp] = key_most;
       first.least[part * kWarps + warp] = key_least;
     }
-    if (part == 0) clear_bins(sh, 0);
+    if (part == 0) clear_bins<THREADS>(sh, 0);
   }
   if (parts > 1) cluster.sync(); else __syncthreads();
   if (part != 0) return;
@@ -353,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) select_kernel(const __grid_c
   key_most = __reduce_max_sync(0xffffffffu, key_most);
   key_least = __reduce_min_sync(0xffffffffu, key_least);
   const float bound = __uint_as_float(__reduce_max_sync(0xffffffffu, bound_bits));
-  const Border<uint32_t> border = find_border(keys, from, to, key_least, key_most, wanted, sh);
+  const Border<uint32_t> border = find_border<THREADS>(keys, from, to, key_least, key_most, wanted, sh);
   // Off by at most: a rounding for each of a lane's 4 products and sums, one for their sum, 5 over lanes and one for every query head,
   // relative to the terms without their signs; and products below the smallest numbers.  The border is off by no more than a page's score.
   const float twice = __fmaf_ru(bound, (group + 16.f) * 0x1p-23f, 1e-40f);
@@ -373,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) select_kernel(const __grid_c
     };
     uint32_t mine_of = 0;
     for (int i = begin; i < end; ++i) mine_of += kind(i);
-    const uint2 counts = add_in_order(mine_of, sh.warps[0]);
+    const uint2 counts = add_in_order<THREADS>(mine_of, sh.warps[0]);
     const uint32_t near = counts.y >> 16, open = p.count - (counts.y & 0xffffu);  // places for the near ones
     if (near <= open || near <= kFewNear) {
       uint32_t taken = ~0u, before = counts.x >> 16;  // which of the near ones are taken; near ones in front of the thread's
@@ -446,9 +455,9 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) select_kernel(const __grid_c
       if (inside && !near) keys64[base + lane] = old > high ? ~0ull : 0;
     }
   }
-  clear_bins(sh, 0);
+  clear_bins<THREADS>(sh, 0);
   __syncthreads();
-  const Border<Key> exact = find_border(keys64, from, to, Key(0), ~Key(0), wanted, sh);
+  const Border<Key> exact = find_border<THREADS>(keys64, from, to, Key(0), ~Key(0), wanted, sh);
   // above in the lower half, equal in the upper one; keys outside [from, to) are whatever they are
   const auto kind = [&](int i) {
     const Key key = keys64[i];
@@ -457,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) select_kernel(const __grid_c
   };
   uint32_t counts = 0;
   for (int i = begin; i < end; ++i) counts += kind(i);
-  const uint32_t front = add_in_order(counts, sh.warps[1]).x;
+  const uint32_t front = add_in_order<THREADS>(counts, sh.warps[1]).x;
   uint32_t higher = front & 0xffffu, same = front >> 16;
   for (int i = begin; i < end; ++i) {
     const uint32_t here = kind(i), is_above = here & 1u, is_equal = here >> 16;
@@ -467,15 +476,14 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) select_kernel(const __grid_c
   }
 }
 
-template <typename T, int LANES, int BLOCKS>
-int launch(const SelectParams& p, int parts, cudaStream_t stream) {
-  const auto kern = select_kernel<T, LANES, BLOCKS>;
-  const size_t smem = static_cast<size_t>(std::max(p.table_width, 1)) * (sizeof(Key) + sizeof(uint32_t));
-  if (smem > 40 * 1024) {
+template <typename T, int LANES, int THREADS, int BLOCKS>
+int launch(const SelectParams& p, int parts, size_t smem, cudaStream_t stream) {
+  const auto kern = select_kernel<T, LANES, THREADS, BLOCKS>;
+  if (smem > 32 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return static_cast<int>(e);
   }
-  return launch_clusters<SelectParams>(kern, static_cast<unsigned>(p.rows) * p.kv_heads * parts, parts, kThreads, smem, stream, p);
+  return launch_clusters<SelectParams>(kern, static_cast<unsigned>(p.rows) * p.kv_heads * parts, parts, THREADS, smem, stream, p);
 }
 
 template <typename T, int LANES>
@@ -483,8 +491,10 @@ int launch(const SelectParams& p, cudaStream_t stream) {
   // two blocks an SM, but a warp's turn of pages for every warp
   const long long segments = static_cast<long long>(p.rows) * p.kv_heads;
   int parts = 1;
-  while (parts < kMostBlocks && segments * parts * 2 <= 2 * kNumSMs && p.table_width >= parts * 2 * kWarps * kAhead / 2) parts *= 2;
-  return segments * parts <= 2 * kNumSMs ? launch<T, LANES, 2>(p, parts, stream) : launch<T, LANES, 3>(p, parts, stream);
+  while (parts < kMostBlocks && segments * parts * 2 <= 2 * kNumSMs && p.table_width >= parts * kMostWarps * kAhead) parts *= 2;
+  const size_t smem = static_cast<size_t>(std::max(p.table_width, 1)) * (sizeof(Key) + sizeof(uint32_t));
+  if (segments * parts <= 2 * kNumSMs) return launch<T, LANES, 256, 2>(p, parts, smem, stream);
+  return smem <= kSmallSmem ? launch<T, LANES, 128, 6>(p, parts, smem, stream) : launch<T, LANES, 256, 3>(p, parts, smem, stream);
 }
 
 template <typename T>

@@ -457,6 +457,29 @@ def test_selection(lengths, heads, kv_heads, dim, page, count, first, last, dtyp
     assert torch.equal(got.cpu(), U.select(q, boxes, table, lengths, page, count, first, last))
 
 
+@pytest.mark.parametrize("rows,heads,kv_heads,dim,longest,count", [
+    (300, 4, 1, 128, 40 * 16, 9),      # more blocks than two an SM
+    (150, 6, 3, 64, 300 * 16, 33),
+    (310, 1, 1, 24, 2500 * 16, 64),    # and more scores than leave room for six
+    (9, 64, 32, 128, 70 * 16 + 1, 70),
+])
+def test_selection_of_many_rows_that_share_a_table(rows, heads, kv_heads, dim, longest, count):
+    gen = torch.Generator().manual_seed(rows)
+    pages = (longest + 15) // 16
+    boxes = torch.randn(pages + 2, kv_heads, 2, dim, generator=gen).sort(2).values.half().to(DEV)
+    table = (torch.randperm(pages + 2, generator=gen)[:pages].int().to(DEV)).expand(rows, -1).contiguous()
+    q = torch.randn(rows, heads, dim, generator=gen).half().to(DEV)
+    lengths = torch.randint(0, longest + 1, (rows,), generator=gen)
+    lengths[0], lengths[1], lengths[2] = longest, 0, 1
+    got = paged.paged_select(q, boxes, table, ints(lengths.tolist()), 16, count)
+    # the same, row by row, and a few of them by definition
+    for i in range(0, rows, 37):
+        one = paged.paged_select(q[i:i + 1], boxes, table[i:i + 1], ints([int(lengths[i])]), 16, count)
+        assert torch.equal(got[i:i + 1], one), i
+    some = [0, 1, 2, rows - 1]
+    assert torch.equal(got[some].cpu(), U.select(q[some], boxes, table[some], [int(lengths[i]) for i in some], 16, count, 1, 1))
+
+
 def test_selection_of_equal_scores_takes_the_lower_pages():
     lengths = [1600, 1600, 333]
     q, k, v, table, held = case(lengths, 4, 2, 64, 16, F16)
