@@ -198,7 +198,8 @@ template <int THREADS, typename K>
 __device__ __forceinline__ Border<K> find_border(const K* keys, int from, int to, K least, K most, uint32_t need, Shared& sh) {
   const int lane = threadIdx.x & 31;
   if (need == 0) return {static_cast<K>(~K(0)), static_cast<K>(~K(0)), 0};
-  for (int round = 0; least != most; ++round) {
+  constexpr int kRounds = (8 * sizeof(K) + kBits - 1) / kBits;  // each leaves kBits fewer
+  for (int round = 0; least != most && round < kRounds; ++round) {
     const K span = most - least;
     const int shift = max(0, static_cast<int>(8 * sizeof(K)) - kBits - leading_zeros(span));  // span >> shift is below kBins
     uint32_t* const bins = sh.bins[round % 3];
@@ -217,7 +218,7 @@ __device__ __forceinline__ Border<K> find_border(const K* keys, int from, int to
     const int first = find_lane(groups[lane], need, in_bin) * 32;
     const int bin = first + find_lane(bins[first + lane], need, in_bin);
     least += static_cast<K>(bin) << shift;
-    most = min(most, least + ((K(1) << shift) - 1));
+    most = least + min(most - least, (K(1) << shift) - 1);  // the last bin may reach over the largest number
     if (in_bin == need) break;
   }
   return {least, most, need};

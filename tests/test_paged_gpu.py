@@ -564,6 +564,26 @@ def test_selection_of_scores_that_are_not_finite():
         assert torch.equal(got.cpu(), U.select(q, boxes, table, lengths, 16, count, 0, 0)), count
 
 
+@pytest.mark.parametrize("value", (float("nan"), float("inf"), float("-inf")))
+@pytest.mark.parametrize("dim,rows", ((128, 3), (8, 3), (40, 320)))
+def test_selection_with_more_infinite_scores_than_are_wanted(dim, rows, value):
+    """The border lies among scores that are not numbers, the largest keys that there are, beside ones of any size."""
+    gen = torch.Generator().manual_seed(dim)
+    pages = 150
+    boxes = torch.randn(pages, 1, 2, dim, generator=gen).sort(2).values.half()
+    strange = torch.randperm(pages, generator=gen)[:60]
+    boxes[strange, :, int(value != float("-inf")), 3] = value
+    boxes = boxes.to(DEV)
+    table = torch.stack([torch.randperm(pages, generator=gen) for _ in range(rows)]).int().to(DEV)
+    q = torch.randn(rows, 2, dim, generator=gen).half().to(DEV)
+    lengths = [pages * 16 - 5 * i for i in range(rows)]
+    some = list(range(0, rows, 45))
+    for count in (1, 2, 3, 7, 30, 61, 62, 63, 100):
+        first = min(1, count - 1)
+        got = paged.paged_select(q, boxes, table, ints(lengths), 16, count, first, 0)
+        assert torch.equal(got[some].cpu(), U.select(q[some], boxes, table[some], [lengths[i] for i in some], 16, count, first, 0)), count
+
+
 def test_selection_by_queries_that_are_not_finite():
     lengths = [1600] * 4
     q, k, v, table, held = case(lengths, 4, 2, 64, 16, F16)
