@@ -208,7 +208,7 @@ def _plain_append(state):
     seq = seq.clamp(max=lengths.numel() - 1)
     at = lengths[seq] - (cu[seq + 1] - row)
     real &= at >= 0
-    at = torch.where(real, at, 0)  # rows of no sequence have no angles of their own
+    at = at.clamp(min=0)
     c, s, interleaved = cos[at], sin[at], state["case"]["interleaved"]
     q_out = (_rotate(q.float(), c, s, interleaved) * real[:, None, None]).to(q.dtype)
     live = real.nonzero().flatten()
