@@ -19,7 +19,7 @@ behind the pages it needs is not read), ``lengths`` int32 ``[rows]`` how many po
 length 0 is idle.  Heads are grouped: query heads ``h * heads / kv_heads`` and the following read key head ``h``.
 
 The operators run on the current stream, read nothing back and can be captured into a CUDA graph.  They have no backward
-pass: operands that require a gradient are refused.  ``PagedKVCache`` owns the tensors and passes them along.
+pass and no forward derivatives: operands that require a gradient or have a tangent are refused.  ``PagedKVCache`` owns the tensors and passes them along.
 """
 from __future__ import annotations
 

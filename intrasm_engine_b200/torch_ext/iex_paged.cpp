@@ -1,8 +1,11 @@
 // Operators of the paged key-value cache: argument checks, outputs, and the calls of the C ABI (paged_append.cu,
-// paged_attention.cu, paged_select.cu).  They serve: operands that require gradients are refused.
+// paged_attention.cu, paged_select.cu).  They serve: operands that require gradients or have tangents are refused.
 #include "iex_torch_ops.h"
 
+#include <ATen/core/LegacyTypeDispatch.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/core/grad_mode.h>
+#include <ATen/core/stack.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -14,13 +17,20 @@ namespace {
 
 constexpr int64_t kMostInt = std::numeric_limits<int>::max();
 
+// Without a derivative an output that has none of its own would say that it is zero.
+void check_not_differentiated(const std::string& name, const at::Tensor& t) {
+  TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), name,
+              " requires a gradient: the operators of the paged cache have no backward pass");
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), name,
+                              " has a tangent: the operators of the paged cache have no forward derivatives");
+}
+
 void check_on(const at::Tensor& first, std::initializer_list<std::pair<const char*, const at::Tensor*>> named) {
   TORCH_CHECK(first.is_cuda(), "the operators of the paged cache take CUDA tensors");
   for (const auto& [name, t] : named) {
     TORCH_CHECK(t->device() == first.device(), name, " should be in the same device as the first argument");
     TORCH_CHECK(!t->is_sparse(), name, " must be a dense tensor");
-    TORCH_CHECK(!(t->requires_grad() && at::GradMode::is_enabled()), name,
-                " requires a gradient: the operators of the paged cache have no backward pass");
+    check_not_differentiated(name, *t);
   }
 }
 
@@ -79,6 +89,18 @@ void check_table(const at::Tensor& block_table, const at::Tensor& lengths) {
 // A cache that is written: what was saved of it before is seen to have changed.
 void written(const at::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// Calls through the dispatcher, ahead of the kernels: a function transform (torch.func.jvp, torch.func.grad) hands these a tensor
+// without what it is differentiated by.
+void refuse_derivatives(const c10::OperatorHandle& op, c10::DispatchKeySet keys, torch::jit::Stack* stack) {
+  const auto& arguments = op.schema().arguments();
+  const auto operands = torch::jit::last(stack, arguments.size());
+  for (size_t i = 0; i < arguments.size(); ++i)
+    if (operands[i].isTensor() && operands[i].toTensor().defined())
+      check_not_differentiated(arguments[i].name(), operands[i].toTensor());
+  at::AutoDispatchBelowAutograd below;
+  op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
 }
 
 const int32_t* ints(const at::Tensor& t) { return t.data_ptr<int>(); }
@@ -222,4 +244,9 @@ TORCH_LIBRARY_IMPL(iex_ops, CUDA, m) {
   m.impl("paged_append", &iex_torch::paged_append);
   m.impl("paged_attention", &iex_torch::paged_attention);
   m.impl("paged_select", &iex_torch::paged_select);
+}
+
+TORCH_LIBRARY_IMPL(iex_ops, Autograd, m) {
+  for (const char* name : {"paged_append", "paged_attention", "paged_select"})
+    m.impl(name, torch::CppFunction::makeFromBoxedFunction<&iex_torch::refuse_derivatives>());
 }

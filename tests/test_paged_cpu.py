@@ -45,6 +45,27 @@ def test_cpu_tensors_reach_no_implementation():
             call()
 
 
+def test_derivatives_are_refused_ahead_of_any_implementation():
+    """Calls through the dispatcher, function transforms among them: no output without a gradient or a tangent."""
+    from torch.autograd import forward_ad
+    q = torch.ones(1, 2, 64, dtype=torch.float16)
+    cache = torch.zeros(3, 2, 16, 64, dtype=torch.float16)
+    boxes = torch.zeros(3, 2, 2, 64, dtype=torch.float16)
+    table, lengths = torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    calls = (lambda q: torch.ops.iex_ops.paged_append(q, q.detach(), q.detach(), cache, cache.clone(), table, lengths),
+             lambda q: torch.ops.iex_ops.paged_attention(q, cache, cache, table, lengths),
+             lambda q: torch.ops.iex_ops.paged_select(q, boxes, table, lengths, 16, 2).float())
+    for call in calls:
+        with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="q has a tangent"):
+            call(forward_ad.make_dual(q, torch.ones_like(q)))
+        with pytest.raises(NotImplementedError, match="q has a tangent"):
+            torch.func.jvp(call, (q,), (torch.ones_like(q),))
+        with pytest.raises(RuntimeError, match="q requires a gradient"):
+            torch.func.grad(lambda x: call(x).sum())(q)
+        with pytest.raises(RuntimeError, match="q requires a gradient"):
+            call(q.clone().requires_grad_(True))
+
+
 def test_schemas_name_what_is_written():
     text = str(torch.ops.iex_ops.paged_append.default._schema)
     assert "Tensor(a!) k_cache" in text and "Tensor(b!) v_cache" in text and "Tensor(c!)? boxes" in text
