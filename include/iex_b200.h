@@ -557,6 +557,7 @@ IEX_API int iex_paged_append(int tokens, int batch, int heads, int kv_heads, int
 
 /* out[r, h] = sum_t softmax_t(scale * q[r, h] . k[t]) v[t] over the positions that row r
  * holds; zero where there are none (or every score is -inf).  heads / kv_heads query heads share a key head.
+ * Products q . k, and scores times log2(e), are fp32: they have to stay in its range; scale * log2(e) must be finite.
  * pages (or NULL) int32 [rows, kv_heads, count]: only the pages with these places in the row
  * of the table, the first min(count, pages held) entries; entries that are no held page are
  * skipped, one that is there twice counts twice.

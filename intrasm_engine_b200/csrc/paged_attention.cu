@@ -746,6 +746,8 @@ extern "C" int iex_paged_attention(int rows, int heads, int kv_heads, int head_d
   using namespace iex::paged;
   if (rows < 0 || num_pages < 0 || table_width < 0 || count < 0) return IEX_ERR_BAD_ARG;
   if (!iex_paged_attention_supported(heads, kv_heads, head_dim, page_size)) return IEX_ERR_UNSUPPORTED;
+  const float scale_log2 = static_cast<float>(scale * 1.4426950408889634);  // of a score, in an exponent of 2
+  if (!std::isfinite(scale_log2)) return IEX_ERR_BAD_ARG;
   if (rows == 0) return IEX_OK;
   if (!q || !out || !lengths || (table_width > 0 && !block_table) || (num_pages > 0 && (!k_cache || !v_cache)))
     return IEX_ERR_BAD_ARG;
@@ -756,7 +758,6 @@ extern "C" int iex_paged_attention(int rows, int heads, int kv_heads, int head_d
   const size_t need =
       iex_paged_attention_workspace_bytes(rows, heads, kv_heads, head_dim, num_pages, page_size, table_width, pages != nullptr, count);
   if (need > 0 && (!workspace || workspace_bytes < need)) return IEX_ERR_BAD_ARG;
-  const float scale_log2 = static_cast<float>(scale * 1.4426950408889634);
   if (pages != nullptr && shared_workspace_bytes(rows, heads, kv_heads, head_dim, num_pages, page_size, table_width, count) > 0) {
     SharedCall c{rows, heads, kv_heads, head_dim, num_pages, log2_of(page_size), table_width, count, {q, q_row, q_head},
                  k_cache, v_cache, k_page, v_page, block_table, lengths, pages, scale_log2, out};

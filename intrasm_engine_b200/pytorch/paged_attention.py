@@ -63,6 +63,7 @@ def paged_append(q, k, v, k_cache, v_cache, block_table, lengths, cu_tokens=None
 def paged_attention(q, k_cache, v_cache, block_table, lengths, pages=None, scale: float | None = None) -> torch.Tensor:
     """``softmax(scale * q k^T) v`` of every row of ``q`` ``[rows, heads, head_dim]`` over the positions of its own row of
     ``block_table``; ``scale`` is ``head_dim ** -0.5`` by default.  Zeros for a row that holds nothing.
+    Scores are held in 32 bits, times ``log2(e)``; a ``scale`` that leaves their range is refused.
 
     A piece of a prompt is several rows with the same row of the table, each with the length that it sees.  ``pages`` int32
     ``[rows, kv_heads, count]`` restricts a row to these places of its row of the table, as ``paged_select`` returns them: of

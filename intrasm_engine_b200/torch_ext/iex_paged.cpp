@@ -188,7 +188,9 @@ at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const
     count = pages->size(2);
   }
   const double factor = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(kc.dim));
-  TORCH_CHECK(std::isfinite(static_cast<float>(factor)), "scale must be finite in 32 bits");
+  // the kernels' factor, of exponents of 2
+  TORCH_CHECK(std::isfinite(static_cast<float>(static_cast<float>(factor) * 1.4426950408889634)),
+              "scale * log2(e) must be finite in 32 bits");
   c10::cuda::CUDAGuard guard(q.device());
   at::Tensor out = empty(q, {rows, heads, kc.dim});
   if (rows == 0) return out;

@@ -73,6 +73,19 @@ def test_schemas_name_what_is_written():
     assert {"paged_append", "paged_attention", "paged_select"} <= set(ops.OP_NAMES)
 
 
+def test_attention_refuses_scales_that_overflow_as_exponents_of_two():
+    """The kernels' factor is scale * log2(e) in fp32: finite up to 2.3586e38.  Refused before any launch."""
+    x = 4096  # an aligned address that nothing reads
+    def attention(scale, rows):
+        return _lib.lib.iex_paged_attention(rows, 4, 2, 64, 0, x, 256, 64, x, 2048, x, 2048, 3, 16, x, 2, x, None, 0, scale, x, None, 0,
+                                            None)
+    for rows in (0, 1):
+        for scale in (3e38, -3e38, 2.36e38, 3.4028e38, float("inf"), float("nan")):
+            assert attention(scale, rows) == -1, scale
+    for scale in (2.35e38, -2.35e38, 0.0, 0.125):
+        assert attention(scale, 0) == 0, scale
+
+
 def test_entry_points_check_their_arguments():
     """The C ABI returns a status before any launch: nothing here needs a device."""
     lib, bad, unsupported, too_large = _lib.lib, -1, -2, -3

@@ -372,6 +372,16 @@ def test_attention_refuses_scales_that_are_not_finite_in_32_bits():
             paged.paged_attention(q, k, v, table, held, scale=scale)
 
 
+def test_attention_refuses_scales_whose_product_with_log2_e_overflows():
+    q, k, v, table, held = case([50, 20], 4, 2, 64, 16, F16)
+    for scale in (3e38, -3e38, 2.36e38):
+        with pytest.raises(RuntimeError, match="scale"):
+            paged.paged_attention(q, k, v, table, held, scale=scale)
+    q[...] = 0.0  # scores of 0, whatever the scale
+    for scale in (2.35e38, -2.35e38):
+        U.check_attention(paged.paged_attention(q, k, v, table, held, scale=scale), q, k, v, table, [50, 20], scale=scale)
+
+
 def test_attention_of_sequences_with_a_common_beginning():
     lengths = [100, 77, 64]
     q, k, v, table, held = case(lengths, 4, 2, 64, 16, F16)
