@@ -34,7 +34,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kMostWarps = 8;     // of a block
 constexpr int kAhead = 8;         // boxes that a lane has on their way
-constexpr int kMaxPages = 16384;  // 12 bytes of shared memory each
+constexpr int kMaxPages = 16384, kPageBytes = sizeof(unsigned long long) + sizeof(uint32_t);  // shared memory of each
 constexpr int kBits = 10, kBins = 1 << kBits;  // of a round
 constexpr int kMostBlocks = 8;                 // of a cluster
 constexpr size_t kSmallSmem = 22 * 1024;       // of which an SM has room for 6, beside what is fixed
@@ -481,7 +481,8 @@ template <typename T, int LANES, int THREADS, int BLOCKS>
 int launch(const SelectParams& p, int parts, size_t smem, cudaStream_t stream) {
   const auto kern = select_kernel<T, LANES, THREADS, BLOCKS>;
   if (smem > 32 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    // the kernel's, not the call's: with one value for all calls, host threads that launch at the same time agree on it
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxPages * kPageBytes);
     if (e != cudaSuccess) return static_cast<int>(e);
   }
   return launch_clusters<SelectParams>(kern, static_cast<unsigned>(p.rows) * p.kv_heads * parts, parts, THREADS, smem, stream, p);
@@ -493,7 +494,7 @@ int launch(const SelectParams& p, cudaStream_t stream) {
   const long long segments = static_cast<long long>(p.rows) * p.kv_heads;
   int parts = 1;
   while (parts < kMostBlocks && segments * parts * 2 <= 2 * kNumSMs && p.table_width >= parts * kMostWarps * kAhead) parts *= 2;
-  const size_t smem = static_cast<size_t>(std::max(p.table_width, 1)) * (sizeof(Key) + sizeof(uint32_t));
+  const size_t smem = static_cast<size_t>(std::max(p.table_width, 1)) * kPageBytes;
   if (segments * parts <= 2 * kNumSMs) return launch<T, LANES, 256, 2>(p, parts, smem, stream);
   return smem <= kSmallSmem ? launch<T, LANES, 128, 6>(p, parts, smem, stream) : launch<T, LANES, 256, 3>(p, parts, smem, stream);
 }
