@@ -30,7 +30,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kIndexThreads = 1024;
 constexpr int kTileRows = 64, kThreads = 128, kPositions = 64;
-constexpr int kMostPages = 16384;  // 12 bytes of shared memory each
+constexpr int kMostPages = 16384, kPageBytes = 3 * sizeof(int);  // shared memory of each
 constexpr int kIndexBlocks = 8;    // of a cluster, at most
 constexpr int kMostGroup = 16;
 
@@ -419,9 +419,10 @@ template <typename T, int PIECES>
 int launch(const Params& p, cudaStream_t stream) {
   const SharedCall& c = p.c;
   constexpr int bytes = (kTileRows + 2 * kPositions) * (64 * PIECES + 8) * 2;
-  const int counters = 3 * c.num_pages * static_cast<int>(sizeof(int));
+  const int counters = c.num_pages * kPageBytes;
   if (counters > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(index_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, counters);
+    // the kernel's, not the call's: with one value for all calls, host threads that launch at the same time agree on it
+    const cudaError_t e = cudaFuncSetAttribute(index_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostPages * kPageBytes);
     if (e != cudaSuccess) return static_cast<int>(e);
   }
   if (bytes > 40 * 1024) {

@@ -53,3 +53,33 @@ def test_selection_from_a_wide_and_from_a_narrow_table():
     torch.cuda.synchronize()
     assert at_once(calls, 4000) == []
     assert all(torch.equal(a, out) for a, (_, _, out, _) in zip(alone, outs))
+
+
+def test_listed_pages_of_a_large_and_of_a_small_cache():
+    rows, count, dim, page, width = 4096, 16, 8, 256, 32
+    q = torch.randn(rows, 1, dim, device=DEV).half()
+    held = torch.full((rows,), width * page, device=DEV, dtype=torch.int32)
+    pages = torch.rand(rows, 1, width, device=DEV).argsort(-1)[..., :count].int().contiguous()
+    calls, outs = [], []
+    for total in (6000, 3500, 5000, 3450):
+        k, v = (torch.randn(total, 1, page, dim, device=DEV).half() for _ in range(2))
+        table = torch.randint(0, total, (1, width), device=DEV, dtype=torch.int32).expand(rows, -1).contiguous()
+        need = _lib.lib.iex_paged_attention_workspace_bytes(rows, 1, 1, dim, total, page, width, 1, count)
+        assert need > 2 << 20  # by page; row by row needs less
+        out, ws = torch.empty_like(q), torch.empty(need, device=DEV, dtype=torch.uint8)
+        stream = torch.cuda.Stream()
+        outs.append((out, ws, k, v, table, stream))
+        calls.append(lambda total=total, k=k, v=v, table=table, out=out, ws=ws, stream=stream: _lib.lib.iex_paged_attention(
+            rows, 1, 1, dim, 0, q.data_ptr(), dim, dim, k.data_ptr(), page * dim, v.data_ptr(), page * dim, total, page,
+            table.data_ptr(), width, held.data_ptr(), pages.data_ptr(), count, 0.125, out.data_ptr(), ws.data_ptr(),
+            ws.numel(), stream.cuda_stream))
+    torch.cuda.synchronize()
+    for call in calls:
+        assert call() == 0
+    torch.cuda.synchronize()
+    alone = [o[0].clone() for o in outs]
+    for o in outs:
+        o[0].fill_(float("nan"))
+    torch.cuda.synchronize()
+    assert at_once(calls, 400) == []
+    assert all(torch.equal(a, o[0]) for a, o in zip(alone, outs))
