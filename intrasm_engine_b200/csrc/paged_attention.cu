@@ -22,7 +22,8 @@
 //   O^T = V^T P^T  a lane's 16 bytes of four positions, bytes paired up by prmt, are its fragments of four; the scores'
 //                  accumulators become P^T by movmatrix
 // The running maximum, sum and O are fp32.  P enters the second product as a 16-bit head and the 16-bit rest, so that what is lost of it
-// does not show beside the output's own rounding; fp16 weights carry 2^15, which keeps small ones out of the subnormals.
+// does not show beside the output's own rounding; fp16 weights carry 2^15, which keeps small ones out of the subnormals.  bfloat16 values may be
+// so large that their sum leaves fp32 although their average does not: see Walk::run and join.
 #include <algorithm>
 #include <cmath>
 
@@ -94,6 +95,12 @@ template <typename T, int PIECES, int NT>
 struct Walk {
   static constexpr int kHeads = 8 * NT, kDim = 64 * PIECES, kPitch = kDim + 4;
   float o[NT][PIECES][4][4], top[NT][2], sum[NT][2];
+
+  // Where keep() puts o[n][i][j][e].
+  static __device__ __forceinline__ int place(int n, int i, int j, int e) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    return (n * 8 + 2 * q + (e & 1)) * kPitch + i * 64 + g * 8 + 2 * j + (e >> 1);
+  }
 
   // `scratch`: kHeads x kPitch of shared memory that is this warp's; `here`: query heads that there are; `early`: the lane's page of the
   // first 32, looked up before the row's length was known
@@ -185,9 +192,13 @@ struct Walk {
         }
     };
 
-    // A rest of a weight that is 0 or below would turn an infinite element of v into NaN.  So where elements of the product
-    // come out not finite, it is formed a second time with all weights above zero as 1, and those elements are taken from there.
-    for (bool again = false;;) {
+    // Where elements of the product come out not finite, either v has infinite or NaN elements, of which a rest of a weight that is
+    // 0 or below makes NaN, or large elements of v add up to more than fp32 holds.  The product is formed a second time with all weights
+    // above zero as one number of which no sum overflows: what is not finite then is taken from there.  What is, is formed a third
+    // time, with weights made as small, and divided by the weights' sum.
+    enum { kReal, kPlaces, kSmaller };
+    int pass = kReal;
+    for (;;) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         top[n][0] = top[n][1] = -INFINITY;
@@ -254,16 +265,17 @@ struct Walk {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[n][i][j][e] *= old[e & 1];
           }
-          if (again) {
+          if (pass != kReal) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = s[n][e] > 0.f ? 1.f : s[n][e];
+            for (int e = 0; e < 4; ++e)
+              s[n][e] = pass == kSmaller ? s[n][e] * Half2<T>::kSmall : s[n][e] > 0.f ? Half2<T>::kSmall : s[n][e];
           }
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             const uint32_t both = Half2<T>::pack(s[n][2 * t], s[n][2 * t + 1]);
             const float2 kept = Half2<T>::unpack(both);
             head[n][t] = transposed(both);
-            rest[n][t] = transposed(again ? 0 : Half2<T>::pack(s[n][2 * t] - kept.x, s[n][2 * t + 1] - kept.y));
+            rest[n][t] = transposed(pass == kPlaces ? 0 : Half2<T>::pack(s[n][2 * t] - kept.x, s[n][2 * t + 1] - kept.y));
           }
         }
 #pragma unroll
@@ -277,27 +289,14 @@ struct Walk {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               mma<T>(o[n][i][j], a0, a1, a2, a3, head[n][0], head[n][1]);
-              if (!again) mma<T>(o[n][i][j], a0, a1, a2, a3, rest[n][0], rest[n][1]);
+              if (pass != kPlaces) mma<T>(o[n][i][j], a0, a1, a2, a3, rest[n][0], rest[n][1]);
             }
           }
         request_v(next);
         now = next;
       }
-      if (again) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < PIECES; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float before = scratch[(n * 8 + 2 * q + (e & 1)) * kPitch + i * 64 + g * 8 + 2 * j + (e >> 1)];
-                if (fabsf(before) < INFINITY) o[n][i][j][e] = before;
-              }
-        break;
-      }
-      bool odd = false;
+      if (pass == kSmaller) break;
+      bool odd = false;  // another pass is needed
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -305,15 +304,44 @@ struct Walk {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) odd |= (n * 8 + 2 * q + (e & 1) < here) & !(fabsf(o[n][i][j][e]) < INFINITY);
+            for (int e = 0; e < 4; ++e) {
+              float& mine = o[n][i][j][e];
+              const bool there = n * 8 + 2 * q + (e & 1) < here;
+              if (pass == kReal) {
+                odd |= there & !finite(mine);
+              } else {
+                const float before = scratch[place(n, i, j, e)];
+                const bool large = Half2<T>::kOverflows && !finite(before) && finite(mine);
+                odd |= there & large;
+                mine = finite(before) ? before : large ? INFINITY : mine;
+              }
+            }
       if (!__any_sync(0xffffffffu, odd)) break;
       keep(scratch);
-      again = true;
+      pass = pass == kReal ? kPlaces : kSmaller;
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) sum[n][e] = sum_over_positions(sum[n][e]);
+    if (Half2<T>::kOverflows && pass == kSmaller) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float factor = to_average<T>(sum[n][e & 1]);
+#pragma unroll
+          for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float& mine = o[n][i][j][e];
+              const float before = scratch[place(n, i, j, e)];
+              mine = finite(before) ? before * factor : finite(mine) ? mine * factor * (1.f / Half2<T>::kSmall) : before;
+            }
+        }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) sum[n][0] = -sum[n][0], sum[n][1] = -sum[n][1];
+    }
   }
 
   // The product as it is, [kHeads][kPitch]; every lane writes what it alone reads again.
@@ -346,7 +374,7 @@ struct Walk {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int h = n * 8 + 2 * q + e;
-        const float factor = sum[n][e] == 0.f ? 0.f : 1.f / sum[n][e];
+        const float factor = to_average<T>(sum[n][e]);
         T* const to = static_cast<T*>(p.out) + (static_cast<long long>(row) * p.heads + head0 + h) * p.dim;
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
@@ -363,27 +391,50 @@ struct Walk {
 struct Joined {
   float high, sum, o[4];
 };
-template <typename Stats, typename Product>
-__device__ __forceinline__ Joined join(int from, int until, Stats stats, Product product) {
+// `each` calls what it gets for every part, in order; stats: its maximum and sum; product: its elements.  No more than MOST parts:
+// products that are finite may add up to more than fp32 holds, so that they and the sums get a factor.
+template <typename T, int MOST, typename Each, typename Stats, typename Product>
+__device__ __forceinline__ Joined join(Each each, Stats stats, Product product) {
+  constexpr float kUnit = Half2<T>::kOverflows ? 1.f / MOST : 1.f;
+  static_assert((MOST & (MOST - 1)) == 0, "an exact factor");
   Joined j{-INFINITY, 0.f, {0.f, 0.f, 0.f, 0.f}};
-  for (int i = from; i < until; ++i) j.high = fmaxf(j.high, stats(i).x);
+  bool any_averaged = false;
+  each([&](int i) {
+    const float2 s = stats(i);
+    j.high = fmaxf(j.high, s.x);
+    any_averaged |= averaged<T>(s.y);
+  });
   const float base = j.high == -INFINITY ? 0.f : j.high;
-  for (int i = from; i < until; ++i) {
+  each([&](int i) {
     const float2 s = stats(i);
     const float4 v = product(i);
-    const float weight = exp2f(s.x - base);
-    j.sum += s.y * weight;
+    const float weight = exp2f(s.x - base) * kUnit;
+    j.sum += (Half2<T>::kOverflows ? fabsf(s.y) : s.y) * weight;
     j.o[0] += v.x * weight;
     j.o[1] += v.y * weight;
     j.o[2] += v.z * weight;
     j.o[3] += v.w * weight;
+  });
+  if (any_averaged) {  // then this is an average, too
+    const float factor = to_average<T>(j.sum);
+    j.o[0] = j.o[1] = j.o[2] = j.o[3] = 0.f;
+    each([&](int i) {
+      const float2 s = stats(i);
+      const float4 v = product(i);
+      const float weight = exp2f(s.x - base) * kUnit * factor * (averaged<T>(s.y) ? -s.y : 1.f);
+      j.o[0] += v.x * weight;
+      j.o[1] += v.y * weight;
+      j.o[2] += v.z * weight;
+      j.o[3] += v.w * weight;
+    });
+    j.sum = -j.sum;
   }
   return j;
 }
 template <typename T>
 __device__ __forceinline__ void write4(const AttentionParams& p, int row, int head, int d, float sum, float o0, float o1, float o2,
                                        float o3) {
-  const float factor = sum == 0.f ? 0.f : 1.f / sum;
+  const float factor = to_average<T>(sum);
   T* const to = static_cast<T*>(p.out) + (static_cast<long long>(row) * p.heads + head) * p.dim + d;
   *reinterpret_cast<uint2*>(to) = make_uint2(Half2<T>::pack(o0 * factor, o1 * factor), Half2<T>::pack(o2 * factor, o3 * factor));
 }
@@ -519,26 +570,18 @@ __global__ void __launch_bounds__(32 * warps_of(PIECES, NT), 1) attention_kernel
     for (; turn < most_heads; turn += kWarps) {
       if (turn >= here) continue;
       const int h = turn;
-      float high = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-      for (uint32_t m = members; m != 0; m &= m - 1) high = fmaxf(high, stats_of_warps[(__ffs(m) - 1) * kHeads + h].x);
-      const float base = high == -INFINITY ? 0.f : high;
-      for (uint32_t m = members; m != 0; m &= m - 1) {
-        const int i = (__ffs(m) - 1) * kHeads + h;
-        const float2 s = stats_of_warps[i];
-        const float4 v = d < p.dim ? *reinterpret_cast<const float4*>(parts_of_warps + i * kPitch + d) : float4{};
-        const float weight = exp2f(s.x - base);
-        sum += s.y * weight;
-        o[0] += v.x * weight;
-        o[1] += v.y * weight;
-        o[2] += v.z * weight;
-        o[3] += v.w * weight;
-      }
+      const Joined j = join<T, 32>(
+          [&](auto add) {
+            for (uint32_t m = members; m != 0; m &= m - 1) add(__ffs(m) - 1);
+          },
+          [&](int i) { return stats_of_warps[i * kHeads + h]; },
+          [&](int i) { return d < p.dim ? *reinterpret_cast<const float4*>(parts_of_warps + (i * kHeads + h) * kPitch + d) : float4{}; });
       if (begins && finished) {
-        if (d < p.dim) write4<T>(p, seg_row, head0 + h, d, sum, o[0], o[1], o[2], o[3]);
+        if (d < p.dim) write4<T>(p, seg_row, head0 + h, d, j.sum, j.o[0], j.o[1], j.o[2], j.o[3]);
       } else {
         const long long slot = (static_cast<long long>(blockIdx.x) * 2 + begins) * kHeads + h;
-        if (d < p.dim) *reinterpret_cast<float4*>(p.product + slot * kDim + d) = make_float4(o[0], o[1], o[2], o[3]);
-        if (lane == 0) p.stats[slot] = make_float2(high, sum);
+        if (d < p.dim) *reinterpret_cast<float4*>(p.product + slot * kDim + d) = make_float4(j.o[0], j.o[1], j.o[2], j.o[3]);
+        if (lane == 0) p.stats[slot] = make_float2(j.high, j.sum);
       }
     }
     turn -= most_heads;
@@ -590,8 +633,11 @@ __global__ void __launch_bounds__(32 * kClusterWarps, 1) cluster_kernel(const __
   if (blocks > 1) cluster_wait_begun();
   for (int x = threadIdx.x; x < here * vectors; x += kThreads) {
     const int h = x / vectors, d = (x - h * vectors) * 4;
-    const Joined j = join(
-        0, working, [&](int i) { return stats_of_warps[i][h]; },
+    const Joined j = join<T, kClusterWarps>(
+        [&](auto add) {
+          for (int i = 0; i < working; ++i) add(i);
+        },
+        [&](int i) { return stats_of_warps[i][h]; },
         [&](int i) { return *reinterpret_cast<const float4*>(parts_of_warps + (i * kHeads + h) * kPitch + d); });
     if (blocks == 1) {
       write4<T>(p, row, head0 + h, d, j.sum, j.o[0], j.o[1], j.o[2], j.o[3]);
@@ -606,8 +652,11 @@ __global__ void __launch_bounds__(32 * kClusterWarps, 1) cluster_kernel(const __
   for (int x = threadIdx.x; x < heads_each * vectors; x += kThreads) {
     const int nth = x / vectors, h = nth * blocks + rank, d = (x - nth * vectors) * 4;
     if (h >= here) break;
-    const Joined j = join(
-        0, blocks, [&](int i) { return received_stats[i * heads_each + nth]; },
+    const Joined j = join<T, kMostBlocks>(
+        [&](auto add) {
+          for (int i = 0; i < blocks; ++i) add(i);
+        },
+        [&](int i) { return received_stats[i * heads_each + nth]; },
         [&](int i) { return *reinterpret_cast<const float4*>(&received[i * heads_each + nth][d]); });
     write4<T>(p, row, head0 + h, d, j.sum, j.o[0], j.o[1], j.o[2], j.o[3]);
   }
@@ -630,26 +679,51 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = lane * 4;
   const int n = open.y - static_cast<int>(blockIdx.x) + 1;
   // every warp joins a quarter of the parts, and the first one the quarters
+  static_assert(kNumSMs <= 256 * kJoinWarps, "parts of a warp");
+  constexpr float kUnit = Half2<T>::kOverflows ? 1.f / 256 : 1.f;  // as in join()
   float high = -INFINITY, sum = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  bool any_averaged = false;
+  const auto slot_of = [&](int i) { return (static_cast<long long>(blockIdx.x + i) * 2 + (i == 0)) * kHeads + h; };
+  const auto product_of = [&](long long slot) { return *reinterpret_cast<const float4*>(p.product + slot * kDim + (d < p.dim ? d : 0)); };
   for (int i = warp; i < n; i += kJoinWarps) {
-    const long long slot = (static_cast<long long>(blockIdx.x + i) * 2 + (i == 0)) * kHeads + h;
+    const long long slot = slot_of(i);
     const float2 s = p.stats[slot];
-    const float4 v = *reinterpret_cast<const float4*>(p.product + slot * kDim + (d < p.dim ? d : 0));
+    const float4 v = product_of(slot);
     const float next = fmaxf(high, s.x), base = next == -INFINITY ? 0.f : next;
-    const float old = exp2f(high - base), weight = exp2f(s.x - base);
+    const float old = exp2f(high - base), weight = exp2f(s.x - base) * kUnit;
     high = next;
-    sum = sum * old + s.y * weight;
+    any_averaged |= averaged<T>(s.y);
+    sum = sum * old + (Half2<T>::kOverflows ? fabsf(s.y) : s.y) * weight;
     o.x = o.x * old + v.x * weight;
     o.y = o.y * old + v.y * weight;
     o.z = o.z * old + v.z * weight;
     o.w = o.w * old + v.w * weight;
   }
+  if (any_averaged) {
+    const float factor = to_average<T>(sum), base = high == -INFINITY ? 0.f : high;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = warp; i < n; i += kJoinWarps) {
+      const long long slot = slot_of(i);
+      const float2 s = p.stats[slot];
+      const float4 v = product_of(slot);
+      const float weight = exp2f(s.x - base) * kUnit * factor * (averaged<T>(s.y) ? -s.y : 1.f);
+      o.x += v.x * weight;
+      o.y += v.y * weight;
+      o.z += v.z * weight;
+      o.w += v.w * weight;
+    }
+    sum = -sum;
+  }
   if (lane == 0) stats[warp] = make_float2(high, sum);
   products[warp][lane] = o;
   __syncthreads();
   if (warp != 0 || d >= p.dim) return;
-  const Joined j = join(0, kJoinWarps, [&](int i) { return stats[i]; }, [&](int i) { return products[i][lane]; });
+  const Joined j = join<T, kJoinWarps>(
+      [&](auto add) {
+        for (int i = 0; i < kJoinWarps; ++i) add(i);
+      },
+      [&](int i) { return stats[i]; }, [&](int i) { return products[i][lane]; });
   write4<T>(p, row, head0 + h, d, j.sum, j.o[0], j.o[1], j.o[2], j.o[3]);
 }
 

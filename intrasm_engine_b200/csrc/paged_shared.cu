@@ -14,7 +14,8 @@
 // of P in O = P V; P enters as a 16-bit head and rest.
 //
 // Rows of one tile see different numbers of the page's positions.  An infinite or NaN value of v that one row sees must not
-// reach the others (0 x Inf): rows whose product comes out not finite are summed again, position by position.
+// reach the others (0 x Inf): rows whose product comes out not finite are summed again, position by position, and, as large bfloat16
+// values may be the reason, handed on as averages.
 #include <algorithm>
 
 #include <cooperative_groups.h>
@@ -337,6 +338,7 @@ __global__ void __launch_bounds__(kThreads) page_kernel(const __grid_constant__ 
       found &= ~(0xfu << row_here * 4);
       const long long slot = (head_at + entry_of[m]) * group + m % group;
       const int d = lane * 4;
+      constexpr float kSmall = Half2<T>::kOverflows ? 1.f / (2 * kMaxPage) : 1.f;  // of which the page's sum does not overflow
       float top = -INFINITY, total = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
       for (int t = 0; t < valid_of[m]; ++t) {
         float score = 0.f;
@@ -349,12 +351,37 @@ __global__ void __launch_bounds__(kThreads) page_kernel(const __grid_constant__ 
         top = now;
         total = total * before + weight;
         if (d < c.dim)
-          for (int i = 0; i < 4; ++i) acc[i] = acc[i] * before + weight * as_float(v_page[static_cast<long long>(t) * c.dim + d + i]);
+          for (int i = 0; i < 4; ++i) acc[i] = acc[i] * before + weight * kSmall * as_float(v_page[static_cast<long long>(t) * c.dim + d + i]);
+      }
+      if (Half2<T>::kOverflows) {
+        const float factor = to_average<T>(total);
+        for (float& v : acc) v = v * factor * (1.f / kSmall);
+        total = -total;
       }
       __syncwarp();
       if (d < c.dim) *reinterpret_cast<float4*>(p.product + slot * c.dim + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
       if (lane == 0) p.stats[slot] = make_float2(top, total);
     }
+  }
+}
+
+// Four elements of a query head's average, where an entry's are averages; total: of the weights.
+template <typename T>
+__device__ __noinline__ void join_averages(const Params& p, long long first, int g, int group, int d, float base, float unit, float total,
+                                           float (&o)[4]) {
+  const SharedCall& c = p.c;
+  const float factor = to_average<T>(total);
+  o[0] = o[1] = o[2] = o[3] = 0.f;
+  for (int i = 0; i < c.count; ++i) {
+    const long long slot = first + static_cast<long long>(i) * group + g;
+    const float2 s = p.stats[slot];
+    if (s.x == -INFINITY && s.y == 0.f) continue;
+    const float4 v = *reinterpret_cast<const float4*>(p.product + slot * c.dim + d);
+    const float weight = exp2f(s.x - base) * unit * factor * (averaged<T>(s.y) ? -s.y : 1.f);
+    o[0] += v.x * weight;
+    o[1] += v.y * weight;
+    o[2] += v.z * weight;
+    o[3] += v.w * weight;
   }
 }
 
@@ -366,11 +393,18 @@ __global__ void __launch_bounds__(kThreads) join_entries_kernel(const __grid_con
   const SharedCall& c = p.c;
   const int row = blockIdx.x / c.kv_heads, kv = blockIdx.x - row * c.kv_heads, group = c.heads / c.kv_heads, vectors = c.dim / 4;
   const long long first = (static_cast<long long>(kv) * p.entries + static_cast<long long>(row) * c.count) * group;
+  // products that are finite may add up to more than fp32 holds: an exact factor, no more than one over their number
+  const float unit = Half2<T>::kOverflows ? __int_as_float((127 - 32 + __clz(c.count)) << 23) : 1.f;
   for (int x = threadIdx.x; x < group * vectors; x += kThreads) {
     const int g = x / vectors, d = (x - g * vectors) * 4;
     float high = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    bool any_averaged = false;
 #pragma unroll 4
-    for (int i = 0; i < c.count; ++i) high = fmaxf(high, p.stats[first + static_cast<long long>(i) * group + g].x);
+    for (int i = 0; i < c.count; ++i) {
+      const float2 s = p.stats[first + static_cast<long long>(i) * group + g];
+      high = fmaxf(high, s.x);
+      any_averaged |= averaged<T>(s.y);
+    }
     const float base = high == -INFINITY ? 0.f : high;
 #pragma unroll 4
     for (int i = 0; i < c.count; ++i) {
@@ -379,14 +413,15 @@ __global__ void __launch_bounds__(kThreads) join_entries_kernel(const __grid_con
       const float4 v = *reinterpret_cast<const float4*>(p.product + slot * c.dim + d);
       // nothing was written for an entry that is no page; a NaN maximum (of no score that is a number) is not -inf
       const bool there = s.x != -INFINITY || s.y != 0.f;
-      const float weight = there ? exp2f(s.x - base) : 0.f;
-      sum += there ? s.y * weight : 0.f;
+      const float weight = there ? exp2f(s.x - base) * unit : 0.f;
+      sum += there ? (Half2<T>::kOverflows ? fabsf(s.y) : s.y) * weight : 0.f;
       o[0] += there ? v.x * weight : 0.f;
       o[1] += there ? v.y * weight : 0.f;
       o[2] += there ? v.z * weight : 0.f;
       o[3] += there ? v.w * weight : 0.f;
     }
-    const float factor = sum == 0.f ? 0.f : 1.f / sum;
+    const float factor = any_averaged ? 1.f : to_average<T>(sum);
+    if (any_averaged) join_averages<T>(p, first, g, group, d, base, unit, sum, o);
     T* const to = static_cast<T*>(c.out) + (static_cast<long long>(row) * c.heads + kv * group + g) * c.dim + d;
     *reinterpret_cast<uint2*>(to) = make_uint2(Half2<T>::pack(o[0] * factor, o[1] * factor), Half2<T>::pack(o[2] * factor, o[3] * factor));
   }

@@ -116,6 +116,76 @@ def test_infinite_values_among_many_rows(dtype):
     assert ((got - ref).abs() <= bound)[keep].all()
 
 
+def with_large_values(v, seed=0):
+    """v with values whose sums leave fp32 and whose averages do not: of 8 elements of a head two all positive, two of both signs, two
+    as they were, two small ones.  What nobody holds stays NaN."""
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    large = v.clone()
+    size = (torch.rand(v.shape, generator=gen, device=DEV) * 0.8 + 2.5) * 1e38
+    sign = torch.where(torch.rand(v.shape, generator=gen, device=DEV) < 0.5, -1.0, 1.0)
+    large[..., 0::8] = size[..., 0::8].to(v.dtype)
+    large[..., 1::8] = (size * sign)[..., 1::8].to(v.dtype)
+    large[..., 4::8] = size[..., 4::8].to(v.dtype)
+    large[..., 5::8] = (size * sign)[..., 5::8].to(v.dtype)
+    large[..., 3::8] *= 1e-36
+    large[..., 7::8] *= 1e-37
+    return torch.where(torch.isnan(v), v, large)
+
+
+def check_large(got, q, k, v, table, lengths, pages=None):
+    """Infinite and NaN elements as the definition has them, finite ones within its bound."""
+    ref, bound = U.attention(q, k, v, table, lengths, pages)
+    got = got.cpu().double()
+    plain = torch.isfinite(ref)
+    assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(torch.isinf(got), torch.isinf(ref))
+    assert torch.equal(got[torch.isinf(ref)], ref[torch.isinf(ref)])
+    tiny = torch.finfo(BF16).smallest_normal * torch.finfo(BF16).eps
+    bound = bound + U.unit(BF16) * (ref.abs() + bound) + tiny
+    assert ((got - ref).abs() <= bound)[plain].all()
+    return plain
+
+
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim,page", [
+    ([700, 0, 90], 4, 2, 64, 32),          # clusters of several blocks
+    ([40, 17, 300] * 20, 8, 2, 128, 16),   # of one block
+    ([300, 16] * 40, 8, 8, 64, 32),        # shares of warps
+    ([3000, 200, 5] * 12, 24, 2, 128, 64),  # segments of several blocks, 16 query heads each
+    ([20000] * 20, 8, 8, 128, 256),
+    ([6000, 4000], 1, 1, 72, 16),
+])
+def test_values_whose_sums_leave_the_range_of_32_bits(lengths, heads, kv_heads, dim, page):
+    """bfloat16 reaches as far as fp32: an average of its largest values is a number, their sum is not."""
+    q, k, v, table, held = case(lengths, heads, kv_heads, dim, page, BF16)
+    v = with_large_values(v)
+    got = paged.paged_attention(q, k, v, table, held)
+    assert check_large(got, q, k, v, table, lengths).all()
+    # with infinite and NaN elements among them
+    row = 0
+    def put(head, position, element, value):
+        v[int(table[row, position // page]), head, position % page, element] = value
+    put(0, 5, 0, float("inf"))
+    put(0, 7, 1, float("nan"))
+    put(0, lengths[0] - 1, 2, float("-inf"))
+    put(0, 11, 4, float("inf"))
+    put(0, 12, 4, float("-inf"))
+    plain = check_large(paged.paged_attention(q, k, v, table, held), q, k, v, table, lengths)
+    assert int((~plain).sum()) == 4 * (heads // kv_heads)
+
+
+def test_shared_pages_with_values_whose_sums_leave_the_range_of_32_bits():
+    for args in ((128, 16, 4, 128, 64, 40 * 64 - 5, 8), (300, 16, 2, 104, 256, 12 * 256 - 200, 5)):
+        q, k, v, table, lengths, lists = shared_case(*args, BF16, seed=4)
+        assert takes_shared_pages(q, k, table, lists)
+        v = with_large_values(v)
+        got = paged.paged_attention(q, k, v, table, ints(lengths), pages=lists.to(DEV))
+        assert check_large(got, q, k, v, table, lengths, lists).all()
+        page = k.size(2)
+        v[int(table[0, 1]), 0, 5, 0] = float("inf")
+        v[int(table[0, 1]), 1, page - 1, 1] = float("nan")
+        plain = check_large(paged.paged_attention(q, k, v, table, ints(lengths), pages=lists.to(DEV)), q, k, v, table, lengths, lists)
+        assert not plain.all()
+
+
 def test_scores_of_minus_infinity_weigh_nothing():
     q, k, v, table, held = case([150, 40], 2, 1, 64, 16, BF16)
     q.fill_(1.0)
