@@ -72,7 +72,9 @@ void check_q(const at::Tensor& q, int64_t kv_heads, int64_t dim, int64_t page_si
   TORCH_CHECK(q.scalar_type() == type, "q and the cache must have one type");
   TORCH_CHECK(q.dim() == 3 && q.size(2) == dim, "q must be [rows, heads, head_dim], with the cache's head_dim");
   TORCH_CHECK(kv_heads > 0 && q.size(1) > 0 && q.size(1) % kv_heads == 0, "heads must be a multiple of kv_heads");
-  TORCH_CHECK(iex_paged_attention_supported(q.size(1), kv_heads, dim, page_size),
+  // no other sizes by their lower 32 bits
+  TORCH_CHECK(page_size > 0 && std::max({q.size(1), dim, page_size}) <= kMostInt &&
+                  iex_paged_attention_supported(q.size(1), kv_heads, dim, page_size),
               "head_dim must be a multiple of 8 up to 128 and page_size 16, 32, 64, 128 or 256; got ", dim, " and ", page_size);
   TORCH_CHECK(q.size(0) * q.size(1) <= kMostInt, "q has too many rows");
 }

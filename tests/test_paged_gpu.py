@@ -718,6 +718,19 @@ def test_selection_is_bounded_and_refuses():
     refused(held=held[:1])
 
 
+def test_sizes_are_not_read_by_their_lower_32_bits():
+    q, k, v, table, held = case([500, 200], 4, 2, 64, 16, F16)
+    boxes = U.boxes_of(k, table, [500, 200], 16)
+    for page in (2 ** 32 + 16, -2 ** 32 + 16, 2 ** 31 + 16):
+        with pytest.raises(RuntimeError):
+            paged.paged_select(q, boxes, table, held, page, 8)
+    none = k.new_zeros(1).expand(0, 1, 2 ** 32 + 16, 64)  # a cache without pages, and q without rows
+    with pytest.raises(RuntimeError):
+        paged.paged_attention(q[:0], none, none, table[:0], held[:0])
+    with pytest.raises(RuntimeError):
+        paged.paged_attention(q.new_zeros(1).expand(0, 2 ** 32 + 2, 64), k, v, table[:0], held[:0])
+
+
 # ------------------------------------------------------------------------------------------------- appending
 
 APPENDS = [
