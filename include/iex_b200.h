@@ -528,9 +528,11 @@ IEX_API void* iex_graph_combine(void* const* graphs, int count);
  *   head_dim           a multiple of 8 up to 128; page_size 16, 32, 64, 128 or 256
  * Rows of q, k and v are x_row, their heads x_head elements apart (multiples of 8, base
  * addresses on 16 bytes), elements of a head contiguous; other outputs are contiguous.
- * Lengths and tables come from the device and are bounded there: a length is read as one
- * between 0 and table_width * page_size, positions on a page outside [0, num_pages) as not
- * held.  Nothing behind a row's length is read, whatever its bits.
+ * Lengths and tables come from the device and are bounded there: attention and selection read
+ * a length as one between 0 and table_width * page_size (appending drops tokens behind the
+ * table), positions on a page outside [0, num_pages) as not held.  No key, value or box behind a
+ * row's length is used, whatever its bits; entries of the row of the table behind it may be
+ * loaded, and are not used.
  * ------------------------------------------------------------------------------------ */
 
 /* Appends: sequence i has cu_tokens[i + 1] - cu_tokens[i] new tokens (int32, ascending from
@@ -577,10 +579,11 @@ IEX_API int iex_paged_attention(int rows, int heads, int kv_heads, int head_dim,
                                 void* workspace, size_t workspace_bytes, void* stream);
 
 /* pages [rows, kv_heads, count]: the pages of each row and key head with the largest
- * sum over its query heads of sum_d max(q[d] lo[d], q[d] hi[d]), lo and hi from boxes, the
- * `first` first and `last` last held pages always among them (first + last <= count); in
- * ascending order, -1 behind them.  Ties go to the lower page, NaN is above all, pages not of the cache
- * come last.  At most iex_paged_select_max_pages() columns of the table. */
+ * sum over its query heads of sum_d max(q[d], 0) hi[d] + min(q[d], 0) lo[d], lo and hi from
+ * boxes, the `first` first and `last` last held pages always among them (first + last <=
+ * count); in ascending order, -1 behind them.  Ties go to the lower page, NaN is above all, pages
+ * not of the cache come last.  A factor of 0 counts: an infinite lo[d] or hi[d] that no query
+ * head of the key head has a factor for makes NaN.  Scores are as in 64 bits.  At most iex_paged_select_max_pages() columns of the table. */
 IEX_API int iex_paged_select_max_pages(void);
 IEX_API int iex_paged_select(int rows, int heads, int kv_heads, int head_dim, int bf16,
                              const void* q, long long q_row, long long q_head, const void* boxes,

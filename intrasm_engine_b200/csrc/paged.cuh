@@ -2,8 +2,9 @@
 //
 // The cache: keys and values [pages, kv_heads, page_size, head_dim], one contiguous slab per page and head, pages at any
 // distance.  Row r of the block table names the pages of a sequence in order, lengths[r] says how many positions it holds.
-// Both come from the device and are not trusted: a length is read as one between 0 and what the row of the table can hold, and
-// positions of a page that is not one of the cache's are as if they were not held.
+// Both come from the device and are not trusted: attention and selection read a length as one between 0 and what the row of the table
+// can hold (held()), appending drops tokens behind the table, and positions of a page that is not one of the cache's are as if they
+// were not held.
 #pragma once
 #include <cuda_bf16.h>
 

@@ -4,7 +4,8 @@
 //
 //   sum_g sum_d max(q[g, d] lo[d], q[g, d] hi[d]) = sum_d hi[d] sum_g max(q[g, d], 0) + lo[d] sum_g min(q[g, d], 0):
 //
-// two products a dimension however many query heads there are.  The `first` first and `last` last pages are always taken, then
+// two products a dimension however many query heads there are.  (Where lo or hi is infinite and its factor 0 the right side, which is
+// what the score is, is NaN.)  The `first` first and `last` last pages are always taken, then
 // those with the largest scores (NaN above all, ties to the lower page).
 //
 // Which of two pages is taken depends on their scores' difference, so what counts is scores in 64 bits, whose terms are added in one order

@@ -15,7 +15,7 @@ or, reading ``count`` pages of each sequence only, chosen for every row and key 
 ``k_cache`` and ``v_cache`` are ``[pages, kv_heads, page_size, head_dim]``, float16 or bfloat16, ``page_size`` 16, 32, 64, 128 or
 256, ``head_dim`` a multiple of 8 up to 128; each page is contiguous, pages may lie at any distance (``cache[:, 0]`` and
 ``cache[:, 1]`` of one ``[pages, 2, ...]`` tensor will do).  ``block_table`` int32 ``[rows, width]`` names each sequence's pages in order (what lies
-behind the pages it needs is not read), ``lengths`` int32 ``[rows]`` how many positions it holds, new tokens included; a row of
+behind the pages it needs may be anything), ``lengths`` int32 ``[rows]`` how many positions it holds, new tokens included; a row of
 length 0 is idle.  Heads are grouped: query heads ``h * heads / kv_heads`` and the following read key head ``h``.
 
 The operators run on the current stream, read nothing back and can be captured into a CUDA graph.  They have no backward
@@ -80,7 +80,8 @@ def paged_select(q, boxes, block_table, lengths, page_size: int, count: int, fir
 
     The ``first`` first and ``last`` last pages held are always taken, the others by the most that a key inside a page's box could give,
     ``sum_d hi_d max(q_d, 0) + lo_d min(q_d, 0)`` summed over the query heads of the key head, in 64 bits; NaN counts as the
-    largest, ties go to the lower page.  A row that holds no more than ``count`` pages takes all of them."""
+    largest, ties go to the lower page.  An infinite ``lo_d`` or ``hi_d`` with a factor of 0 makes NaN, so that a page with a key that
+    overflowed is taken.  A row that holds no more than ``count`` pages takes all of them."""
     out = ops.native.paged_select(q, boxes, block_table, lengths, page_size, count, first, last)
     if out is None:
         out = torch.ops.iex_ops.paged_select(q, boxes, block_table, lengths, page_size, count, first, last)

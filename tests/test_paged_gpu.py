@@ -664,6 +664,20 @@ def test_selection_with_more_infinite_scores_than_are_wanted(dim, rows, value):
         assert torch.equal(got[some].cpu(), U.select(q[some], boxes, table[some], [lengths[i] for i in some], 16, count, first, 0)), count
 
 
+def test_selection_takes_a_page_with_a_key_that_overflowed():
+    """An infinite element of a box makes NaN where no query head has a factor for it, and an infinite score where one has."""
+    q, k, v, table, held = case([1600], 2, 1, 64, 16, F16)
+    boxes = U.boxes_of(k, table, [1600], 16)
+    q[...] = q.abs()            # of lo no element has a factor
+    q[0, :, 5] = torch.tensor([1.0, -1.0], device=DEV).half()
+    lower, upper = int(table[0, 37]), int(table[0, 61])
+    boxes[lower, 0, 0, 9] = float("-inf")
+    boxes[upper, 0, 0, 5] = float("-inf")
+    for count, expected in ((1, [37]), (2, [37, 61])):
+        assert paged.paged_select(q, boxes, table, held, 16, count, 0, 0)[0, 0].tolist() == expected
+        assert U.select(q, boxes, table, [1600], 16, count, 0, 0)[0, 0].tolist() == expected
+
+
 def test_selection_by_queries_that_are_not_finite():
     lengths = [1600] * 4
     q, k, v, table, held = case(lengths, 4, 2, 64, 16, F16)
