@@ -136,3 +136,18 @@ def test_entry_points_check_their_arguments():
         assert append(**kwargs) == unsupported, kwargs
     for width, page in ((2 ** 23, 256), (2 ** 27, 16), (2 ** 31 - 1, 256)):
         assert append(width=width, page=page) == too_large
+
+
+# of the cases of test_paged_gpu.SHARED, in order: whether pages are read once for many rows
+SHARED_PATHS = [True, True, True, True, True, False, False, True, False, True]
+
+
+def test_cases_of_shared_pages_take_the_path_that_they_stand_for():
+    from .test_paged_gpu import SHARED
+    assert len(SHARED) == len(SHARED_PATHS)
+    for (rows, heads, kv_heads, dim, page, longest, count), shared in zip(SHARED, SHARED_PATHS):
+        width = (longest + page - 1) // page
+        def need(pages):
+            return _lib.lib.iex_paged_attention_workspace_bytes(rows, heads, kv_heads, dim, pages, page, width, 1, count)
+        # of a cache with more pages than are ever sorted, rows read their pages one by one
+        assert (need(width + 2) != need(1 << 20)) == shared, (rows, heads, kv_heads, dim, page, longest, count)

@@ -435,6 +435,58 @@ def test_shared_pages_in_graphs_and_whatever_scratch_memory_held():
         assert all(torch.equal(o, expected[i]) for o in outs[i])
 
 
+def check_listed(got, q, k, v, table, lengths, lists):
+    """As U.check_attention, for many rows: in 64 bits on the GPU, some rows at a time."""
+    (rows, heads, dim), kv_heads, page = q.shape, k.size(1), k.size(2)
+    group, width, slots = heads // kv_heads, table.size(1), torch.arange(k.size(2), device=DEV)
+    count, heads_of = lists.size(2), torch.arange(kv_heads, device=DEV)[:, None]
+    for at in range(0, rows, 64):
+        some = slice(at, min(at + 64, rows))
+        held = lengths[some].long().clamp(0, width * page)[:, None, None]
+        pages, nth = (held + page - 1) // page, lists[some].long()
+        real = (torch.arange(count, device=DEV) < pages) & (nth >= 0) & (nth < pages)
+        nth = torch.where(real, nth, 0)
+        where = table[some].long()[:, None].expand(-1, kv_heads, -1).gather(2, nth)
+        real &= (where >= 0) & (where < k.size(0))
+        where = torch.where(real, where, 0)
+        seen = (real[..., None] & (nth[..., None] * page + slots < held[..., None])).flatten(2)  # [rows, kv_heads, positions]
+        keys, values = (t[where, heads_of].flatten(2, 3).double().masked_fill(~seen[..., None], 0) for t in (k, v))
+        mine = q[some].double().view(-1, kv_heads, group, dim)
+        scores = torch.einsum("rhgd,rhsd->rhgs", mine, keys) * dim ** -0.5
+        weights = torch.softmax(scores.masked_fill(~seen[:, :, None], -1e30), -1) * seen[:, :, None]
+        ref = torch.einsum("rhgs,rhsd->rhgd", weights, values)
+        size = torch.einsum("rhgd,rhsd->rhgs", mine.abs(), keys.abs()) * dim ** -0.5
+        loss = weights * torch.expm1((2 * (dim + 3) * 2.0 ** -23 * size).clamp(max=30))
+        bound = (torch.einsum("rhgs,rhsd->rhgd", loss, values.abs()) + loss.sum(-1, keepdim=True) * ref.abs()
+                 + (2.0 ** -16 + count * page * 2.0 ** -23) * torch.einsum("rhgs,rhsd->rhgd", weights, values.abs()))
+        bound = bound + U.unit(got.dtype) * (ref.abs() + bound) + torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps
+        assert ((got[some].double().view_as(ref) - ref).abs() <= bound).all(), at
+
+
+@pytest.mark.parametrize("dtype", U.DTYPES)
+@pytest.mark.parametrize("rows,heads,kv_heads,dim,page,total,width,count", [
+    (4096, 1, 1, 128, 128, 4000, 32, 16),    # counters of more than 40 KB; more entries than a block takes in one turn
+    (4096, 2, 1, 16, 256, 16384, 24, 16),    # the largest cache that is sorted
+    (3000, 3, 3, 64, 128, 1100, 40, 24),     # two pages to a thread
+    (1500, 6, 6, 40, 128, 2000, 33, 30),
+])
+def test_shared_pages_of_large_caches(rows, heads, kv_heads, dim, page, total, width, count, dtype):
+    gen = torch.Generator(device=DEV).manual_seed(total)
+    k, v = (torch.randn(total, kv_heads, page, dim, device=DEV, generator=gen).to(dtype) for _ in range(2))
+    q = torch.randn(rows, heads, dim, device=DEV, generator=gen).to(dtype)
+    table = torch.randint(0, total, (rows, width), device=DEV, generator=gen, dtype=torch.int32)
+    lengths = torch.randint(0, width * page + 1, (rows,), device=DEV, generator=gen, dtype=torch.int32)
+    lengths[:4] = ints([width * page, 0, 1, 2 ** 31 - 1])
+    lists = torch.rand(rows, kv_heads, width, device=DEV, generator=gen).argsort(-1)[..., :count].int().contiguous()
+    lists[5, :, 1], lists[6, 0, 0], lists[7] = lists[5, :, 0], -7, 2 ** 31 - 1
+    table[8, ::2], table[9, ::3] = -1, total
+    table[-1] = total - 1  # the last page
+    assert takes_shared_pages(q, k, table, lists)
+    got = paged.paged_attention(q, k, v, table, lengths, pages=lists)
+    check_listed(got, q, k, v, table, lengths, lists)
+    assert not got[1].any() and not got[7].any()
+
+
 def test_attention_refuses_scales_that_are_not_finite_in_32_bits():
     q, k, v, table, held = case([50, 20], 4, 2, 64, 16, F16)
     for scale in (1e300, -1e39, float("nan")):
