@@ -34,6 +34,7 @@ constexpr int kTileRows = 64, kThreads = 128, kPositions = 64;
 constexpr int kMostPages = 16384, kPageBytes = 3 * sizeof(int);  // shared memory of each
 constexpr int kIndexBlocks = 8;    // of a cluster, at most
 constexpr int kMostGroup = 16;
+constexpr size_t kMostScratch = 512u << 20;  // of a call; entries are then fewer than 2^24
 
 struct Item {
   int page, begin, n, most;  // entries list[begin .. begin + n) of the head; positions of the page that any entry sees
@@ -479,7 +480,7 @@ size_t shared_workspace_bytes(int rows, int heads, int kv_heads, int head_dim, i
   const int group = heads / kv_heads;
   if (group > kMostGroup || num_pages <= 0 || num_pages > kMostPages || count <= 0 || count > table_width || kv_heads > 65535) return 0;
   const double entries = static_cast<double>(rows) * count;
-  if (entries > 1 << 18) return 0;  // one block sorts a head's
+  if (entries * heads * head_dim * sizeof(float) > kMostScratch) return 0;
   // us of the two ways; of 30 measurements (rows 32 .. 4096, 1 .. 16 query heads to a key head, pages of 16 .. 256) all but three
   // within a quarter.  Row by row: keys and values from L2.  Here: the sort, a product to and fro for every entry and query head,
   // and a block's work.
@@ -491,13 +492,15 @@ size_t shared_workspace_bytes(int rows, int heads, int kv_heads, int head_dim, i
   //   64,    8 x 4, 128,  64,  256, 16                     38        45
   //   1024,  2 x 8, 128,  64,  256, 16                    119       156
   //   256,   8 x 4, 128,  64, 4096, 16                    160       311
+  //   16384, 1 x 1,  64,  64, 1000, 60                   1656       548
+  //   20000, 1 x 1, 128,  64,  500, 33                   2105       491
   const int dim = head_dim > 64 ? 128 : 64, tiles = (page_size + kPositions - 1) / kPositions;
   const double pairs = entries * heads, blocks = kv_heads * (entries / (kTileRows / group) + 0.5 * std::min<double>(num_pages, entries));
   const double one_by_one = 12.0 + entries * kv_heads * 4 * page_size * dim * (group > 8 ? 1.25 : 1.0) / 9.7e6;
   const double shared = 15.0 + 6e-4 * entries + 1e-6 * pairs * head_dim + blocks * (6e-3 + 8.8e-5 * tiles * dim);
   if (one_by_one < 1.05 * shared) return 0;
   const Sizes s = sizes(rows, heads, kv_heads, head_dim, num_pages, count);
-  return s.all <= 512u << 20 ? s.all : 0;
+  return s.all <= kMostScratch ? s.all : 0;
 }
 
 int shared_attention(const SharedCall& call, bool bf16, void* workspace, cudaStream_t stream) {

@@ -142,6 +142,16 @@ def test_entry_points_check_their_arguments():
 SHARED_PATHS = [True, True, True, True, True, False, False, True, False, True]
 
 
+def test_scratch_of_shared_pages_is_bounded():
+    """By its size alone, whatever the number of entries; sizes whose products leave 64 bits take none."""
+    def need(rows, count, heads=1, dim=64, width=1 << 20):
+        return _lib.lib.iex_paged_attention_workspace_bytes(rows, heads, heads, dim, 900, 64, width, 1, count)
+    assert 60 << 20 < need(8192, 30) < 80 << 20 and 80 << 20 < need(8192, 40) < 100 << 20  # 2^18 entries are in between
+    assert 500 << 20 < need(1 << 15, 58) <= 512 << 20
+    for rows, count in ((1 << 15, 64), (1 << 20, 1 << 20), (2 ** 31 - 1, 1 << 20)):
+        assert need(rows, count) < 1 << 20
+
+
 def test_cases_of_shared_pages_take_the_path_that_they_stand_for():
     from .test_paged_gpu import SHARED
     assert len(SHARED) == len(SHARED_PATHS)

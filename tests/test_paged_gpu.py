@@ -469,6 +469,7 @@ def check_listed(got, q, k, v, table, lengths, lists):
     (4096, 2, 1, 16, 256, 16384, 24, 16),    # the largest cache that is sorted
     (3000, 3, 3, 64, 128, 1100, 40, 24),     # two pages to a thread
     (1500, 6, 6, 40, 128, 2000, 33, 30),
+    (8192, 1, 1, 64, 64, 900, 60, 40),       # more than 2^18 entries
 ])
 def test_shared_pages_of_large_caches(rows, heads, kv_heads, dim, page, total, width, count, dtype):
     gen = torch.Generator(device=DEV).manual_seed(total)
