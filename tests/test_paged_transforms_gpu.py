@@ -97,6 +97,17 @@ def test_dispatch_mode_sees_the_operators(call):
     assert torch.equal(graph(*[a.clone() for a in other]), f(*[a.clone() for a in other]))
 
 
+def test_vmap_gives_the_same_or_is_refused(call):
+    """Over queries: the operators that write nothing run one by one, appending is refused."""
+    f, args, names = call
+    both = torch.stack([args[0], -args[0]])
+    if "k" in names:
+        with pytest.raises(RuntimeError):
+            torch.vmap(lambda q: f(q, *args[1:]))(both)
+    else:
+        assert torch.equal(torch.vmap(lambda q: f(q, *args[1:]))(both), torch.stack([f(q, *args[1:]) for q in both]))
+
+
 def test_negative_view(call):
     """A query that only says it is negated."""
     f, args, _ = call
