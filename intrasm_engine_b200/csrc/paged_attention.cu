@@ -4,7 +4,7 @@
 //
 // with heads / kv_heads query heads to a key head, or over the positions of the pages that pages[r, kv_head] lists.  A segment is
 // what one row and one key head (up to 16 of its query heads) have to read, in chunks of 16 positions.  One to sixteen flops a byte: HBM bounds it.
-// 64 rows up to 4096, 32 query and 8 key heads of 128: 103 us, 6.3 TB/s; 2 rows of 131071: 147 us, 6.5 TB/s; 1 row of 500, 32 heads: 5.7 us.
+// 64 rows up to 4096, 32 query and 8 key heads of 128: 104 us, 6.2 TB/s; 2 rows of 131071: 147 us, 6.5 TB/s; 1 row of 500, 32 heads: 5.8 us.
 //
 // Work, where segments are many or uneven (attention_kernel): the chunks of all segments, in order, are shared out evenly to the
 // warps of one block per SM, whatever the rows' lengths, a segment's start counted as kStart chunks; a warp that has a whole segment
@@ -740,8 +740,9 @@ size_t product_bytes(int heads, int head_dim) {
 //
 // attention_kernel with join_kernel behind it takes 13 us before anything is read (how the work is shared out, joining twice), a
 // cluster 6; but it keeps all SMs busy until the end, where clusters leave some idle and last as long as the longest row.
-// Rows are taken to hold kFill of the most on average, with listed pages all.  Measured, attention_kernel / clusters, us: 1 row of 500, 32
-// heads 14.9 / 5.9; 4 rows up to 4096, 8 key heads 17.4 / 15.9; 16 rows of 32 listed pages of 64 29.0 / 27.7; 1 row of 16384, 8 key heads
+// Rows are taken to hold kFill of the most on average, with listed pages all: a short row in a wide table is taken for a long one (1 row of
+// 500, 32 heads: 5.8 us up to 85 columns of 64, 14.4 above).  Measured, attention_kernel / clusters, us: 1 row of 500, 32
+// heads 14.4 / 5.8; 4 rows up to 4096, 8 key heads 17.4 / 15.9; 16 rows of 32 listed pages of 64 29.0 / 27.7; 1 row of 16384, 8 key heads
 // 20.1 / 26.2; 32 rows up to 8192, one key head 27.2 / 33.0.
 int cluster_blocks(long long segments, long long most_chunks, int head_dim, bool listed) {
   constexpr double kSaved = 7.0, kFill = 0.65, kRate = 6.5e6;  // us, -, bytes a us

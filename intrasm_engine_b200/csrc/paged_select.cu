@@ -19,8 +19,8 @@
 // a rule).  Up to 32 pages near the border are then compared with one another in 64 bits, more of them searched like all were.  So
 // many blocks that they fill the GPU, or one each where rows and key heads do.
 //
-// 1 row of 512 pages, 8 key heads of 128: 5.4 us, latency (lengths and queries, boxes, the cluster's barrier, the search); 16 rows:
-// 9.9 us (19 MB of boxes); 256 rows of 256 pages: 37 us, issue slots (70 %; 70 instructions a box and warp, half of them the search's) and 268 MB from L2.
+// 1 row of 512 pages, 8 key heads of 128: 6.1 us, latency (lengths and queries, boxes, the cluster's barrier, the search); 16 rows:
+// 10.2 us (19 MB of boxes); 256 rows of 256 pages: 37 us, issue slots (70 %; 70 instructions a box and warp, half of them the search's) and 268 MB from L2.
 #include <algorithm>
 
 #include <cooperative_groups.h>
@@ -226,7 +226,7 @@ __device__ __forceinline__ Border<K> find_border(const K* keys, int from, int to
 }
 
 // LANES: side by side on a box, 8 elements each.  THREADS, BLOCKS of an SM at once: 256, 2 where there are no more blocks (all of a
-// lane's boxes then find registers: 9.9 us for 16 rows x 8 key heads x 512 pages, with a third block 11.1); else 128, 6 (what every warp does
+// lane's boxes then find registers: 16 rows x 8 key heads x 512 pages take 11 % less than with a third block); else 128, 6 (what every warp does
 // for itself counts there: 256 rows x 8 key heads x 256 pages 37 us, with 256, 3 44), or 256, 3 where the scores' shared memory leaves no
 // room for 6 (the same with 4096 pages: 453 us, with 128 threads 562, with 256, 2 498).
 template <typename T, int LANES, int THREADS, int BLOCKS>

@@ -5,7 +5,7 @@
 // Here a page is read once for up to 64 of the (entry, query head) pairs that list it: index_kernel sorts the entries of the lists
 // by page, page_kernel forms the softmax and the product of such a tile with its page, join_entries_kernel adds up each row's
 // entries in the order of its list.  What is written and read between them, a product of fp32 for every entry and query head, is
-// 2 G / page of the keys and values that would be read (G query heads to a key head).  85 us at the same sizes: 11 us of sorting
+// 2 G / page of the keys and values that would be read (G query heads to a key head).  83 us at the same sizes: 11 us of sorting
 // (latency), 63 us of page_kernel (378 MB through L2, 6 TB/s), 18 us of joining (108 MB, 6 TB/s), with their launches overlapped; 96
 // us instead of 420 where each of 32 key heads has its own query head.
 //
