@@ -18,7 +18,7 @@ namespace {
 constexpr int64_t kMostInt = std::numeric_limits<int>::max();
 
 // Without a derivative an output that has none of its own would say that it is zero.
-void check_not_differentiated(const std::string& name, const at::Tensor& t) {
+void check_not_differentiated(const char* name, const at::Tensor& t) {
   TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), name,
               " requires a gradient: the operators of the paged cache have no backward pass");
   TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), name,
@@ -100,7 +100,7 @@ void refuse_derivatives(const c10::OperatorHandle& op, c10::DispatchKeySet keys,
   const auto operands = torch::jit::last(stack, arguments.size());
   for (size_t i = 0; i < arguments.size(); ++i)
     if (operands[i].isTensor() && operands[i].toTensor().defined())
-      check_not_differentiated(arguments[i].name(), operands[i].toTensor());
+      check_not_differentiated(arguments[i].name().c_str(), operands[i].toTensor());
   at::AutoDispatchBelowAutograd below;
   op.redispatchBoxed(keys & c10::after_autograd_keyset, stack);
 }
